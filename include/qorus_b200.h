@@ -206,6 +206,183 @@ q_error_code q_b200_gemm_q4(const void* d_packed, uint32_t M, uint32_t K, const 
 q_error_code q_b200_gemv_f32(const float* d_w, uint32_t M, uint32_t K,
                              const float* d_x, float* d_y, void* stream);
 
+/* ---- serving operators on device buffers ---------------------------------
+ * One step of a batch that decodes drafted tokens behind a shared prompt:
+ * rotate (q_b200_rope), store keys and values in pages (q_b200_kv_append),
+ * attend over the shared prompt's pages and each sequence's own
+ * (q_b200_attn_prefix), accept or replace the drafts (q_b200_verify_draft).
+ * They stand beside upstream's q_rope_f32_avx2 (qorus.h:153), its KV store
+ * and attention (src/models/model.c:1088-1652) and q_sample_token
+ * (src/main.c:852-991), which work on one sequence from host buffers.
+ *
+ * Every pointer in the argument records is a device pointer of the current
+ * device unless it is a plan (host); a pointer that is not is refused with
+ * Q_ERR_INVALID_ARG.  Strides count elements.  Calls are asynchronous on
+ * `stream`, allocate nothing, keep no state between calls and may be
+ * captured in a CUDA graph; calls on different streams may overlap as long
+ * as they share no output or workspace.  What the device alone can see to be
+ * wrong (a page, sequence or token out of range, a length above its bound)
+ * is skipped and leaves code 4 in the status word (q_b200_device_status):
+ * nothing out of range is touched, results that hang on it are unspecified. */
+
+typedef enum { Q_B200_F32 = 0, Q_B200_F16 = 1, Q_B200_BF16 = 2 } q_b200_dtype;
+
+/* One layer of a paged cache: row r of KV head h in page p begins at
+ * k (or v) + p * page_stride + h * head_stride + r * row_stride.  The pool
+ * of q_b200_batch_init_paged is one (q_b200_batch_kv_view fills this in). */
+typedef struct {
+    void* k;
+    void* v;
+    uint64_t page_stride, head_stride, row_stride;
+    uint32_t n_pages, page_rows, n_kv_heads, head_dim;
+    uint32_t dtype;    /* q_b200_dtype */
+    uint32_t reserved; /* 0 */
+} q_b200_paged_kv;
+
+/* Pairs that rotate together: (2i, 2i+1), or (i, i + rot_dim/2). */
+typedef enum { Q_B200_ROPE_INTERLEAVED = 0, Q_B200_ROPE_HALF = 1 } q_b200_rope_layout;
+
+/* How the frequencies f_i = base^(-2i/rot_dim) are scaled for contexts
+ * longer than original_len, by `factor`:
+ *   LINEAR  f / factor
+ *   BANDED  waves longer than original_len/low are slowed by factor, those
+ *           shorter than original_len/high kept, linear in original_len/wave
+ *           between
+ *   YARN    the same by pair index: pairs that turn more than `high` times
+ *           in original_len are kept, those that turn less than `low` times
+ *           slowed, linear in the index between; cosine and sine are
+ *           multiplied by gain (0: 0.1 ln(factor) + 1) */
+typedef enum {
+    Q_B200_ROPE_PLAIN = 0,
+    Q_B200_ROPE_LINEAR = 1,
+    Q_B200_ROPE_BANDED = 2,
+    Q_B200_ROPE_YARN = 3
+} q_b200_rope_scaling;
+
+typedef struct {
+    uint32_t kind;     /* q_b200_rope_scaling */
+    uint32_t reserved; /* 0 */
+    double factor, low, high, original_len;
+    double gain; /* YARN only; 0: derived from factor */
+} q_b200_rope_scale;
+
+/* Filled by q_b200_rope_plan_init, kept by the caller on the host. */
+typedef struct {
+    uint32_t rot_dim, layout;
+    float gain;
+    uint32_t reserved;
+    double turns[128]; /* turns per position of each pair, f / 2 pi */
+} q_b200_rope_plan;
+
+/* rot_dim even, 2..256; scale NULL = plain. */
+q_error_code q_b200_rope_plan_init(q_b200_rope_plan* plan, uint32_t rot_dim, q_b200_rope_layout layout,
+                                   double base, const q_b200_rope_scale* scale);
+
+/* out[t][h] = x[t][h] rotated by position pos[t] (any int32: a negative one
+ * turns back), elements rot_dim..head_dim-1 copied.  transpose != 0 applies
+ * the transposed rotation (the way back up to gain^2, and the gradient).
+ * out may be x with x's strides.  The angle is formed in 64 bits and the
+ * pair rotated in fp32, rounded once to dtype. */
+typedef struct {
+    const void* x;
+    void* out;
+    const int32_t* pos; /* [n_tokens] */
+    const q_b200_rope_plan* plan;
+    uint64_t x_token_stride, x_head_stride, out_token_stride, out_head_stride;
+    uint32_t n_tokens, n_heads, head_dim; /* head_dim <= 256 */
+    uint32_t dtype;                       /* of x and out */
+    uint32_t transpose;
+    uint32_t reserved; /* 0 */
+} q_b200_rope_args;
+q_error_code q_b200_rope(const q_b200_rope_args* args, void* stream);
+
+/* Token t's keys (rotated by pos[t]) and values go to row row[t] of sequence
+ * seq[t]'s pages; with q its queries are rotated into q_out beside them.  A
+ * token with a negative row is padding: nothing of it is read or written.
+ * Two tokens must not name the same row of the same page. */
+typedef struct {
+    q_b200_paged_kv kv;
+    const void* k; /* [n_tokens][n_kv_heads][head_dim] */
+    const void* v;
+    const void* q; /* [n_tokens][n_heads][head_dim]; NULL: none */
+    void* q_out;
+    uint64_t k_token_stride, k_head_stride, v_token_stride, v_head_stride;
+    uint64_t q_token_stride, q_head_stride, q_out_token_stride, q_out_head_stride;
+    const uint32_t* pages; /* [n_seqs][pages_per_seq] */
+    const uint32_t* seq;   /* [n_tokens]; NULL: token t is sequence t's */
+    const int32_t* row;    /* [n_tokens] */
+    const int32_t* pos;    /* [n_tokens]; NULL: row */
+    const q_b200_rope_plan* plan; /* NULL: nothing rotates */
+    uint32_t n_tokens, n_seqs, pages_per_seq, n_heads;
+    uint32_t dtype;    /* of k, v, q, q_out; the cache has its own */
+    uint32_t reserved; /* 0 */
+} q_b200_append_args;
+q_error_code q_b200_kv_append(const q_b200_append_args* args, void* stream);
+
+/* Attention of new tokens over a prefix that all sequences share (its rows
+ * in prefix_pages, read once for all of them where that pays) and over each
+ * sequence's own rows (0..lens[b]-1 in pages[b], its new tokens' rows last
+ * among them).  The i-th of sequence b's n new tokens sees the whole prefix
+ * and its own rows 0..lens[b]-n+i; head h reads KV head
+ * h / (n_heads / n_kv_heads).  A token that sees no row gives zeros.  q and
+ * out have the cache's dtype; scores, softmax and sums are fp32.  Tokens of
+ * no sequence (from q_start[n_seqs] on) are left as they are in out.
+ * head_dim 32, 64 or 128. */
+typedef struct {
+    q_b200_paged_kv kv;
+    const void* q; /* [n_tokens][n_heads][head_dim] */
+    void* out;
+    uint64_t q_token_stride, q_head_stride, out_token_stride, out_head_stride;
+    const uint32_t* q_start;      /* [n_seqs + 1] first token of each; NULL: one token each */
+    const uint32_t* pages;        /* [n_seqs][pages_per_seq] */
+    const uint32_t* lens;         /* [n_seqs] own rows, at most max_len */
+    const uint32_t* prefix_pages; /* NULL: no prefix */
+    const uint32_t* prefix_len;   /* one number, at most max_prefix */
+    void* work; /* q_b200_attn_work_bytes(args) bytes, 16-byte aligned */
+    uint64_t work_bytes;
+    uint32_t n_tokens, n_seqs, n_heads, pages_per_seq;
+    uint32_t max_q;               /* most new tokens of one sequence */
+    uint32_t max_len, max_prefix; /* bounds that the work is split by */
+    float scale;                  /* on q.k, usually 1/sqrt(head_dim) */
+} q_b200_attn_args;
+/* Bytes that q_b200_attn_prefix needs in work (0: none, or args refused);
+ * the pointers in args are not looked at. */
+size_t q_b200_attn_work_bytes(const q_b200_attn_args* args);
+q_error_code q_b200_attn_prefix(const q_b200_attn_args* args, void* stream);
+
+/* Speculative decoding's test.  Draft i of sequence b, token x, is accepted
+ * while uniform[b][i] * q_i(x) < p_i(x); at the first that is not, the next
+ * token is drawn from max(p_i - q_i, 0), and after the last accepted draft
+ * from the target's own row, by the smallest index whose running sum
+ * exceeds uniform[b][n_draft] times the whole (sums in 64 bits).  p and q
+ * are rows of probabilities (PROBS; they need not sum to one) or the softmax
+ * of logits / temperature (LOGITS; below 1e-6 the test is whether the draft
+ * is the first maximum of the target, and q is not used).  draft NULL: q is
+ * one at the drafted token.  NaN and negative weights count as zero; where
+ * the difference has no weight the row p is used, and a row without weight
+ * gives token 0. */
+typedef enum { Q_B200_PROBS = 0, Q_B200_LOGITS = 1 } q_b200_verify_kind;
+typedef struct {
+    const void* target; /* [n_seqs][n_draft + 1][vocab] */
+    const void* draft;  /* [n_seqs][n_draft][vocab]; may be NULL */
+    uint64_t target_seq_stride, target_row_stride, draft_seq_stride, draft_row_stride;
+    const uint32_t* draft_tokens; /* [n_seqs][n_draft] */
+    const uint32_t* draft_len;    /* [n_seqs] drafts of each; NULL: n_draft */
+    const float* uniform;         /* [n_seqs][n_draft + 1] in [0, 1) */
+    uint32_t* tokens;             /* [n_seqs][n_draft + 1]: accepted, the drawn one, then UINT32_MAX */
+    uint32_t* n_tokens;           /* [n_seqs] accepted + 1 */
+    uint32_t n_seqs, n_draft, vocab; /* n_draft 0..31 */
+    uint32_t dtype, kind;
+    float temperature; /* LOGITS only */
+} q_b200_verify_args;
+q_error_code q_b200_verify_draft(const q_b200_verify_args* args, void* stream);
+
+/* The paged caches of a batched context as one layer's q_b200_paged_kv, with
+ * the device page table (the caches' own, current after the last call that
+ * took or wrote rows). */
+q_error_code q_b200_batch_kv_view(q_context* ctx, uint32_t layer, q_b200_paged_kv* kv, const uint32_t** pages,
+                                  uint32_t* pages_per_seq);
+
 /* ---- device errors and bounded waits -------------------------------------
  * No counterpart upstream (upstream's kernels run on the calling thread and
  * cannot hang).  Every device-side wait of this library (a copy that should
@@ -223,8 +400,8 @@ q_error_code q_b200_gemv_f32(const float* d_w, uint32_t M, uint32_t K,
 q_error_code q_b200_set_wait_limit_ns(uint64_t ns);
 
 /* Status word of the current device: 0 if no wait ran out since the last
- * read, else the code of the first one (1-3 copy waits, 5 grid barrier,
- * 6 peer flag).  Reading clears it; when it was set, this first waits for
+ * read, else the code of the first one (1-3 copy waits, 4 an index or
+ * length that a serving operator skipped, 5 grid barrier, 6 peer flag).  Reading clears it; when it was set, this first waits for
  * all work on the device and re-zeroes the library's ticket and barrier
  * counters, which a wait that gave up can leave non-zero. */
 uint32_t q_b200_device_status(void);

@@ -1,0 +1,571 @@
+// api_serve.cu — the serving operators' entry points: argument checks, plans
+// and launches (kernels: rotate.cuh, attn_prefix.cuh, verify.cuh).
+//
+// Nothing is allocated and nothing is kept between calls; checks that need
+// no device come first, so that a refusal is the same with and without one.
+#include <cmath>
+
+#include "attn_prefix.cuh"
+#include "runtime.cuh"
+#include "verify.cuh"
+
+using namespace qb200;
+
+namespace {
+
+uint32_t size_of(uint32_t dtype) { return dtype == Q_B200_F32 ? 4u : 2u; }
+bool known(uint32_t dtype) { return dtype <= Q_B200_BF16; }
+
+// Device memory (or managed memory) of the current device: a host pointer or
+// another GPU's would fault in the kernel.
+struct DevicePtrs {
+    int dev = -1;
+    bool ok = true;
+    DevicePtrs() { ok = cuda_ok(cudaGetDevice(&dev), "cudaGetDevice"); }
+    DevicePtrs& operator()(const void* p) {
+        if (!ok || !p) return *this;
+        cudaPointerAttributes at;
+        ok = cuda_ok(cudaPointerGetAttributes(&at, p), "cudaPointerGetAttributes");
+        if (ok && !(at.type == cudaMemoryTypeManaged || (at.type == cudaMemoryTypeDevice && at.device == dev))) {
+            set_last_error("a pointer is not of the current device", cudaErrorInvalidValue);
+            ok = false;
+        }
+        return *this;
+    }
+};
+
+FastDiv fast_div_of(uint32_t d) {
+    uint32_t s = 0;
+    while ((1ull << s) < d) ++s;
+    return {d, (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
+}
+
+uint64_t align_of(std::initializer_list<uint64_t> v) {  // largest power of two that divides all
+    uint64_t all = 0;
+    for (uint64_t x : v) all |= x;
+    return all ? (all & (~all + 1)) : ~0ull;
+}
+uint64_t addr(const void* p) { return (uint64_t)(uintptr_t)p; }
+
+q_error_code check_cache(const q_b200_paged_kv& kv) {
+    if (!kv.k || !kv.v) return Q_ERR_INVALID_ARG;
+    if (!known(kv.dtype)) return Q_ERR_INVALID_DTYPE;
+    if (kv.reserved) return Q_ERR_INVALID_ARG;
+    if (kv.n_pages == 0 || kv.page_rows == 0 || kv.n_kv_heads == 0 || kv.head_dim == 0) return Q_ERR_INVALID_SIZE;
+    if (kv.page_rows > (1u << 30)) return Q_ERR_INVALID_SIZE;
+    if (kv.row_stride < kv.head_dim && kv.page_rows > 1) return Q_ERR_INVALID_SIZE;
+    if ((addr(kv.k) | addr(kv.v)) & (size_of(kv.dtype) - 1)) return Q_ERR_MISALIGNED;
+    return Q_OK;
+}
+
+q_error_code check_plan(const q_b200_rope_plan* p, uint32_t head_dim) {
+    if (p->rot_dim < 2 || p->rot_dim > 256 || p->rot_dim % 2 || p->rot_dim > head_dim) return Q_ERR_INVALID_SIZE;
+    if (p->layout > Q_B200_ROPE_HALF) return Q_ERR_INVALID_ARG;
+    return Q_OK;
+}
+
+// ---- rotation -------------------------------------------------------------------
+
+template <typename TI, typename TC>
+cudaError_t launch_rotate(RotateArgs& a, uint32_t E, uint32_t HB, cudaStream_t st) {
+    const uint32_t rot = a.rot;
+    a.rot_units = rot / (2 * E);
+    a.units = a.rot_units + (a.head_dim - rot) / E;
+    uint32_t chunks = 0;
+    for (RotateRows& p : a.part) {
+        p.chunks = (p.heads + HB - 1) / HB;
+        chunks += p.chunks;
+    }
+    if (chunks == 0) return cudaSuccess;
+    a.by_units = fast_div_of(a.units);
+    a.by_chunks = fast_div_of(chunks);
+    // the item index is 31 bits: longer inputs go in runs of tokens
+    const uint64_t per = (uint64_t)chunks * a.units;
+    const uint32_t run = (uint32_t)std::min<uint64_t>(a.n_tokens, (1ull << 30) / per + 1), all = a.n_tokens;
+    void (*kern)(const RotateArgs) = nullptr;
+    if (E == 8) kern = HB == 4 ? rotate_kernel<TI, TC, 8, 4> : rotate_kernel<TI, TC, 8, 1>;
+    else if (E == 4) kern = HB == 4 ? rotate_kernel<TI, TC, 4, 4> : rotate_kernel<TI, TC, 4, 1>;
+    else kern = HB == 4 ? rotate_kernel<TI, TC, 1, 4> : rotate_kernel<TI, TC, 1, 1>;
+    for (uint32_t t0 = 0; t0 < all; t0 += run) {
+        RotateArgs b = a;
+        b.n_tokens = std::min(run, all - t0);
+        b.n_items = per * b.n_tokens;
+        for (RotateRows& p : b.part) {
+            if (!p.heads) continue;
+            p.src = (const TI*)p.src + t0 * p.src_token;
+            if (!p.paged) p.dst = (TI*)p.dst + t0 * p.dst_token;
+        }
+        if (b.pos) b.pos += t0;
+        if (b.row) b.row += t0;
+        if (b.seq) b.seq += t0;
+        else if (b.row && t0) b.pages += (size_t)t0 * b.pages_per_seq, b.n_seqs -= std::min(t0, b.n_seqs);
+        const cudaError_t e = launch_ex(kern, dim3((uint32_t)((b.n_items + ROT_THREADS - 1) / ROT_THREADS)),
+                                        dim3(ROT_THREADS), 0, st, false, b);
+        if (e != cudaSuccess) return e;
+    }
+    return cudaSuccess;
+}
+
+void set_plan(RotateArgs& a, const q_b200_rope_plan* plan, bool transpose) {
+    a.rot = plan ? plan->rot_dim : 0;
+    a.interleaved = plan && plan->layout == Q_B200_ROPE_INTERLEAVED;
+    a.gain = plan ? plan->gain : 1.0f;
+    a.sign = transpose ? -a.gain : a.gain;
+    if (plan) std::memcpy(a.turns, plan->turns, sizeof(double) * (plan->rot_dim / 2));
+}
+
+// Elements of a vector: as many as 16 bytes of the narrowest type hold, if
+// every row part begins on such a vector (`by`: the divisor in bytes of all
+// addresses and strides of elements of `es` bytes) and the row divides.
+bool vectors_fit(uint32_t E, uint32_t es, uint64_t by, const RotateArgs& a) {
+    if (by < std::min<uint64_t>(16, (uint64_t)E * es)) return false;
+    const uint32_t pair = a.interleaved ? a.rot % (2 * E) : (a.rot / 2) % E;
+    return pair == 0 && (a.head_dim - a.rot) % E == 0;
+}
+
+// Heads that a thread takes: four where that still leaves two full waves of
+// threads (the angle is formed once and four heads' loads are in flight),
+// else one, for the shortest path through few tokens.
+uint32_t heads_per_thread(uint64_t items_of_one) { return items_of_one / 4 >= 148ull * 2048 * 2 ? 4u : 1u; }
+
+}  // namespace
+
+extern "C" {
+
+q_error_code q_b200_rope_plan_init(q_b200_rope_plan* plan, uint32_t rot_dim, q_b200_rope_layout layout, double base,
+                                   const q_b200_rope_scale* scale) {
+    if (!plan) return Q_ERR_INVALID_ARG;
+    if (rot_dim < 2 || rot_dim > 256 || rot_dim % 2) return Q_ERR_INVALID_SIZE;
+    if ((uint32_t)layout > Q_B200_ROPE_HALF || !(base > 1.0) || !std::isfinite(base)) return Q_ERR_INVALID_ARG;
+    const uint32_t kind = scale ? scale->kind : (uint32_t)Q_B200_ROPE_PLAIN;
+    if (kind > Q_B200_ROPE_YARN || (scale && scale->reserved)) return Q_ERR_INVALID_ARG;
+    if (kind != Q_B200_ROPE_PLAIN && !(scale->factor > 0.0 && std::isfinite(scale->factor))) return Q_ERR_INVALID_ARG;
+    if (kind >= Q_B200_ROPE_BANDED &&
+        !(scale->original_len > 0.0 && scale->low > 0.0 && scale->high > scale->low && std::isfinite(scale->high) &&
+          std::isfinite(scale->original_len)))
+        return Q_ERR_INVALID_ARG;
+    if (kind == Q_B200_ROPE_YARN && !(scale->gain >= 0.0 && std::isfinite(scale->gain))) return Q_ERR_INVALID_ARG;
+    const double tau = 6.283185307179586476925286766559;
+    std::memset(plan, 0, sizeof *plan);
+    plan->rot_dim = rot_dim;
+    plan->layout = layout;
+    plan->gain = 1.0f;
+    double low = 0.0, high = 0.0;
+    if (kind == Q_B200_ROPE_YARN) {
+        // pair index whose wave turns n times in original_len
+        auto pair_of = [&](double n) { return rot_dim * std::log(scale->original_len / (n * tau)) / (2.0 * std::log(base)); };
+        low = std::max(std::floor(pair_of(scale->high)), 0.0);
+        high = std::min(std::ceil(pair_of(scale->low)), (double)rot_dim - 1.0);
+        plan->gain = (float)(scale->gain > 0.0 ? scale->gain : 0.1 * std::log(scale->factor) + 1.0);
+    }
+    for (uint32_t i = 0; i < rot_dim / 2; ++i) {
+        double f = std::pow(base, -2.0 * i / rot_dim);
+        if (kind == Q_B200_ROPE_LINEAR) {
+            f /= scale->factor;
+        } else if (kind == Q_B200_ROPE_BANDED) {
+            const double turns = scale->original_len * f / tau;
+            const double s = std::min(std::max((turns - scale->low) / (scale->high - scale->low), 0.0), 1.0);
+            f = (1.0 - s) * f / scale->factor + s * f;
+        } else if (kind == Q_B200_ROPE_YARN) {
+            const double s = std::min(std::max((i - low) / std::max(high - low, 0.001), 0.0), 1.0);
+            f = f / scale->factor * s + f * (1.0 - s);
+        }
+        plan->turns[i] = f / tau;
+    }
+    return Q_OK;
+}
+
+q_error_code q_b200_rope(const q_b200_rope_args* r, void* stream) {
+    if (!r || !r->x || !r->out || !r->pos || !r->plan) return Q_ERR_INVALID_ARG;
+    if (!known(r->dtype)) return Q_ERR_INVALID_DTYPE;
+    if (r->reserved || r->transpose > 1) return Q_ERR_INVALID_ARG;
+    if (r->n_tokens == 0 || r->n_heads == 0 || r->head_dim == 0 || r->head_dim > 256) return Q_ERR_INVALID_SIZE;
+    if (q_error_code rc = check_plan(r->plan, r->head_dim)) return rc;
+    const uint32_t es = size_of(r->dtype);
+    if (((addr(r->x) | addr(r->out)) & (es - 1)) || (addr(r->pos) & 3)) return Q_ERR_MISALIGNED;
+    // in place means the same elements; another overlay would be read after it is written
+    if (r->x == r->out && (r->x_token_stride != r->out_token_stride || r->x_head_stride != r->out_head_stride))
+        return Q_ERR_ALIASING;
+    if (!DevicePtrs()(r->x)(r->out)(r->pos).ok) return Q_ERR_INVALID_ARG;
+    RotateArgs a{};
+    set_plan(a, r->plan, r->transpose != 0);
+    a.pos = r->pos;
+    a.n_tokens = r->n_tokens;
+    a.head_dim = r->head_dim;
+    RotateRows& p = a.part[2];
+    p.src = r->x;
+    p.dst = r->out;
+    p.src_token = r->x_token_stride;
+    p.src_head = r->x_head_stride;
+    p.dst_token = r->out_token_stride;
+    p.dst_head = r->out_head_stride;
+    p.heads = r->n_heads;
+    p.rotate = 1;
+    const uint64_t by = align_of({addr(r->x), addr(r->out), r->x_token_stride * es, r->x_head_stride * es,
+                                  r->out_token_stride * es, r->out_head_stride * es});
+    uint32_t E = es == 4 ? 4 : 8;
+    while (E > 1 && !vectors_fit(E, es, by, a)) E = E == 8 ? 4 : 1;
+    const uint32_t HB = heads_per_thread((uint64_t)r->n_tokens * r->n_heads * r->head_dim / (2 * E));
+    cudaStream_t st = (cudaStream_t)stream;
+    switch (r->dtype) {
+        case Q_B200_F32: Q_CUDA((launch_rotate<float, float>(a, E, HB, st))); break;
+        case Q_B200_F16: Q_CUDA((launch_rotate<__half, __half>(a, E, HB, st))); break;
+        default: Q_CUDA((launch_rotate<__nv_bfloat16, __nv_bfloat16>(a, E, HB, st))); break;
+    }
+    return Q_OK;
+}
+
+q_error_code q_b200_kv_append(const q_b200_append_args* r, void* stream) {
+    if (!r || !r->k || !r->v || !r->pages || !r->row) return Q_ERR_INVALID_ARG;
+    if (q_error_code rc = check_cache(r->kv)) return rc;
+    if (!known(r->dtype)) return Q_ERR_INVALID_DTYPE;
+    if (r->reserved || (r->q && !r->q_out)) return Q_ERR_INVALID_ARG;
+    if (r->n_tokens == 0 || r->n_seqs == 0 || r->pages_per_seq == 0 || (r->q && r->n_heads == 0)) return Q_ERR_INVALID_SIZE;
+    if (r->kv.head_dim > 256 || (!r->seq && r->n_tokens > r->n_seqs)) return Q_ERR_INVALID_SIZE;
+    if (r->plan)
+        if (q_error_code rc = check_plan(r->plan, r->kv.head_dim)) return rc;
+    const uint32_t es = size_of(r->dtype), ec = size_of(r->kv.dtype);
+    if (((addr(r->k) | addr(r->v) | addr(r->q) | addr(r->q_out)) & (es - 1)) ||
+        ((addr(r->pages) | addr(r->seq) | addr(r->row) | addr(r->pos)) & 3))
+        return Q_ERR_MISALIGNED;
+    if (r->q && r->q == r->q_out && (r->q_token_stride != r->q_out_token_stride || r->q_head_stride != r->q_out_head_stride))
+        return Q_ERR_ALIASING;
+    if (!DevicePtrs()(r->kv.k)(r->kv.v)(r->k)(r->v)(r->q)(r->q ? r->q_out : nullptr)(r->pages)(r->seq)(r->row)(r->pos).ok)
+        return Q_ERR_INVALID_ARG;
+    RotateArgs a{};
+    set_plan(a, r->plan, false);
+    a.pos = r->pos;
+    a.row = r->row;
+    a.seq = r->seq;
+    a.pages = r->pages;
+    a.page_stride = r->kv.page_stride;
+    a.row_stride = r->kv.row_stride;
+    a.page_rows = fast_div_of(r->kv.page_rows);
+    a.n_pages = r->kv.n_pages;
+    a.pages_per_seq = r->pages_per_seq;
+    a.n_seqs = r->n_seqs;
+    a.n_tokens = r->n_tokens;
+    a.head_dim = r->kv.head_dim;
+    const uint64_t hs = r->kv.head_stride;
+    a.part[0] = {r->k, r->kv.k, r->k_token_stride, r->k_head_stride, 0, hs, r->kv.n_kv_heads, 0, r->plan ? 1u : 0u, 1u};
+    a.part[1] = {r->v, r->kv.v, r->v_token_stride, r->v_head_stride, 0, hs, r->kv.n_kv_heads, 0, 0u, 1u};
+    if (r->q)
+        a.part[2] = {r->q, r->q_out, r->q_token_stride, r->q_head_stride, r->q_out_token_stride, r->q_out_head_stride,
+                     r->n_heads, 0, r->plan ? 1u : 0u, 0u};
+    uint64_t in = align_of({addr(r->k), addr(r->v), r->k_token_stride * es, r->k_head_stride * es, r->v_token_stride * es,
+                            r->v_head_stride * es});
+    if (r->q)
+        in = std::min(in, align_of({addr(r->q), addr(r->q_out), r->q_token_stride * es, r->q_head_stride * es,
+                                    r->q_out_token_stride * es, r->q_out_head_stride * es}));
+    const uint64_t to = align_of({addr(r->kv.k), addr(r->kv.v), r->kv.page_stride * ec, hs * ec, r->kv.row_stride * ec});
+    uint32_t E = es == 4 && ec == 4 ? 4 : 8;
+    while (E > 1 && !(vectors_fit(E, es, in, a) && vectors_fit(E, ec, to, a))) E = E == 8 ? 4 : 1;
+    const uint32_t heads = 2 * r->kv.n_kv_heads + (r->q ? r->n_heads : 0);
+    const uint32_t HB = heads_per_thread((uint64_t)r->n_tokens * heads * r->kv.head_dim / (2 * E));
+    cudaStream_t st = (cudaStream_t)stream;
+    auto go = [&](auto ti) -> cudaError_t {
+        using TI = decltype(ti);
+        switch (r->kv.dtype) {
+            case Q_B200_F32: return launch_rotate<TI, float>(a, E, HB, st);
+            case Q_B200_F16: return launch_rotate<TI, __half>(a, E, HB, st);
+            default: return launch_rotate<TI, __nv_bfloat16>(a, E, HB, st);
+        }
+    };
+    switch (r->dtype) {
+        case Q_B200_F32: Q_CUDA(go(float())); break;
+        case Q_B200_F16: Q_CUDA(go(__half())); break;
+        default: Q_CUDA(go(__nv_bfloat16())); break;
+    }
+    return Q_OK;
+}
+
+}  // extern "C"
+
+// ---- attention --------------------------------------------------------------------
+
+namespace {
+
+struct AttnPass {
+    uint32_t wm = 0, tiles = 0, items = 0, splits = 0;
+};
+struct AttnPlan {
+    bool shared = false;  // a pass of its own for the prefix
+    AttnPass pre, own;
+    uint32_t parts = 1;   // 1: written to out directly
+};
+
+uint32_t cdiv(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
+
+// Vectors of a CTA: 16, 32 or 64, the fewest that hold all of an item's.
+uint32_t groups_of(uint32_t vecs) { return vecs <= 16 ? 1 : vecs <= 32 ? 2 : 4; }
+
+AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t rows, uint32_t step, uint32_t want) {
+    AttnPass p;
+    p.wm = groups_of(vecs);
+    p.tiles = cdiv(vecs, 16 * p.wm);
+    p.items = p.tiles * seqs;
+    // cut the rows until the grid fills the GPU, but leave a part four tiles
+    const uint64_t ctas = (uint64_t)p.items * kv_heads;
+    p.splits = (uint32_t)std::min<uint64_t>({std::max<uint64_t>(1, want / ctas), std::max<uint32_t>(1, cdiv(rows, 4 * step)), 64});
+    return p;
+}
+
+q_error_code check_attn(const q_b200_attn_args* r) {
+    if (!known(r->kv.dtype)) return Q_ERR_INVALID_DTYPE;
+    const q_b200_paged_kv& kv = r->kv;
+    if (kv.n_pages == 0 || kv.page_rows == 0 || kv.page_rows > (1u << 30) || kv.n_kv_heads == 0) return Q_ERR_INVALID_SIZE;
+    if (kv.head_dim != 32 && kv.head_dim != 64 && kv.head_dim != 128) return Q_ERR_INVALID_SIZE;
+    if (r->n_tokens == 0 || r->n_seqs == 0 || r->n_heads == 0 || r->max_q == 0 || r->pages_per_seq == 0) return Q_ERR_INVALID_SIZE;
+    if (r->n_heads % kv.n_kv_heads || kv.n_kv_heads > 65535) return Q_ERR_INVALID_SIZE;
+    if ((uint64_t)r->n_tokens * r->n_heads >= (1u << 30) || (uint64_t)r->n_seqs * r->max_q * r->n_heads >= (1u << 30))
+        return Q_ERR_INVALID_SIZE;
+    if ((uint64_t)r->max_len + r->max_prefix >= (1u << 30)) return Q_ERR_INVALID_SIZE;
+    if ((uint64_t)r->pages_per_seq * kv.page_rows < r->max_len) return Q_ERR_INVALID_SIZE;
+    return Q_OK;
+}
+
+AttnPlan plan_attn(const q_b200_attn_args* r) {
+    const uint32_t G = r->n_heads / r->kv.n_kv_heads, step = r->kv.dtype == Q_B200_F32 ? 32 : 64;
+    AttnPlan p;
+    const uint32_t prefix = r->max_prefix, want = 2 * 148;
+    // A pass of its own reads the prefix once instead of once per sequence
+    // (from L2 after the first); it costs a join of at least two parts.
+    p.shared = prefix >= 2 * step && r->n_seqs > 1;
+    if (p.shared) {
+        p.pre = plan_pass(r->n_tokens * G, 1, r->kv.n_kv_heads, prefix, step, want);
+        p.own = plan_pass(r->max_q * G, r->n_seqs, r->kv.n_kv_heads, std::max(1u, r->max_len), step, want);
+        p.parts = p.pre.splits + p.own.splits;
+    } else {
+        p.own = plan_pass(r->max_q * G, r->n_seqs, r->kv.n_kv_heads, std::max(1u, prefix + r->max_len), step, want);
+        p.parts = p.own.splits;
+    }
+    return p;
+}
+
+size_t attn_bytes(const q_b200_attn_args* r, const AttnPlan& p) {
+    return p.parts == 1 ? 0 : (size_t)p.parts * r->n_tokens * r->n_heads * (r->kv.head_dim * 4 + 8);
+}
+
+template <typename T, int HD, int WM>
+cudaError_t launch_rows(const PrefixArgs& a, const AttnPass& p, uint32_t kv_heads, cudaStream_t st) {
+    const size_t smem = attn_rows_smem<T, HD, WM>();
+    if (cudaError_t e = ensure_smem_attr((const void*)attn_rows_kernel<T, HD, WM>, (int)smem)) return e;
+    return launch_ex(attn_rows_kernel<T, HD, WM>, dim3(p.splits, p.items, kv_heads), dim3(ATTN_THREADS), smem, st, false, a);
+}
+
+template <typename T, int HD>
+cudaError_t launch_pass(PrefixArgs a, const AttnPass& p, bool shared, uint32_t part0, uint32_t kv_heads, cudaStream_t st) {
+    a.shared = shared;
+    a.tiles = p.tiles;
+    a.splits = p.splits;
+    a.part0 = part0;
+    if (p.wm == 1) return launch_rows<T, HD, 1>(a, p, kv_heads, st);
+    if (p.wm == 2) return launch_rows<T, HD, 2>(a, p, kv_heads, st);
+    return launch_rows<T, HD, 4>(a, p, kv_heads, st);
+}
+
+template <typename T, int HD>
+cudaError_t launch_attn(PrefixArgs& a, const AttnPlan& p, uint32_t kv_heads, cudaStream_t st) {
+    cudaError_t e = cudaSuccess;
+    if (p.shared && (e = launch_pass<T, HD>(a, p.pre, true, 0, kv_heads, st))) return e;
+    a.with_prefix = !p.shared;
+    const uint32_t part0 = p.parts == 1 ? ~0u : p.shared ? p.pre.splits : 0u;
+    if ((e = launch_pass<T, HD>(a, p.own, false, part0, kv_heads, st))) return e;
+    if (p.parts == 1) return e;
+    a.n_parts = p.parts;
+    return launch_ex(attn_join_kernel<T, HD>, dim3(cdiv((uint64_t)a.n_tokens * a.n_heads, 4)), dim3(128), 0, st, false, a);
+}
+
+template <typename T>
+cudaError_t launch_attn_dim(PrefixArgs& a, const AttnPlan& p, const q_b200_paged_kv& kv, cudaStream_t st) {
+    if (kv.head_dim == 32) return launch_attn<T, 32>(a, p, kv.n_kv_heads, st);
+    if (kv.head_dim == 64) return launch_attn<T, 64>(a, p, kv.n_kv_heads, st);
+    return launch_attn<T, 128>(a, p, kv.n_kv_heads, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t q_b200_attn_work_bytes(const q_b200_attn_args* r) {
+    if (!r || check_attn(r) != Q_OK) return 0;
+    return attn_bytes(r, plan_attn(r));
+}
+
+q_error_code q_b200_attn_prefix(const q_b200_attn_args* r, void* stream) {
+    if (!r || !r->q || !r->out || !r->pages || !r->lens) return Q_ERR_INVALID_ARG;
+    if (q_error_code rc = check_cache(r->kv)) return rc;
+    if (q_error_code rc = check_attn(r)) return rc;
+    if (r->max_prefix && (!r->prefix_pages || !r->prefix_len)) return Q_ERR_INVALID_ARG;
+    if (!r->q_start && (r->max_q != 1 || r->n_tokens != r->n_seqs)) return Q_ERR_INVALID_SIZE;
+    if (!std::isfinite(r->scale)) return Q_ERR_INVALID_ARG;
+    if (r->q == r->out) return Q_ERR_ALIASING;
+    const uint32_t es = size_of(r->kv.dtype);
+    const uint64_t in = align_of({addr(r->q), addr(r->kv.k), addr(r->kv.v), r->q_token_stride * es, r->q_head_stride * es,
+                                  r->kv.page_stride * es, r->kv.head_stride * es, r->kv.row_stride * es});
+    const uint64_t to = align_of({addr(r->out), r->out_token_stride * es, r->out_head_stride * es});
+    if (in < 16 || to < 16) return Q_ERR_MISALIGNED;
+    if ((addr(r->q_start) | addr(r->pages) | addr(r->lens) | addr(r->prefix_pages) | addr(r->prefix_len)) & 3) return Q_ERR_MISALIGNED;
+    const AttnPlan p = plan_attn(r);
+    const size_t need = attn_bytes(r, p);
+    if (need && !r->work) return Q_ERR_INVALID_ARG;
+    if (need && r->work_bytes < need) return Q_ERR_INVALID_SIZE;
+    if (need && (addr(r->work) & 15)) return Q_ERR_MISALIGNED;
+    const bool pre = r->max_prefix > 0;
+    if (!DevicePtrs()(r->kv.k)(r->kv.v)(r->q)(r->out)(r->q_start)(r->pages)(r->lens)(pre ? r->prefix_pages : nullptr)(
+             pre ? r->prefix_len : nullptr)(need ? r->work : nullptr).ok)
+        return Q_ERR_INVALID_ARG;
+    PrefixArgs a{};
+    a.q = r->q;
+    a.out = r->out;
+    a.k = r->kv.k;
+    a.v = r->kv.v;
+    a.q_token = r->q_token_stride;
+    a.q_head = r->q_head_stride;
+    a.o_token = r->out_token_stride;
+    a.o_head = r->out_head_stride;
+    a.page_stride = r->kv.page_stride;
+    a.head_stride = r->kv.head_stride;
+    a.row_stride = r->kv.row_stride;
+    a.q_start = r->q_start;
+    a.pages = r->pages;
+    a.lens = r->lens;
+    a.prefix_pages = pre ? r->prefix_pages : nullptr;
+    a.prefix_len = pre ? r->prefix_len : nullptr;
+    a.part_o = (float*)r->work;
+    a.part_ml = (float2*)((float*)r->work + (size_t)p.parts * r->n_tokens * r->n_heads * r->kv.head_dim);
+    a.page_rows = fast_div_of(r->kv.page_rows);
+    a.group = r->n_heads / r->kv.n_kv_heads;
+    a.by_group = fast_div_of(a.group);
+    a.n_pages = r->kv.n_pages;
+    a.pages_per_seq = r->pages_per_seq;
+    a.n_tokens = r->n_tokens;
+    a.n_seqs = r->n_seqs;
+    a.n_heads = r->n_heads;
+    a.max_q = r->max_q;
+    a.max_len = r->max_len;
+    a.max_prefix = r->max_prefix;
+    a.c = r->scale * 1.44269504088896341f;
+    cudaStream_t st = (cudaStream_t)stream;
+    switch (r->kv.dtype) {
+        case Q_B200_F32: Q_CUDA(launch_attn_dim<float>(a, p, r->kv, st)); break;
+        case Q_B200_F16: Q_CUDA(launch_attn_dim<__half>(a, p, r->kv, st)); break;
+        default: Q_CUDA(launch_attn_dim<__nv_bfloat16>(a, p, r->kv, st)); break;
+    }
+    return Q_OK;
+}
+
+}  // extern "C"
+
+// ---- drafts -------------------------------------------------------------------------
+
+namespace {
+
+template <typename T, int KIND>
+cudaError_t launch_verify(const VerifyArgs& a, uint32_t n_seqs, uint32_t CL, cudaStream_t st) {
+    const void* kern = (const void*)verify_kernel<T, KIND>;
+    if (CL > 8)
+        if (cudaError_t e = cudaFuncSetAttribute(kern, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) return e;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n_seqs * CL);
+    cfg.blockDim = dim3(VER_THREADS);
+    cfg.stream = st;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = CL;
+    attr[0].val.clusterDim.y = 1;
+    attr[0].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+    return cudaLaunchKernelEx(&cfg, verify_kernel<T, KIND>, a);
+}
+
+template <typename T>
+cudaError_t launch_verify_kind(const VerifyArgs& a, int kind, uint32_t n_seqs, uint32_t CL, cudaStream_t st) {
+    if (kind == VER_PROBS) return launch_verify<T, VER_PROBS>(a, n_seqs, CL, st);
+    if (kind == VER_LOGITS) return launch_verify<T, VER_LOGITS>(a, n_seqs, CL, st);
+    return launch_verify<T, VER_GREEDY>(a, n_seqs, CL, st);
+}
+
+}  // namespace
+
+extern "C" {
+
+q_error_code q_b200_verify_draft(const q_b200_verify_args* r, void* stream) {
+    if (!r || !r->target || !r->uniform || !r->tokens || !r->n_tokens) return Q_ERR_INVALID_ARG;
+    if (r->n_draft && !r->draft_tokens) return Q_ERR_INVALID_ARG;
+    if (!known(r->dtype)) return Q_ERR_INVALID_DTYPE;
+    if (r->kind > Q_B200_LOGITS) return Q_ERR_INVALID_ARG;
+    if (r->n_seqs == 0 || r->vocab == 0 || r->vocab > (1u << 30) || r->n_draft > VER_MAX_DRAFT || r->n_seqs > (1u << 26))
+        return Q_ERR_INVALID_SIZE;
+    if (r->kind == Q_B200_LOGITS && !(r->temperature >= 0.0f && std::isfinite(r->temperature))) return Q_ERR_INVALID_ARG;
+    const uint32_t es = size_of(r->dtype);
+    if (((addr(r->target) | addr(r->draft)) & (es - 1)) ||
+        ((addr(r->draft_tokens) | addr(r->draft_len) | addr(r->uniform) | addr(r->tokens) | addr(r->n_tokens)) & 3))
+        return Q_ERR_MISALIGNED;
+    if ((const void*)r->tokens == (const void*)r->draft_tokens || (const void*)r->tokens == (const void*)r->n_tokens)
+        return Q_ERR_ALIASING;
+    if (!DevicePtrs()(r->target)(r->draft)(r->draft_tokens)(r->draft_len)(r->uniform)(r->tokens)(r->n_tokens).ok)
+        return Q_ERR_INVALID_ARG;
+    VerifyArgs a{};
+    a.target = r->target;
+    a.draft = r->n_draft ? r->draft : nullptr;
+    a.t_seq = r->target_seq_stride;
+    a.t_row = r->target_row_stride;
+    a.d_seq = r->draft_seq_stride;
+    a.d_row = r->draft_row_stride;
+    a.draft_tokens = r->draft_tokens;
+    a.draft_len = r->draft_len;
+    a.uniform = r->uniform;
+    a.tokens = r->tokens;
+    a.n_tokens = r->n_tokens;
+    a.n_draft = r->n_draft;
+    a.vocab = r->vocab;
+    uint64_t by = align_of({addr(r->target), a.t_seq * es, a.t_row * es});
+    if (a.draft) by = std::min(by, align_of({addr(r->draft), a.d_seq * es, a.d_row * es}));
+    a.vec = by >= 16;
+    const int kind = r->kind == Q_B200_PROBS ? VER_PROBS : r->temperature < 1e-6f ? VER_GREEDY : VER_LOGITS;
+    if (kind == VER_LOGITS) {
+        a.cd = 1.44269504088896340736 / (double)r->temperature;
+        a.c = (float)a.cd;
+    }
+    // CTAs of a sequence: as many as fill the GPU, but each with 2048 entries
+    uint32_t CL = VER_MAX_CL;
+    while (CL > 1 && ((uint64_t)r->n_seqs * CL > 148 || (uint64_t)CL * 2048 > r->vocab)) CL /= 2;
+    a.seg = (cdiv(r->vocab, (uint64_t)CL * VER_WARPS) + 7) & ~7u;
+    cudaStream_t st = (cudaStream_t)stream;
+    switch (r->dtype) {
+        case Q_B200_F32: Q_CUDA(launch_verify_kind<float>(a, kind, r->n_seqs, CL, st)); break;
+        case Q_B200_F16: Q_CUDA(launch_verify_kind<__half>(a, kind, r->n_seqs, CL, st)); break;
+        default: Q_CUDA(launch_verify_kind<__nv_bfloat16>(a, kind, r->n_seqs, CL, st)); break;
+    }
+    return Q_OK;
+}
+
+q_error_code q_b200_batch_kv_view(q_context* ctx, uint32_t layer, q_b200_paged_kv* kv, const uint32_t** pages,
+                                  uint32_t* pages_per_seq) {
+    if (!ctx || !kv || !pages || !pages_per_seq) return Q_ERR_INVALID_ARG;
+    DevState* s = state_of(ctx, false);
+    if (!s || !s->batch.kv || !s->batch.d_pages) return Q_ERR_INVALID_ARG;  // not a batch with paged caches
+    if (layer >= s->cfg.n_layers) return Q_ERR_INVALID_SIZE;
+    if (q_error_code rc = batch_sync_pages(s)) return rc;
+    const BatchState& b = s->batch;
+    const uint64_t head = (uint64_t)b.page_rows * 2 * s->hd;
+    *kv = q_b200_paged_kv{};
+    kv->k = b.kv + layer * s->tp.nkv * head;
+    kv->v = b.kv + layer * s->tp.nkv * head + s->hd;
+    kv->page_stride = (uint64_t)s->cfg.n_layers * s->tp.nkv * head;
+    kv->head_stride = head;
+    kv->row_stride = 2 * s->hd;
+    kv->n_pages = b.n_pages;
+    kv->page_rows = b.page_rows;
+    kv->n_kv_heads = s->tp.nkv;
+    kv->head_dim = s->hd;
+    kv->dtype = Q_B200_F32;
+    *pages = b.d_pages;
+    *pages_per_seq = b.pages_per_seq;
+    return Q_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,647 @@
+// attn_prefix.cuh — attention of a batch's new tokens over a shared prefix
+// and each sequence's own paged rows (q_b200_attn_prefix).
+//
+//   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(y_j - m),  y_j = scale log2(e) q.k_j
+//
+// over the rows j that the token sees, in one pass: a running maximum m and
+// sum l, and the accumulated output multiplied by 2^(m_old - m_new) when m
+// moves.  The rows may be cut into parts that different CTAs take; a part
+// leaves (m, l, o) in fp32 in the workspace and attn_join_kernel adds them
+// in part order (the same result on every run).
+//
+// attn_rows_kernel: one CTA takes 16 WM query vectors (tokens x the G heads
+// that share a KV head) and a range of rows in tiles that a ring of cp.async
+// stages brings in; a row's page is looked up by the thread that copies it,
+// so pages may have any size and end anywhere in a tile.  Its 4 warps are WM
+// groups of 16 vectors x 4/WM groups of the tile's rows; with WM = 1 (a
+// decoded token's few heads) every warp has rows of its own and the warps
+// are joined at the end.  Products are mma.sync: m16n8k16 for fp16 and
+// bf16; for fp32 m16n8k8 tf32 on halves v = hi + lo of 11 bits each, hi.hi +
+// hi.lo + lo.hi (the dropped lo.lo is 2^-22 relative), with the hi.hi sums
+// folded into fp32 every few products because the tensor core truncates
+// when it accumulates.  P is rounded to the cache's type for P.V (fp16,
+// bf16), as the products' operand type asks; l sums what is multiplied.
+//
+// Bound: bytes of K and V for few query vectors per row.
+#pragma once
+
+#include <type_traits>
+
+#include "rotate.cuh"
+
+namespace qb200 {
+
+struct PrefixArgs {
+    const void* q;
+    void* out;
+    const void* k;
+    const void* v;
+    uint64_t q_token, q_head, o_token, o_head;
+    uint64_t page_stride, head_stride, row_stride;
+    const uint32_t* q_start;
+    const uint32_t* pages;
+    const uint32_t* lens;
+    const uint32_t* prefix_pages;
+    const uint32_t* prefix_len;
+    float* part_o;    // [parts][n_tokens][n_heads][HD]
+    float2* part_ml;  // [parts][n_tokens][n_heads]
+    FastDiv page_rows, by_group;
+    uint32_t n_pages, pages_per_seq, n_tokens, n_seqs, n_heads, group;
+    uint32_t max_q, max_len, max_prefix;
+    uint32_t tiles;      // row tiles of an item (prefix: of all tokens; own: of one sequence)
+    uint32_t splits;     // parts that an item's rows are cut into
+    uint32_t part0;      // this launch's first part; ~0: the only part, written to out
+    uint32_t n_parts;    // of the join
+    uint32_t shared;     // 1: the prefix for all tokens; 0: per sequence
+    uint32_t with_prefix;  // own pass: the prefix's rows come before the own ones
+    float c;             // scale * log2(e)
+};
+
+template <typename T>
+struct AttnTraits;
+template <>
+struct AttnTraits<__half> {
+    static constexpr int KT = 64, STAGES = 3;
+};
+template <>
+struct AttnTraits<__nv_bfloat16> {
+    static constexpr int KT = 64, STAGES = 3;
+};
+template <>
+struct AttnTraits<float> {
+    static constexpr int KT = 32, STAGES = 3;
+};
+
+static constexpr uint32_t ATTN_THREADS = 128;
+
+template <typename T, int HD, int WM>
+constexpr size_t attn_rows_smem() {
+    return (size_t)AttnTraits<T>::STAGES * AttnTraits<T>::KT * HD * sizeof(T) * 2 + 16 * WM * HD * sizeof(T);
+}
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+    asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+                 : "r"(addr));
+}
+
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __half) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1, __nv_bfloat16) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile(
+        "mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+        : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// v = hi + lo, each of 11 significant bits rounded to nearest (the tensor
+// core reads the upper 19 bits of an operand).
+__device__ __forceinline__ void split_tf32(uint32_t v, uint32_t& hi, uint32_t& lo) {
+    hi = (v + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(__uint_as_float(v) - __uint_as_float(hi)) + 0x1000u;
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
+}
+
+// 16-byte chunk c of row r in a tile of HD-wide rows: chunks are exchanged
+// within 128 bytes so that 8 rows' equal chunks lie in 8 different banks
+// groups.  Rows of 64 bytes (two to a bank line) turn every second row.
+template <typename T, int HD>
+__device__ __forceinline__ uint32_t tile_off(uint32_t r, uint32_t c) {
+    constexpr uint32_t RB = HD * sizeof(T);
+    if constexpr (RB >= 128) return r * RB + ((c ^ (r & 7)) << 4);
+    else return r * RB + ((c ^ ((r >> 1) & 3)) << 4);
+}
+// fp32 values are read element by element along rows 2t, 2t+1: rows 0, 2, 4,
+// 6 have to differ by two chunks.
+template <int HD>
+__device__ __forceinline__ uint32_t v32_off(uint32_t r, uint32_t c) {
+    return r * HD * 4 + ((c ^ (((r >> 1) & 3) << 1)) << 4);
+}
+
+template <typename T, int HD>
+__device__ __forceinline__ uint32_t vt_off(uint32_t r, uint32_t c) {
+    if constexpr (sizeof(T) == 4) return v32_off<HD>(r, c);
+    else return tile_off<T, HD>(r, c);
+}
+// Whether the 16 bytes at a shared address hold finite numbers only.
+template <typename T>
+__device__ __forceinline__ bool finite16(uint32_t addr) {
+    uint32_t x[4];
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(x[0]), "=r"(x[1]), "=r"(x[2]), "=r"(x[3]) : "r"(addr));
+    constexpr uint32_t E = sizeof(T) == 4 ? 0x7f800000u : 0u;
+    bool ok = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if constexpr (E != 0u) {
+            ok &= (x[i] & E) != E;
+        } else {
+            constexpr uint32_t lo = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+            ok &= (x[i] & lo) != lo && (x[i] & (lo << 16)) != (lo << 16);
+        }
+    }
+    return ok;
+}
+
+// What a CTA has to do.
+struct AttnItem {
+    uint32_t tok0, n_tok;   // tokens that its vectors come from
+    uint32_t vec0, n_vec;   // vectors (token, head in group) of this tile
+    uint32_t seq;           // own rows of this sequence
+    uint32_t n_prefix;      // rows 0..n_prefix-1 are the prefix's
+    uint32_t n_rows;        // all rows
+    uint32_t r0, r1;        // this part's
+    int32_t see0;           // vector of token i sees rows < see0 + i (own), all when >= n_rows
+};
+
+__device__ __forceinline__ bool attn_item(const PrefixArgs& a, uint32_t item, uint32_t split, uint32_t vecs, uint32_t step,
+                                          AttnItem& w) {
+    uint32_t P = 0, L = 0;
+    if ((a.shared || a.with_prefix) && a.prefix_pages) {
+        P = __ldg(a.prefix_len);
+        if (P > a.max_prefix) {
+            qdev_fail(QDEV_BAD_ARG);
+            P = a.max_prefix;
+        }
+    }
+    uint32_t tile = item;
+    w.seq = 0;
+    if (a.shared) {
+        w.tok0 = 0;
+        w.n_tok = a.n_tokens;
+        w.see0 = 0x40000000;
+    } else {
+        w.seq = item / a.tiles;
+        tile = item - w.seq * a.tiles;
+        if (a.q_start) {
+            const uint32_t s0 = __ldg(a.q_start + w.seq), s1 = __ldg(a.q_start + w.seq + 1);
+            const bool bad = s0 > s1 || s1 > a.n_tokens || s1 - s0 > a.max_q;
+            if (bad) qdev_fail(QDEV_BAD_ARG);
+            w.tok0 = s0;
+            w.n_tok = bad ? 0 : s1 - s0;
+        } else {
+            w.tok0 = w.seq;
+            w.n_tok = 1;
+        }
+        L = __ldg(a.lens + w.seq);
+        if (L > a.max_len) {
+            qdev_fail(QDEV_BAD_ARG);
+            L = a.max_len;
+        }
+        w.see0 = (int32_t)(P + L) - (int32_t)w.n_tok + 1;
+    }
+    w.n_prefix = P;
+    w.n_rows = P + L;
+    w.vec0 = tile * vecs;
+    const uint32_t all = w.n_tok * a.group;
+    if (w.vec0 >= all) return false;
+    w.n_vec = min(vecs, all - w.vec0);
+    const uint32_t chunk = ((w.n_rows + a.splits - 1) / a.splits + step - 1) / step * step;
+    w.r0 = min(split * chunk, w.n_rows);
+    w.r1 = min(w.r0 + chunk, w.n_rows);
+    return true;
+}
+
+// Offset of row r of the item (elements); false where its page is not one.
+__device__ __forceinline__ bool attn_row(const PrefixArgs& a, const AttnItem& w, uint32_t head, uint32_t r, uint64_t& off) {
+    const bool pre = r < w.n_prefix;
+    const uint32_t i = pre ? r : r - w.n_prefix, pi = fast_div(i, a.page_rows);
+    const uint32_t pg = __ldg(pre ? a.prefix_pages + pi : a.pages + (size_t)w.seq * a.pages_per_seq + pi);
+    if (pg >= a.n_pages) {
+        qdev_fail(QDEV_BAD_ARG);
+        off = 0;
+        return false;
+    }
+    off = pg * a.page_stride + head * a.head_stride + (uint64_t)(i - pi * a.page_rows.d) * a.row_stride;
+    return true;
+}
+
+template <typename T, int HD, int WM>
+__global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_constant__ PrefixArgs a) {
+    constexpr bool F32 = sizeof(T) == 4;
+    constexpr int KT = AttnTraits<T>::KT, ST = AttnTraits<T>::STAGES;
+    constexpr int WN = 4 / WM, KW = KT / WN;       // groups of rows, rows of one warp in a tile
+    constexpr int NT = KW / 8, ND = HD / 8;        // score and output tiles of 8 columns
+    constexpr int CH = HD * (int)sizeof(T) / 16;   // 16-byte chunks of a row
+    constexpr int RP = ATTN_THREADS / CH;          // rows that one copy instruction of the CTA brings
+    constexpr uint32_t TILE = KT * HD * sizeof(T);
+    extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ bool s_bad[KT];
+    const uint32_t s_kv = smem_u32(smem), s_q = s_kv + ST * 2 * TILE;
+    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
+    const uint32_t wm = warp % WM, wn = warp / WM;
+    const uint32_t split = blockIdx.x, head = blockIdx.z;
+
+    AttnItem w;
+    if (!attn_item(a, blockIdx.y, split, 16 * WM, KT, w)) return;
+
+    // the query vectors
+    for (uint32_t e = tid; e < 16 * WM * CH; e += ATTN_THREADS) {
+        const uint32_t r = e / CH, c = e % CH;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (r < w.n_vec) {
+            const uint32_t i = fast_div(w.vec0 + r, a.by_group), h = head * a.group + (w.vec0 + r - i * a.group);
+            v = __ldg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(a.q) + (uint64_t)(w.tok0 + i) * a.q_token + h * a.q_head) + c);
+        }
+        *reinterpret_cast<uint4*>(smem + ST * 2 * TILE + tile_off<T, HD>(r, c)) = v;
+    }
+
+    const uint32_t n_tiles = (w.r1 - w.r0 + KT - 1) / KT;
+    const T* kb = reinterpret_cast<const T*>(a.k);
+    const T* vb = reinterpret_cast<const T*>(a.v);
+    const uint32_t lr = tid / CH, lc = tid % CH;
+    auto issue = [&](uint32_t tile) {
+        if (tile < n_tiles) {
+            const uint32_t st = s_kv + (tile % ST) * 2 * TILE;
+#pragma unroll
+            for (int p = 0; p < KT / RP; ++p) {
+                const uint32_t r = p * RP + lr, row = w.r0 + tile * KT + r;
+                uint64_t off = 0;
+                const bool ok = row < w.r1 && attn_row(a, w, head, row, off);
+                const uint32_t n = ok ? 16u : 0u;  // nothing read, zeros written
+                cp_async16(st + tile_off<T, HD>(r, lc), kb + off + lc * (16 / sizeof(T)), n);
+                cp_async16(st + TILE + (F32 ? v32_off<HD>(r, lc) : tile_off<T, HD>(r, lc)), vb + off + lc * (16 / sizeof(T)), n);
+            }
+        }
+        cp_async_commit();
+    };
+#pragma unroll
+    for (int s = 0; s < ST - 1; ++s) issue(s);
+    __syncthreads();
+
+    uint32_t qf[F32 ? 1 : HD / 16][4];
+    if constexpr (!F32) {
+#pragma unroll
+        for (int j = 0; j < HD / 16; ++j)
+            ldsm4(s_q + tile_off<T, HD>(wm * 16 + (lane & 15), 2 * j + (lane >> 4)), qf[j]);
+    }
+
+    // vectors g and g + 8 of this warp's 16: rows they see, running maximum and sum
+    int32_t see[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        const uint32_t v = w.vec0 + wm * 16 + g + 8 * h;
+        see[h] = w.see0 + (int32_t)fast_div(v, a.by_group);
+        // tokens before the first own row see the prefix alone
+        if (!a.shared) see[h] = max(see[h], (int32_t)w.n_prefix);
+    }
+    float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.0f, 0.0f};
+    float o[ND][4];
+#pragma unroll
+    for (int n = 0; n < ND; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
+
+    for (uint32_t tile = 0; tile < n_tiles; ++tile) {
+        cp_async_wait<ST - 2>();
+        __syncthreads();
+        issue(tile + ST - 1);
+        const uint32_t sk = s_kv + (tile % ST) * 2 * TILE, sv = sk + TILE;
+        const uint32_t first = w.r0 + tile * KT;  // row of the tile's key 0
+
+        // ---- scores -----------------------------------------------------------------
+        float s[NT][4];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.0f;
+        if constexpr (!F32) {
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int j = 0; j < HD / 32; ++j) {
+                    uint32_t b[4];
+                    ldsm4(sk + tile_off<T, HD>(wn * KW + n * 8 + (lane & 7), 4 * j + (lane >> 3)), b);
+                    mma16(s[n], qf[2 * j], b[0], b[1], T());
+                    mma16(s[n], qf[2 * j + 1], b[2], b[3], T());
+                }
+        } else {
+            float sl[NT][4];
+#pragma unroll
+            for (int n = 0; n < NT; ++n) sl[n][0] = sl[n][1] = sl[n][2] = sl[n][3] = 0.0f;
+#pragma unroll 2
+            for (int j = 0; j < HD / 16; ++j) {  // two k8 steps
+                uint32_t qh[2][4], ql[2][4];
+#pragma unroll
+                for (int e = 0; e < 2; ++e) {
+                    uint32_t q[4];
+                    ldsm4(s_q + tile_off<T, HD>(wm * 16 + (lane & 15), 2 * (2 * j + e) + (lane >> 4)), q);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) split_tf32(q[i], qh[e][i], ql[e][i]);
+                }
+#pragma unroll
+                for (int n = 0; n < NT; ++n) {
+                    uint32_t b[4], bh[4], bl[4];
+                    ldsm4(sk + tile_off<T, HD>(wn * KW + n * 8 + (lane & 7), 4 * j + (lane >> 3)), b);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) split_tf32(b[i], bh[i], bl[i]);
+                    float hh[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                    for (int e = 0; e < 2; ++e) {
+                        mma8(hh, qh[e], bh[2 * e], bh[2 * e + 1]);
+                        mma8(sl[n], qh[e], bl[2 * e], bl[2 * e + 1]);
+                        mma8(sl[n], ql[e], bh[2 * e], bh[2 * e + 1]);
+                    }
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[n][i] += hh[i];
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < NT; ++n)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) s[n][i] += sl[n][i];
+        }
+
+        // ---- mask, running maximum, exponentials ----------------------------------------
+        const bool edge = first + KT > w.r1 || (int32_t)(first + KT) > w.see0;
+        float mx[2] = {m[0], m[1]};
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float y = s[n][i] * a.c;
+                if (edge) {
+                    const uint32_t row = first + wn * KW + n * 8 + 2 * t + (i & 1);
+                    if (row >= w.r1 || (int32_t)row >= see[i >> 1]) y = -INFINITY;
+                }
+                s[n][i] = y;
+                // a NaN score is carried into the sum, not into the maximum
+                mx[i >> 1] = fmaxf(mx[i >> 1], y);
+            }
+        float corr[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+            mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+            corr[h] = m[h] == mx[h] ? 1.0f : exp2f(m[h] - mx[h]);
+            m[h] = mx[h];
+            l[h] *= corr[h];
+        }
+        uint32_t pf[F32 ? 1 : NT][2];
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) s[n][i] = s[n][i] == -INFINITY ? 0.0f : exp2f(s[n][i] - m[i >> 1]);
+            if constexpr (!F32) {
+                pf[n][0] = pack2<T>(s[n][0], s[n][1]);
+                pf[n][1] = pack2<T>(s[n][2], s[n][3]);
+                const float2 x = unpack2<T>(pf[n][0]), y = unpack2<T>(pf[n][1]);
+                l[0] += x.x + x.y;
+                l[1] += y.x + y.y;
+            } else {
+                l[0] += s[n][0] + s[n][1];
+                l[1] += s[n][2] + s[n][3];
+            }
+        }
+
+        // A row that only some of the tokens see may hold anything as far as the others are
+        // concerned, and their weight 0 times an infinity or NaN in V would reach them: such
+        // rows leave the tile and are added, where seen, after the product.
+        const uint32_t hid0 = max((int32_t)first, w.see0), hid1 = min(first + KT, w.r1);
+        bool bad = false;
+        if (w.n_tok > 1 && !a.shared && hid0 < hid1) {
+            for (uint32_t e = tid + (hid0 - first) * CH; e < (hid1 - first) * CH; e += ATTN_THREADS)
+                bad |= !finite16<T>(sv + vt_off<T, HD>(e / CH, e % CH));
+            bad = __syncthreads_or(bad);
+            if (bad) {
+                if (tid < KT) s_bad[tid] = false;
+                __syncthreads();
+                for (uint32_t e = tid + (hid0 - first) * CH; e < (hid1 - first) * CH; e += ATTN_THREADS)
+                    if (!finite16<T>(sv + vt_off<T, HD>(e / CH, e % CH))) s_bad[e / CH] = true;
+                __syncthreads();
+                for (uint32_t e = tid + (hid0 - first) * CH; e < (hid1 - first) * CH; e += ATTN_THREADS)
+                    if (s_bad[e / CH])
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + vt_off<T, HD>(e / CH, e % CH)), "r"(0) : "memory");
+                __syncthreads();
+            }
+        }
+
+        // ---- P V ------------------------------------------------------------------------
+        if constexpr (!F32) {
+            if (corr[0] != 1.0f || corr[1] != 1.0f) {
+#pragma unroll
+                for (int n = 0; n < ND; ++n) {
+                    o[n][0] *= corr[0];
+                    o[n][1] *= corr[0];
+                    o[n][2] *= corr[1];
+                    o[n][3] *= corr[1];
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < NT / 2; ++j) {
+                const uint32_t pa[4] = {pf[2 * j][0], pf[2 * j][1], pf[2 * j + 1][0], pf[2 * j + 1][1]};
+#pragma unroll
+                for (int n = 0; n < ND / 2; ++n) {
+                    uint32_t b[4];
+                    ldsm4_t(sv + tile_off<T, HD>(wn * KW + j * 16 + (lane & 15), 2 * n + (lane >> 4)), b);
+                    mma16(o[2 * n], pa, b[0], b[1], T());
+                    mma16(o[2 * n + 1], pa, b[2], b[3], T());
+                }
+            }
+        } else {
+            // key 2t is column t of the product's A operand and key 2t + 1 column t + 4
+            uint32_t ph[NT][4], pl[NT][4];
+#pragma unroll
+            for (int j = 0; j < NT; ++j) {
+                split_tf32(__float_as_uint(s[j][0]), ph[j][0], pl[j][0]);
+                split_tf32(__float_as_uint(s[j][2]), ph[j][1], pl[j][1]);
+                split_tf32(__float_as_uint(s[j][1]), ph[j][2], pl[j][2]);
+                split_tf32(__float_as_uint(s[j][3]), ph[j][3], pl[j][3]);
+            }
+#pragma unroll
+            for (int n = 0; n < ND; ++n) {
+                float hh[4] = {0.0f, 0.0f, 0.0f, 0.0f}, ll[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const uint32_t r = wn * KW + j * 8 + 2 * t, c = 2 * n + (g >> 2);
+                    uint32_t b0, b1, h0, l0, h1, l1;
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(b0) : "r"(sv + v32_off<HD>(r, c) + (g & 3) * 4));
+                    asm volatile("ld.shared.b32 %0, [%1];" : "=r"(b1) : "r"(sv + v32_off<HD>(r + 1, c) + (g & 3) * 4));
+                    split_tf32(b0, h0, l0);
+                    split_tf32(b1, h1, l1);
+                    mma8(hh, ph[j], h0, h1);
+                    mma8(ll, ph[j], l0, l1);
+                    mma8(ll, pl[j], h0, h1);
+                }
+#pragma unroll
+                for (int i = 0; i < 4; ++i) o[n][i] = fmaf(o[n][i], corr[i >> 1], hh[i] + ll[i]);
+            }
+        }
+        if (bad) {
+            for (uint32_t r = max(hid0 - first, wn * KW); r < min(hid1 - first, (wn + 1) * KW); ++r) {
+                uint64_t off;
+                if (!s_bad[r] || !attn_row(a, w, head, first + r, off)) continue;
+                float p[2] = {0.0f, 0.0f};  // of vectors g and g + 8, held by the quad's lane that has column r
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        if (n == (int)((r - wn * KW) >> 3) && (uint32_t)(i & 1) == (r & 1)) p[i >> 1] = s[n][i];
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    p[h] = __shfl_sync(0xffffffffu, p[h], (lane & ~3u) | ((r >> 1) & 3));
+                    if ((int32_t)(first + r) >= see[h]) continue;
+#pragma unroll
+                    for (int n = 0; n < ND; ++n)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) o[n][2 * h + i] = fmaf(p[h], (float)vb[off + n * 8 + 2 * t + i], o[n][2 * h + i]);
+                }
+            }
+        }
+    }
+    cp_async_wait<0>();
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+        l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+    }
+    __syncthreads();
+
+    // ---- join the groups of rows, then this part's result -----------------------------------
+    float* s_o = reinterpret_cast<float*>(smem);                 // [16 WM][HD + 4]
+    float* s_ml = s_o + 16 * WM * (HD + 4);                      // [WN][16 WM][2]
+    const uint32_t v0 = wm * 16 + g;
+    if (WN > 1) {
+        if (t == 0) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                s_ml[(wn * 16 * WM + v0 + 8 * h) * 2] = m[h];
+                s_ml[(wn * 16 * WM + v0 + 8 * h) * 2 + 1] = l[h];
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            float M = -INFINITY, Lsum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < WN; ++k) M = fmaxf(M, s_ml[(k * 16 * WM + v0 + 8 * h) * 2]);
+#pragma unroll
+            for (int k = 0; k < WN; ++k) {
+                const float mk = s_ml[(k * 16 * WM + v0 + 8 * h) * 2], lk = s_ml[(k * 16 * WM + v0 + 8 * h) * 2 + 1];
+                Lsum += mk == -INFINITY ? lk : lk * exp2f(mk - M);
+            }
+            const float f = m[h] == -INFINITY ? 1.0f : exp2f(m[h] - M);
+#pragma unroll
+            for (int n = 0; n < ND; ++n) {
+                o[n][2 * h] *= f;
+                o[n][2 * h + 1] *= f;
+            }
+            m[h] = M;
+            l[h] = Lsum;
+        }
+    }
+    for (int k = 0; k < WN; ++k) {
+        if ((int)wn == k) {
+#pragma unroll
+            for (int n = 0; n < ND; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    float2* d = reinterpret_cast<float2*>(s_o + (v0 + 8 * h) * (HD + 4) + n * 8 + 2 * t);
+                    float2 x = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+                    if (k > 0) {
+                        x.x += d->x;
+                        x.y += d->y;
+                    }
+                    *d = x;
+                }
+        }
+        __syncthreads();
+    }
+    if (wn == 0 && t == 0) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            s_ml[(v0 + 8 * h) * 2] = m[h];
+            s_ml[(v0 + 8 * h) * 2 + 1] = l[h];
+        }
+    }
+    __syncthreads();
+    for (uint32_t e = tid; e < w.n_vec * (HD / 4); e += ATTN_THREADS) {
+        const uint32_t r = e / (HD / 4), c = e % (HD / 4);
+        const uint32_t i = fast_div(w.vec0 + r, a.by_group), h = head * a.group + (w.vec0 + r - i * a.group);
+        const uint64_t tok = w.tok0 + i;
+        float4 x = *reinterpret_cast<const float4*>(s_o + r * (HD + 4) + c * 4);
+        const float pm = s_ml[r * 2], pl = s_ml[r * 2 + 1];
+        if (a.part0 == ~0u) {
+            const float inv = pl == 0.0f ? 0.0f : 1.0f / pl;
+            float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+            if (pl == 0.0f) y[0] = y[1] = y[2] = y[3] = 0.0f;
+            store_vec<T, 4>(reinterpret_cast<T*>(a.out) + tok * a.o_token + h * a.o_head + c * 4, y);
+        } else {
+            const uint64_t at = ((uint64_t)(a.part0 + split) * a.n_tokens + tok) * a.n_heads + h;
+            reinterpret_cast<float4*>(a.part_o + at * HD)[c] = x;
+            if (c == 0) a.part_ml[at] = make_float2(pm, pl);
+        }
+    }
+}
+
+// One warp adds the parts of one (token, head), in part order.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ PrefixArgs a) {
+    const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    if (id >= a.n_tokens * a.n_heads) return;
+    const uint32_t tok = id / a.n_heads, h = id - tok * a.n_heads;
+    if (a.q_start && (tok < __ldg(a.q_start) || tok >= __ldg(a.q_start + a.n_seqs))) return;  // no sequence's token
+    const uint64_t stride = (uint64_t)a.n_tokens * a.n_heads;
+    float M = -INFINITY;
+    for (uint32_t p = lane; p < a.n_parts; p += 32) M = fmaxf(M, a.part_ml[p * stride + id].x);
+    M = warp_max(M);
+    float L = 0.0f, o[HD / 32];
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) o[i] = 0.0f;
+    for (uint32_t p = 0; p < a.n_parts; ++p) {
+        const float2 ml = a.part_ml[p * stride + id];
+        if (ml.y == 0.0f) continue;  // no row of this part is seen (a NaN sum is)
+        const float f = ml.x == -INFINITY ? 1.0f : exp2f(ml.x - M);
+        L += ml.y * f;
+#pragma unroll
+        for (int i = 0; i < HD / 32; ++i) o[i] = fmaf(a.part_o[(p * stride + id) * HD + i * 32 + lane], f, o[i]);
+    }
+    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+#pragma unroll
+    for (int i = 0; i < HD / 32; ++i) {
+        T* d = reinterpret_cast<T*>(a.out) + (uint64_t)tok * a.o_token + (uint64_t)h * a.o_head + i * 32 + lane;
+        *d = (T)(o[i] * inv);
+    }
+}
+
+}  // namespace qb200

@@ -10,4 +10,5 @@
 #include "api_model.cu"
 #include "api_ops.cu"
 #include "api_noalloc.cu"
+#include "api_serve.cu"
 #include "tokenizer.cu"

@@ -31,6 +31,10 @@ ERRORS = {
     -13: "Q_ERR_MISALIGNED", -14: "Q_ERR_INVALID_DTYPE", -15: "Q_ERR_INVALID_SIZE",
 }
 Q_F32, Q_Q8_0, Q_Q4_0 = 0, 1, 2
+Q_B200_F32, Q_B200_F16, Q_B200_BF16 = 0, 1, 2
+Q_B200_ROPE_INTERLEAVED, Q_B200_ROPE_HALF = 0, 1
+Q_B200_ROPE_PLAIN, Q_B200_ROPE_LINEAR, Q_B200_ROPE_BANDED, Q_B200_ROPE_YARN = 0, 1, 2, 3
+Q_B200_PROBS, Q_B200_LOGITS = 0, 1
 
 
 class QorusError(RuntimeError):
@@ -92,7 +96,55 @@ class q_generation_state(C.Structure):
                 ("top_p", C.c_float), ("current_pos", C.c_uint32)]
 
 
+class q_b200_paged_kv(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p)] + [(n, C.c_uint64) for n in (
+        "page_stride", "head_stride", "row_stride")] + [(n, C.c_uint32) for n in (
+            "n_pages", "page_rows", "n_kv_heads", "head_dim", "dtype", "reserved")]
+
+
+class q_b200_rope_scale(C.Structure):
+    _fields_ = [("kind", C.c_uint32), ("reserved", C.c_uint32)] + [(n, C.c_double) for n in (
+        "factor", "low", "high", "original_len", "gain")]
+
+
+class q_b200_rope_plan(C.Structure):
+    _fields_ = [("rot_dim", C.c_uint32), ("layout", C.c_uint32), ("gain", C.c_float),
+                ("reserved", C.c_uint32), ("turns", C.c_double * 128)]
+
+
+class q_b200_rope_args(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("x", "out", "pos", "plan")] + [(n, C.c_uint64) for n in (
+        "x_token_stride", "x_head_stride", "out_token_stride", "out_head_stride")] + [(n, C.c_uint32) for n in (
+            "n_tokens", "n_heads", "head_dim", "dtype", "transpose", "reserved")]
+
+
+class q_b200_append_args(C.Structure):
+    _fields_ = [("kv", q_b200_paged_kv)] + [(n, C.c_void_p) for n in ("k", "v", "q", "q_out")] + [
+        (n, C.c_uint64) for n in ("k_token_stride", "k_head_stride", "v_token_stride", "v_head_stride",
+                                  "q_token_stride", "q_head_stride", "q_out_token_stride",
+                                  "q_out_head_stride")] + [
+        (n, C.c_void_p) for n in ("pages", "seq", "row", "pos", "plan")] + [
+        (n, C.c_uint32) for n in ("n_tokens", "n_seqs", "pages_per_seq", "n_heads", "dtype", "reserved")]
+
+
+class q_b200_attn_args(C.Structure):
+    _fields_ = [("kv", q_b200_paged_kv), ("q", C.c_void_p), ("out", C.c_void_p)] + [
+        (n, C.c_uint64) for n in ("q_token_stride", "q_head_stride", "out_token_stride", "out_head_stride")] + [
+        (n, C.c_void_p) for n in ("q_start", "pages", "lens", "prefix_pages", "prefix_len", "work")] + [
+        ("work_bytes", C.c_uint64)] + [(n, C.c_uint32) for n in (
+            "n_tokens", "n_seqs", "n_heads", "pages_per_seq", "max_q", "max_len", "max_prefix")] + [
+        ("scale", C.c_float)]
+
+
+class q_b200_verify_args(C.Structure):
+    _fields_ = [("target", C.c_void_p), ("draft", C.c_void_p)] + [(n, C.c_uint64) for n in (
+        "target_seq_stride", "target_row_stride", "draft_seq_stride", "draft_row_stride")] + [
+        (n, C.c_void_p) for n in ("draft_tokens", "draft_len", "uniform", "tokens", "n_tokens")] + [
+        (n, C.c_uint32) for n in ("n_seqs", "n_draft", "vocab", "dtype", "kind")] + [("temperature", C.c_float)]
+
+
 _vp, _sz, _u32, _u64, _f, _i = C.c_void_p, C.c_size_t, C.c_uint32, C.c_uint64, C.c_float, C.c_int
+_d = C.c_double
 # Every function include/qorus.h and include/qorus_b200.h declare.
 _SIGS = {
     "q_init_memory": (_i, [_vp, C.c_char_p]),
@@ -148,6 +200,13 @@ _SIGS = {
     "q_b200_gemv_q4_noalloc": (_i, [_vp, _u32, _u32, _vp, _vp, _vp]),
     "q_b200_gemm_q4": (_i, [_vp, _u32, _u32, _vp, _u32, _vp, _vp]),
     "q_b200_gemv_f32": (_i, [_vp, _u32, _u32, _vp, _vp, _vp]),
+    "q_b200_rope_plan_init": (_i, [_vp, _u32, _i, _d, _vp]),
+    "q_b200_rope": (_i, [_vp, _vp]),
+    "q_b200_kv_append": (_i, [_vp, _vp]),
+    "q_b200_attn_work_bytes": (_sz, [_vp]),
+    "q_b200_attn_prefix": (_i, [_vp, _vp]),
+    "q_b200_verify_draft": (_i, [_vp, _vp]),
+    "q_b200_batch_kv_view": (_i, [_vp, _u32, _vp, _vp, _vp]),
     "q_b200_tp_unique_id": (_i, [_vp, _sz]),
     "q_b200_tp_init": (_i, [_vp, _u32, _u32, _vp, _sz]),
     "q_b200_tp_ipc_handle": (_i, [_vp, _vp, _sz]),
