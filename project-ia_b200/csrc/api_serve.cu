@@ -6,6 +6,7 @@
 #include <cmath>
 
 #include "attn_prefix.cuh"
+#include "attn_prefix_tc.cuh"
 #include "runtime.cuh"
 #include "verify.cuh"
 
@@ -286,7 +287,8 @@ q_error_code q_b200_kv_append(const q_b200_append_args* r, void* stream) {
 namespace {
 
 struct AttnPass {
-    uint32_t wm = 0, tiles = 0, items = 0, splits = 0;
+    uint32_t wm = 0, tiles = 0, items = 0, splits = 0, parts = 0;
+    bool tc = false, alternate = false;  // the tcgen05 kernel
 };
 struct AttnPlan {
     bool shared = false;  // a pass of its own for the prefix
@@ -307,6 +309,20 @@ AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t row
     // cut the rows until the grid fills the GPU, but leave a part four tiles
     const uint64_t ctas = (uint64_t)p.items * kv_heads;
     p.splits = (uint32_t)std::min<uint64_t>({std::max<uint64_t>(1, want / ctas), std::max<uint32_t>(1, cdiv(rows, 4 * step)), 64});
+    p.parts = p.splits;
+    return p;
+}
+
+// The prefix on tcgen05: a tile of 128 vectors (two where there are more)
+// per CTA, one CTA per SM, the rows cut so that all SMs have one.
+AttnPass plan_tc(uint32_t vecs, uint32_t kv_heads, uint32_t rows) {
+    AttnPass p;
+    p.tc = true;
+    p.alternate = vecs <= 128;
+    p.tiles = p.items = cdiv(vecs, p.alternate ? 128 : 256);
+    const uint32_t ctas = p.items * kv_heads;
+    p.splits = std::min({std::max(1u, 148 / ctas), std::max(1u, cdiv(rows, 2 * TC_ROWS)), ATTN_MAX_PARTS / 2});
+    p.parts = p.alternate ? 2 * p.splits : p.splits;
     return p;
 }
 
@@ -332,9 +348,12 @@ AttnPlan plan_attn(const q_b200_attn_args* r) {
     // (from L2 after the first); it costs a join of at least two parts.
     p.shared = prefix >= 2 * step && r->n_seqs > 1;
     if (p.shared) {
-        p.pre = plan_pass(r->n_tokens * G, 1, r->kv.n_kv_heads, prefix, step, want);
+        const uint32_t vecs = r->n_tokens * G;
+        p.pre = r->kv.dtype != Q_B200_F32 && r->kv.head_dim >= 64 && r->scale > 0.0f && vecs > 32
+                    ? plan_tc(vecs, r->kv.n_kv_heads, prefix)
+                    : plan_pass(vecs, 1, r->kv.n_kv_heads, prefix, step, want);
         p.own = plan_pass(r->max_q * G, r->n_seqs, r->kv.n_kv_heads, std::max(1u, r->max_len), step, want);
-        p.parts = p.pre.splits + p.own.splits;
+        p.parts = p.pre.parts + p.own.parts;
     } else {
         p.own = plan_pass(r->max_q * G, r->n_seqs, r->kv.n_kv_heads, std::max(1u, prefix + r->max_len), step, want);
         p.parts = p.own.splits;
@@ -347,33 +366,48 @@ size_t attn_bytes(const q_b200_attn_args* r, const AttnPlan& p) {
 }
 
 template <typename T, int HD, int WM>
-cudaError_t launch_rows(const PrefixArgs& a, const AttnPass& p, uint32_t kv_heads, cudaStream_t st) {
+cudaError_t launch_rows(const PrefixArgs& a, const AttnPass& p, uint32_t kv_heads, bool pdl, cudaStream_t st) {
     const size_t smem = attn_rows_smem<T, HD, WM>();
     if (cudaError_t e = ensure_smem_attr((const void*)attn_rows_kernel<T, HD, WM>, (int)smem)) return e;
-    return launch_ex(attn_rows_kernel<T, HD, WM>, dim3(p.splits, p.items, kv_heads), dim3(ATTN_THREADS), smem, st, false, a);
+    return launch_ex(attn_rows_kernel<T, HD, WM>, dim3(p.splits, p.items, kv_heads), dim3(ATTN_THREADS), smem, st, pdl, a);
 }
 
 template <typename T, int HD>
-cudaError_t launch_pass(PrefixArgs a, const AttnPass& p, bool shared, uint32_t part0, uint32_t kv_heads, cudaStream_t st) {
-    a.shared = shared;
+cudaError_t launch_pass(PrefixArgs a, const AttnPass& p, uint32_t kv_heads, bool pdl, cudaStream_t st) {
     a.tiles = p.tiles;
     a.splits = p.splits;
-    a.part0 = part0;
-    if (p.wm == 1) return launch_rows<T, HD, 1>(a, p, kv_heads, st);
-    if (p.wm == 2) return launch_rows<T, HD, 2>(a, p, kv_heads, st);
-    return launch_rows<T, HD, 4>(a, p, kv_heads, st);
+    if constexpr (sizeof(T) == 2 && HD >= 64) {
+        if (p.tc) {
+            a.alternate = p.alternate;
+            if (cudaError_t e = ensure_smem_attr((const void*)attn_prefix_tc_kernel<T, HD>, (int)TcShape<HD>::SMEM)) return e;
+            return launch_ex(attn_prefix_tc_kernel<T, HD>, dim3(p.splits, p.items, kv_heads), dim3(TC_THREADS),
+                             TcShape<HD>::SMEM, st, pdl, a);
+        }
+    }
+    if (p.wm == 1) return launch_rows<T, HD, 1>(a, p, kv_heads, pdl, st);
+    if (p.wm == 2) return launch_rows<T, HD, 2>(a, p, kv_heads, pdl, st);
+    return launch_rows<T, HD, 4>(a, p, kv_heads, pdl, st);
 }
 
+// The prefix's pass, then the own rows' beside its tail (programmatic
+// dependent launch: a pass waits for the one before it only when its own
+// rows are done), which adds the prefix's parts itself unless its rows are
+// in parts too: then the join adds all of them.
 template <typename T, int HD>
 cudaError_t launch_attn(PrefixArgs& a, const AttnPlan& p, uint32_t kv_heads, cudaStream_t st) {
     cudaError_t e = cudaSuccess;
-    if (p.shared && (e = launch_pass<T, HD>(a, p.pre, true, 0, kv_heads, st))) return e;
+    if (p.shared) {
+        a.shared = 1;
+        if ((e = launch_pass<T, HD>(a, p.pre, kv_heads, false, st))) return e;
+    }
+    a.shared = 0;
     a.with_prefix = !p.shared;
-    const uint32_t part0 = p.parts == 1 ? ~0u : p.shared ? p.pre.splits : 0u;
-    if ((e = launch_pass<T, HD>(a, p.own, false, part0, kv_heads, st))) return e;
-    if (p.parts == 1) return e;
+    a.part0 = p.shared ? p.pre.parts : 0u;
+    a.last = p.own.splits == 1;
+    a.merge = a.last ? a.part0 : 0u;
+    if ((e = launch_pass<T, HD>(a, p.own, kv_heads, p.shared, st)) || a.last) return e;
     a.n_parts = p.parts;
-    return launch_ex(attn_join_kernel<T, HD>, dim3(cdiv((uint64_t)a.n_tokens * a.n_heads, 4)), dim3(128), 0, st, false, a);
+    return launch_ex(attn_join_kernel<T, HD>, dim3(cdiv((uint64_t)a.n_tokens * a.n_heads, 4)), dim3(128), 0, st, true, a);
 }
 
 template <typename T>

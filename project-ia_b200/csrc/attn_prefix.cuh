@@ -50,8 +50,11 @@ struct PrefixArgs {
     uint32_t max_q, max_len, max_prefix;
     uint32_t tiles;      // row tiles of an item (prefix: of all tokens; own: of one sequence)
     uint32_t splits;     // parts that an item's rows are cut into
-    uint32_t part0;      // this launch's first part; ~0: the only part, written to out
+    uint32_t part0;      // this launch's first part
+    uint32_t last;       // 1: writes out itself, after `merge` parts of the pass before it
+    uint32_t merge;
     uint32_t n_parts;    // of the join
+    uint32_t alternate;  // tcgen05 pass: one tile of vectors, even and odd row tiles
     uint32_t shared;     // 1: the prefix for all tokens; 0: per sequence
     uint32_t with_prefix;  // own pass: the prefix's rows come before the own ones
     float c;             // scale * log2(e)
@@ -72,11 +75,15 @@ struct AttnTraits<float> {
     static constexpr int KT = 32, STAGES = 3;
 };
 
-static constexpr uint32_t ATTN_THREADS = 128;
+static constexpr uint32_t ATTN_CONSUMERS = 128;  // four warps that multiply, one that copies
+static constexpr uint32_t ATTN_THREADS = 160;
+static constexpr uint32_t ATTN_MAX_PARTS = 128;
 
 template <typename T, int HD, int WM>
 constexpr size_t attn_rows_smem() {
-    return (size_t)AttnTraits<T>::STAGES * AttnTraits<T>::KT * HD * sizeof(T) * 2 + 16 * WM * HD * sizeof(T);
+    constexpr size_t ring = (size_t)AttnTraits<T>::STAGES * AttnTraits<T>::KT * HD * sizeof(T) * 2 + 16 * WM * HD * sizeof(T);
+    constexpr size_t join = 64 * (HD + 4 + 3) * 4 + 16 * WM * (2 + ATTN_MAX_PARTS + 1) * 4;
+    return ring > join ? ring : join;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -86,6 +93,24 @@ __device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commi
 template <int N>
 __device__ __forceinline__ void cp_async_wait() {
     asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// Arrives on `bar` once every copy that this thread has issued so far is done.
+__device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
+}
+// Barrier of the consumer warps alone.
+__device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+__device__ __forceinline__ bool consumers_or(bool v) {
+    uint32_t r;
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred.aligned q, 1, 128, p;\n\t"
+        "selp.u32 %0, 1, 0, q;\n\t}"
+        : "=r"(r)
+        : "r"((uint32_t)v)
+        : "memory");
+    return r != 0;
 }
 
 __device__ __forceinline__ void ldsm4(uint32_t addr, uint32_t (&r)[4]) {
@@ -267,20 +292,64 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
     constexpr int WN = 4 / WM, KW = KT / WN;       // groups of rows, rows of one warp in a tile
     constexpr int NT = KW / 8, ND = HD / 8;        // score and output tiles of 8 columns
     constexpr int CH = HD * (int)sizeof(T) / 16;   // 16-byte chunks of a row
-    constexpr int RP = ATTN_THREADS / CH;          // rows that one copy instruction of the CTA brings
+    constexpr int RP = 32 / CH;                    // rows that one copy instruction of the warp brings
     constexpr uint32_t TILE = KT * HD * sizeof(T);
     extern __shared__ __align__(128) uint8_t smem[];
+    __shared__ uint64_t full[ST], empty[ST];
     __shared__ bool s_bad[KT];
     const uint32_t s_kv = smem_u32(smem), s_q = s_kv + ST * 2 * TILE;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
     const uint32_t wm = warp % WM, wn = warp / WM;
     const uint32_t split = blockIdx.x, head = blockIdx.z;
 
+    if (a.shared) pdl_trigger();  // the pass over the own rows may start beside this one
     AttnItem w;
-    if (!attn_item(a, blockIdx.y, split, 16 * WM, KT, w)) return;
+    if (!attn_item(a, blockIdx.y, split, 16 * WM, KT, w)) {
+        pdl_wait();
+        return;
+    }
+    if (tid == 0) {
+        for (int i = 0; i < ST; ++i) {
+            mbar_init(&full[i], 32);
+            mbar_init(&empty[i], 4);
+        }
+        fence_mbar_init();
+    }
+    __syncthreads();
+    const uint32_t n_tiles = (w.r1 - w.r0 + KT - 1) / KT;
+    const T* kb = reinterpret_cast<const T*>(a.k);
+    const T* vb = reinterpret_cast<const T*>(a.v);
 
-    // the query vectors
-    for (uint32_t e = tid; e < 16 * WM * CH; e += ATTN_THREADS) {
+    if (warp == 4) {
+        // ---- producer: row offsets, one row (or two) of the tile per lane, then 16-byte copies ----
+        const uint32_t lr = lane / CH, lc = lane % CH;
+        for (uint32_t tile = 0; tile < n_tiles; ++tile) {
+            const uint32_t slot = tile % ST, st = s_kv + slot * 2 * TILE;
+            uint64_t off[KT / 32];
+#pragma unroll
+            for (int i = 0; i < KT / 32; ++i) {
+                const uint32_t row = w.r0 + tile * KT + i * 32 + lane;
+                if (!(row < w.r1 && attn_row(a, w, head, row, off[i]))) off[i] = ~0ull;  // zeros
+            }
+            if (tile >= ST && !__all_sync(0xffffffffu, mbar_wait(&empty[slot], (tile / ST - 1) & 1, QDEV_WAIT_EMPTY_TIMEOUT))) break;
+#pragma unroll
+            for (int p = 0; p < KT / RP; ++p) {
+                const uint32_t r = p * RP + lr;
+                const uint64_t o = __shfl_sync(0xffffffffu, off[p * RP / 32], r & 31);
+                const uint32_t n = o == ~0ull ? 0u : 16u;
+                const uint64_t at = (o == ~0ull ? 0ull : o) + lc * (16 / sizeof(T));
+                cp_async16(st + tile_off<T, HD>(r, lc), kb + at, n);
+                cp_async16(st + TILE + vt_off<T, HD>(r, lc), vb + at, n);
+            }
+            cp_async_arrive(&full[slot]);
+        }
+        cp_async_wait_all();
+        pdl_wait();
+        return;
+    }
+
+    // ---- consumers -------------------------------------------------------------------------------
+    for (uint32_t e = tid; e < 16 * WM * CH; e += ATTN_CONSUMERS) {
         const uint32_t r = e / CH, c = e % CH;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (r < w.n_vec) {
@@ -289,29 +358,7 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
         }
         *reinterpret_cast<uint4*>(smem + ST * 2 * TILE + tile_off<T, HD>(r, c)) = v;
     }
-
-    const uint32_t n_tiles = (w.r1 - w.r0 + KT - 1) / KT;
-    const T* kb = reinterpret_cast<const T*>(a.k);
-    const T* vb = reinterpret_cast<const T*>(a.v);
-    const uint32_t lr = tid / CH, lc = tid % CH;
-    auto issue = [&](uint32_t tile) {
-        if (tile < n_tiles) {
-            const uint32_t st = s_kv + (tile % ST) * 2 * TILE;
-#pragma unroll
-            for (int p = 0; p < KT / RP; ++p) {
-                const uint32_t r = p * RP + lr, row = w.r0 + tile * KT + r;
-                uint64_t off = 0;
-                const bool ok = row < w.r1 && attn_row(a, w, head, row, off);
-                const uint32_t n = ok ? 16u : 0u;  // nothing read, zeros written
-                cp_async16(st + tile_off<T, HD>(r, lc), kb + off + lc * (16 / sizeof(T)), n);
-                cp_async16(st + TILE + (F32 ? v32_off<HD>(r, lc) : tile_off<T, HD>(r, lc)), vb + off + lc * (16 / sizeof(T)), n);
-            }
-        }
-        cp_async_commit();
-    };
-#pragma unroll
-    for (int s = 0; s < ST - 1; ++s) issue(s);
-    __syncthreads();
+    consumers_sync();
 
     uint32_t qf[F32 ? 1 : HD / 16][4];
     if constexpr (!F32) {
@@ -334,10 +381,10 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
 #pragma unroll
     for (int n = 0; n < ND; ++n) o[n][0] = o[n][1] = o[n][2] = o[n][3] = 0.0f;
 
+    bool alive = true;
     for (uint32_t tile = 0; tile < n_tiles; ++tile) {
-        cp_async_wait<ST - 2>();
-        __syncthreads();
-        issue(tile + ST - 1);
+        // after a wait that ran out the others are not tried: every warp still meets every barrier
+        if (alive) alive = __all_sync(0xffffffffu, mbar_wait(&full[tile % ST], (tile / ST) & 1, QDEV_WAIT_FULL_TIMEOUT));
         const uint32_t sk = s_kv + (tile % ST) * 2 * TILE, sv = sk + TILE;
         const uint32_t first = w.r0 + tile * KT;  // row of the tile's key 0
 
@@ -440,19 +487,19 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
         const uint32_t hid0 = max((int32_t)first, w.see0), hid1 = min(first + KT, w.r1);
         bool bad = false;
         if (w.n_tok > 1 && !a.shared && hid0 < hid1) {
-            for (uint32_t e = tid + (hid0 - first) * CH; e < (hid1 - first) * CH; e += ATTN_THREADS)
+            for (uint32_t e = tid + (hid0 - first) * CH; e < (hid1 - first) * CH; e += ATTN_CONSUMERS)
                 bad |= !finite16<T>(sv + vt_off<T, HD>(e / CH, e % CH));
-            bad = __syncthreads_or(bad);
+            bad = consumers_or(bad);
             if (bad) {
                 if (tid < KT) s_bad[tid] = false;
-                __syncthreads();
-                for (uint32_t e = tid + (hid0 - first) * CH; e < (hid1 - first) * CH; e += ATTN_THREADS)
+                consumers_sync();
+                for (uint32_t e = tid + (hid0 - first) * CH; e < (hid1 - first) * CH; e += ATTN_CONSUMERS)
                     if (!finite16<T>(sv + vt_off<T, HD>(e / CH, e % CH))) s_bad[e / CH] = true;
-                __syncthreads();
-                for (uint32_t e = tid + (hid0 - first) * CH; e < (hid1 - first) * CH; e += ATTN_THREADS)
+                consumers_sync();
+                for (uint32_t e = tid + (hid0 - first) * CH; e < (hid1 - first) * CH; e += ATTN_CONSUMERS)
                     if (s_bad[e / CH])
                         asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(sv + vt_off<T, HD>(e / CH, e % CH)), "r"(0) : "memory");
-                __syncthreads();
+                consumers_sync();
             }
         }
 
@@ -507,6 +554,8 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
                 for (int i = 0; i < 4; ++i) o[n][i] = fmaf(o[n][i], corr[i >> 1], hh[i] + ll[i]);
             }
         }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[tile % ST]);
         if (bad) {
             for (uint32_t r = max(hid0 - first, wn * KW); r < min(hid1 - first, (wn + 1) * KW); ++r) {
                 uint64_t off;
@@ -529,87 +578,123 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
             }
         }
     }
-    cp_async_wait<0>();
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
         l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
     }
-    __syncthreads();
+    consumers_sync();
 
-    // ---- join the groups of rows, then this part's result -----------------------------------
-    float* s_o = reinterpret_cast<float*>(smem);                 // [16 WM][HD + 4]
-    float* s_ml = s_o + 16 * WM * (HD + 4);                      // [WN][16 WM][2]
+    // ---- join the groups of rows: each warp leaves its (m, l, o), then all are added in order ------
+    constexpr int RV = 16 * WM, OP = HD + 4;
+    float* s_o = reinterpret_cast<float*>(smem);     // [WN][RV][OP]
+    float* s_ml = s_o + WN * RV * OP;                // [WN][RV][2]
+    float* s_w = s_ml + WN * RV * 2;                 // [RV][WN]: weight of each warp's share
+    float* s_res = s_w + WN * RV;                    // [RV][2]: joined (m, l)
     const uint32_t v0 = wm * 16 + g;
-    if (WN > 1) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
         if (t == 0) {
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                s_ml[(wn * 16 * WM + v0 + 8 * h) * 2] = m[h];
-                s_ml[(wn * 16 * WM + v0 + 8 * h) * 2 + 1] = l[h];
-            }
+            s_ml[(wn * RV + v0 + 8 * h) * 2] = m[h];
+            s_ml[(wn * RV + v0 + 8 * h) * 2 + 1] = l[h];
         }
-        __syncthreads();
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            float M = -INFINITY, Lsum = 0.0f;
-#pragma unroll
-            for (int k = 0; k < WN; ++k) M = fmaxf(M, s_ml[(k * 16 * WM + v0 + 8 * h) * 2]);
-#pragma unroll
-            for (int k = 0; k < WN; ++k) {
-                const float mk = s_ml[(k * 16 * WM + v0 + 8 * h) * 2], lk = s_ml[(k * 16 * WM + v0 + 8 * h) * 2 + 1];
-                Lsum += mk == -INFINITY ? lk : lk * exp2f(mk - M);
-            }
-            const float f = m[h] == -INFINITY ? 1.0f : exp2f(m[h] - M);
-#pragma unroll
-            for (int n = 0; n < ND; ++n) {
-                o[n][2 * h] *= f;
-                o[n][2 * h + 1] *= f;
-            }
-            m[h] = M;
-            l[h] = Lsum;
-        }
-    }
-    for (int k = 0; k < WN; ++k) {
-        if ((int)wn == k) {
+        if (v0 + 8 * h < w.n_vec) {
 #pragma unroll
             for (int n = 0; n < ND; ++n)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    float2* d = reinterpret_cast<float2*>(s_o + (v0 + 8 * h) * (HD + 4) + n * 8 + 2 * t);
-                    float2 x = make_float2(o[n][2 * h], o[n][2 * h + 1]);
-                    if (k > 0) {
-                        x.x += d->x;
-                        x.y += d->y;
-                    }
-                    *d = x;
-                }
-        }
-        __syncthreads();
-    }
-    if (wn == 0 && t == 0) {
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            s_ml[(v0 + 8 * h) * 2] = m[h];
-            s_ml[(v0 + 8 * h) * 2 + 1] = l[h];
+                *reinterpret_cast<float2*>(s_o + (wn * RV + v0 + 8 * h) * OP + n * 8 + 2 * t) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
         }
     }
-    __syncthreads();
-    for (uint32_t e = tid; e < w.n_vec * (HD / 4); e += ATTN_THREADS) {
+    consumers_sync();
+    if (tid < RV) {
+        float M = -INFINITY, L = 0.0f;
+#pragma unroll
+        for (int k = 0; k < WN; ++k) M = fmaxf(M, s_ml[(k * RV + tid) * 2]);
+#pragma unroll
+        for (int k = 0; k < WN; ++k) {
+            const float mk = s_ml[(k * RV + tid) * 2], f = mk == -INFINITY ? 1.0f : exp2f(mk - M);
+            s_w[tid * WN + k] = f;  // 1 where there is nothing, or a NaN, to add
+            L += s_ml[(k * RV + tid) * 2 + 1] * f;
+        }
+        s_res[tid * 2] = M;
+        s_res[tid * 2 + 1] = L;
+    }
+    consumers_sync();
+    pdl_wait();  // what an earlier pass left is complete
+
+    // with the prefix's parts behind it this is the last pass: their weights go to shared memory
+    float* s_f = s_res + RV * 2;  // [RV][parts + 1], the own share's weight last
+    if (a.merge) {
+        const uint64_t stride = (uint64_t)a.n_tokens * a.n_heads;
+        for (uint32_t r = warp; r < w.n_vec; r += 4) {
+            const uint32_t i = fast_div(w.vec0 + r, a.by_group), h = head * a.group + (w.vec0 + r - i * a.group);
+            const uint64_t id = (uint64_t)(w.tok0 + i) * a.n_heads + h;
+            float pm[ATTN_MAX_PARTS / 32], pl[ATTN_MAX_PARTS / 32], M = s_res[r * 2];
+#pragma unroll
+            for (int k = 0; k < (int)ATTN_MAX_PARTS / 32; ++k) {
+                const uint32_t p = k * 32 + lane;
+                const float2 ml = p < a.merge ? __ldcg(a.part_ml + p * stride + id) : make_float2(-INFINITY, 0.0f);
+                pm[k] = ml.x;
+                pl[k] = ml.y;
+                M = fmaxf(M, ml.x);
+            }
+            M = warp_max(M);
+            const float own = s_res[r * 2] == -INFINITY ? 1.0f : exp2f(s_res[r * 2] - M);
+            float L = 0.0f;
+#pragma unroll
+            for (int k = 0; k < (int)ATTN_MAX_PARTS / 32; ++k) {
+                const uint32_t p = k * 32 + lane;
+                const float f = pm[k] == -INFINITY ? 1.0f : exp2f(pm[k] - M);
+                if (p < a.merge) s_f[r * (a.merge + 1) + p] = f;
+                L += pl[k] * f;
+            }
+            L = warp_sum(L) + s_res[r * 2 + 1] * own;
+            __syncwarp();
+            if (lane == 0) {
+                s_f[r * (a.merge + 1) + a.merge] = own;
+                s_res[r * 2 + 1] = L;
+            }
+        }
+        consumers_sync();
+    }
+    for (uint32_t e = tid; e < w.n_vec * (HD / 4); e += ATTN_CONSUMERS) {
         const uint32_t r = e / (HD / 4), c = e % (HD / 4);
         const uint32_t i = fast_div(w.vec0 + r, a.by_group), h = head * a.group + (w.vec0 + r - i * a.group);
         const uint64_t tok = w.tok0 + i;
-        float4 x = *reinterpret_cast<const float4*>(s_o + r * (HD + 4) + c * 4);
-        const float pm = s_ml[r * 2], pl = s_ml[r * 2 + 1];
-        if (a.part0 == ~0u) {
-            const float inv = pl == 0.0f ? 0.0f : 1.0f / pl;
+        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+        for (int k = 0; k < WN; ++k) {
+            const float4 y = *reinterpret_cast<const float4*>(s_o + (k * RV + r) * OP + c * 4);
+            const float f = s_w[r * WN + k];
+            x.x = fmaf(y.x, f, x.x);
+            x.y = fmaf(y.y, f, x.y);
+            x.z = fmaf(y.z, f, x.z);
+            x.w = fmaf(y.w, f, x.w);
+        }
+        const float L = s_res[r * 2 + 1];
+        if (a.last) {
+            if (a.merge) {
+                const uint64_t stride = (uint64_t)a.n_tokens * a.n_heads * (HD / 4);
+                const float4* po = reinterpret_cast<const float4*>(a.part_o) + (tok * a.n_heads + h) * (HD / 4) + c;
+                const float* f = s_f + r * (a.merge + 1);
+                const float own = f[a.merge];
+                x = make_float4(x.x * own, x.y * own, x.z * own, x.w * own);
+#pragma unroll 4
+                for (uint32_t p = 0; p < a.merge; ++p) {
+                    const float4 y = __ldcg(po + p * stride);
+                    x.x = fmaf(y.x, f[p], x.x);
+                    x.y = fmaf(y.y, f[p], x.y);
+                    x.z = fmaf(y.z, f[p], x.z);
+                    x.w = fmaf(y.w, f[p], x.w);
+                }
+            }
+            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
             float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
-            if (pl == 0.0f) y[0] = y[1] = y[2] = y[3] = 0.0f;
+            if (L == 0.0f) y[0] = y[1] = y[2] = y[3] = 0.0f;
             store_vec<T, 4>(reinterpret_cast<T*>(a.out) + tok * a.o_token + h * a.o_head + c * 4, y);
         } else {
             const uint64_t at = ((uint64_t)(a.part0 + split) * a.n_tokens + tok) * a.n_heads + h;
-            reinterpret_cast<float4*>(a.part_o + at * HD)[c] = x;
-            if (c == 0) a.part_ml[at] = make_float2(pm, pl);
+            __stcg(reinterpret_cast<float4*>(a.part_o + at * HD) + c, x);
+            if (c == 0) __stcg(a.part_ml + at, make_float2(s_res[r * 2], L));
         }
     }
 }
@@ -618,23 +703,24 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ PrefixArgs a) {
     const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    pdl_wait();
     if (id >= a.n_tokens * a.n_heads) return;
     const uint32_t tok = id / a.n_heads, h = id - tok * a.n_heads;
     if (a.q_start && (tok < __ldg(a.q_start) || tok >= __ldg(a.q_start + a.n_seqs))) return;  // no sequence's token
     const uint64_t stride = (uint64_t)a.n_tokens * a.n_heads;
     float M = -INFINITY;
-    for (uint32_t p = lane; p < a.n_parts; p += 32) M = fmaxf(M, a.part_ml[p * stride + id].x);
+    for (uint32_t p = lane; p < a.n_parts; p += 32) M = fmaxf(M, __ldcg(a.part_ml + p * stride + id).x);
     M = warp_max(M);
     float L = 0.0f, o[HD / 32];
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) o[i] = 0.0f;
     for (uint32_t p = 0; p < a.n_parts; ++p) {
-        const float2 ml = a.part_ml[p * stride + id];
+        const float2 ml = __ldcg(a.part_ml + p * stride + id);
         if (ml.y == 0.0f) continue;  // no row of this part is seen (a NaN sum is)
         const float f = ml.x == -INFINITY ? 1.0f : exp2f(ml.x - M);
         L += ml.y * f;
 #pragma unroll
-        for (int i = 0; i < HD / 32; ++i) o[i] = fmaf(a.part_o[(p * stride + id) * HD + i * 32 + lane], f, o[i]);
+        for (int i = 0; i < HD / 32; ++i) o[i] = fmaf(__ldcg(a.part_o + (p * stride + id) * HD + i * 32 + lane), f, o[i]);
     }
     const float inv = L == 0.0f ? 0.0f : 1.0f / L;
 #pragma unroll
