@@ -5,6 +5,7 @@
 // no device come first, so that a refusal is the same with and without one.
 #include <cmath>
 
+#include "attn_few.cuh"
 #include "attn_prefix.cuh"
 #include "attn_prefix_tc.cuh"
 #include "runtime.cuh"
@@ -286,30 +287,44 @@ q_error_code q_b200_kv_append(const q_b200_append_args* r, void* stream) {
 
 namespace {
 
+enum AttnKernel { ATTN_FEW, ATTN_ROWS, ATTN_TC };
 struct AttnPass {
-    uint32_t wm = 0, tiles = 0, items = 0, splits = 0, parts = 0;
-    bool tc = false, alternate = false;  // the tcgen05 kernel
+    AttnKernel kern = ATTN_FEW;
+    uint32_t mb = 1;                 // FEW: blocks of 16 vectors
+    uint32_t tiles = 0, items = 0, splits = 1, parts = 1;
+    bool cluster = false;            // FEW: the splits join within a cluster
+    bool alternate = false;          // TC: one tile of vectors
 };
 struct AttnPlan {
     bool shared = false;  // a pass of its own for the prefix
     AttnPass pre, own;
-    uint32_t parts = 1;   // 1: written to out directly
+    uint32_t parts = 0;   // partial results in the workspace
 };
 
 uint32_t cdiv(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
-// Vectors of a CTA: 16, 32 or 64, the fewest that hold all of an item's.
-uint32_t groups_of(uint32_t vecs) { return vecs <= 16 ? 1 : vecs <= 32 ? 2 : 4; }
-
-AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t rows, uint32_t step, uint32_t want) {
+// A pass of attn_few_kernel (up to 32 vectors) or attn_rows_kernel: the rows
+// are cut until about two CTAs per SM have work, each with at least two
+// tiles.  Up to 8 cuts of the own rows are one cluster's and leave nothing
+// in the workspace.
+AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t rows, uint32_t step, bool own) {
     AttnPass p;
-    p.wm = groups_of(vecs);
-    p.tiles = cdiv(vecs, 16 * p.wm);
+    p.kern = vecs <= 32 ? ATTN_FEW : ATTN_ROWS;
+    p.mb = vecs <= 16 ? 1 : 2;
+    p.tiles = cdiv(vecs, p.kern == ATTN_FEW ? 16 * p.mb : 64);
     p.items = p.tiles * seqs;
-    // cut the rows until the grid fills the GPU, but leave a part four tiles
     const uint64_t ctas = (uint64_t)p.items * kv_heads;
-    p.splits = (uint32_t)std::min<uint64_t>({std::max<uint64_t>(1, want / ctas), std::max<uint32_t>(1, cdiv(rows, 4 * step)), 64});
-    p.parts = p.splits;
+    const uint32_t most = std::max(1u, cdiv(rows, 2 * step));
+    p.splits = (uint32_t)std::min<uint64_t>({std::max<uint64_t>(1, 2 * 148 / ctas), most, 64});
+    if (p.kern == ATTN_FEW && own && p.splits > 1) {
+        p.cluster = p.splits <= 8 || rows <= 8 * 4 * step;
+        if (p.cluster) {
+            uint32_t c = 1;
+            while (c * 2 <= std::min(p.splits, 8u)) c *= 2;
+            p.splits = c;
+        }
+    }
+    p.parts = own && (p.cluster || p.splits == 1) ? 0 : p.splits;
     return p;
 }
 
@@ -317,7 +332,7 @@ AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t row
 // per CTA, one CTA per SM, the rows cut so that all SMs have one.
 AttnPass plan_tc(uint32_t vecs, uint32_t kv_heads, uint32_t rows) {
     AttnPass p;
-    p.tc = true;
+    p.kern = ATTN_TC;
     p.alternate = vecs <= 128;
     p.tiles = p.items = cdiv(vecs, p.alternate ? 128 : 256);
     const uint32_t ctas = p.items * kv_heads;
@@ -343,33 +358,53 @@ q_error_code check_attn(const q_b200_attn_args* r) {
 AttnPlan plan_attn(const q_b200_attn_args* r) {
     const uint32_t G = r->n_heads / r->kv.n_kv_heads, step = r->kv.dtype == Q_B200_F32 ? 32 : 64;
     AttnPlan p;
-    const uint32_t prefix = r->max_prefix, want = 2 * 148;
+    const uint32_t prefix = r->max_prefix;
     // A pass of its own reads the prefix once instead of once per sequence
-    // (from L2 after the first); it costs a join of at least two parts.
+    // (from L2 after the first); it costs a launch and its parts.
     p.shared = prefix >= 2 * step && r->n_seqs > 1;
     if (p.shared) {
         const uint32_t vecs = r->n_tokens * G;
         p.pre = r->kv.dtype != Q_B200_F32 && r->kv.head_dim >= 64 && r->scale > 0.0f && vecs > 32
                     ? plan_tc(vecs, r->kv.n_kv_heads, prefix)
-                    : plan_pass(vecs, 1, r->kv.n_kv_heads, prefix, step, want);
-        p.own = plan_pass(r->max_q * G, r->n_seqs, r->kv.n_kv_heads, std::max(1u, r->max_len), step, want);
-        p.parts = p.pre.parts + p.own.parts;
-    } else {
-        p.own = plan_pass(r->max_q * G, r->n_seqs, r->kv.n_kv_heads, std::max(1u, prefix + r->max_len), step, want);
-        p.parts = p.own.splits;
+                    : plan_pass(vecs, 1, r->kv.n_kv_heads, prefix, step, false);
     }
+    p.own = plan_pass(r->max_q * G, r->n_seqs, r->kv.n_kv_heads, std::max(1u, r->max_len + (p.shared ? 0 : prefix)), step, true);
+    p.parts = (p.shared ? p.pre.parts : 0) + p.own.parts;
     return p;
 }
 
 size_t attn_bytes(const q_b200_attn_args* r, const AttnPlan& p) {
-    return p.parts == 1 ? 0 : (size_t)p.parts * r->n_tokens * r->n_heads * (r->kv.head_dim * 4 + 8);
+    return (size_t)p.parts * r->n_tokens * r->n_heads * (r->kv.head_dim * 4 + 8);
 }
 
-template <typename T, int HD, int WM>
-cudaError_t launch_rows(const PrefixArgs& a, const AttnPass& p, uint32_t kv_heads, bool pdl, cudaStream_t st) {
-    const size_t smem = attn_rows_smem<T, HD, WM>();
-    if (cudaError_t e = ensure_smem_attr((const void*)attn_rows_kernel<T, HD, WM>, (int)smem)) return e;
-    return launch_ex(attn_rows_kernel<T, HD, WM>, dim3(p.splits, p.items, kv_heads), dim3(ATTN_THREADS), smem, st, pdl, a);
+template <typename T, int HD, int MB>
+cudaError_t launch_few(PrefixArgs& a, const AttnPass& p, uint32_t kv_heads, bool pdl, cudaStream_t st) {
+    using S = FewShape<T, HD>;
+    constexpr uint32_t smem = S::smem(MB);
+    if (cudaError_t e = ensure_smem_attr((const void*)attn_few_kernel<T, HD, MB>, smem)) return e;
+    a.cluster = p.cluster;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(p.splits, p.items, kv_heads);
+    cfg.blockDim = dim3(FEW_THREADS);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cudaLaunchAttribute attr[2];
+    uint32_t n = 0;
+    if (p.cluster) {
+        attr[n].id = cudaLaunchAttributeClusterDimension;
+        attr[n].val.clusterDim.x = p.splits;
+        attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
+        ++n;
+    }
+    if (pdl) {
+        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+        attr[n].val.programmaticStreamSerializationAllowed = 1;
+        ++n;
+    }
+    cfg.attrs = attr;
+    cfg.numAttrs = n;
+    g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
+    return cudaLaunchKernelEx(&cfg, attn_few_kernel<T, HD, MB>, a);
 }
 
 template <typename T, int HD>
@@ -377,16 +412,18 @@ cudaError_t launch_pass(PrefixArgs a, const AttnPass& p, uint32_t kv_heads, bool
     a.tiles = p.tiles;
     a.splits = p.splits;
     if constexpr (sizeof(T) == 2 && HD >= 64) {
-        if (p.tc) {
+        if (p.kern == ATTN_TC) {
             a.alternate = p.alternate;
             if (cudaError_t e = ensure_smem_attr((const void*)attn_prefix_tc_kernel<T, HD>, (int)TcShape<HD>::SMEM)) return e;
             return launch_ex(attn_prefix_tc_kernel<T, HD>, dim3(p.splits, p.items, kv_heads), dim3(TC_THREADS),
                              TcShape<HD>::SMEM, st, pdl, a);
         }
     }
-    if (p.wm == 1) return launch_rows<T, HD, 1>(a, p, kv_heads, pdl, st);
-    if (p.wm == 2) return launch_rows<T, HD, 2>(a, p, kv_heads, pdl, st);
-    return launch_rows<T, HD, 4>(a, p, kv_heads, pdl, st);
+    if (p.kern == ATTN_FEW)
+        return p.mb == 1 ? launch_few<T, HD, 1>(a, p, kv_heads, pdl, st) : launch_few<T, HD, 2>(a, p, kv_heads, pdl, st);
+    const size_t smem = attn_rows_smem<T, HD, 4>();
+    if (cudaError_t e = ensure_smem_attr((const void*)attn_rows_kernel<T, HD, 4>, (int)smem)) return e;
+    return launch_ex(attn_rows_kernel<T, HD, 4>, dim3(p.splits, p.items, kv_heads), dim3(ATTN_THREADS), smem, st, pdl, a);
 }
 
 // The prefix's pass, then the own rows' beside its tail (programmatic
@@ -403,11 +440,11 @@ cudaError_t launch_attn(PrefixArgs& a, const AttnPlan& p, uint32_t kv_heads, cud
     a.shared = 0;
     a.with_prefix = !p.shared;
     a.part0 = p.shared ? p.pre.parts : 0u;
-    a.last = p.own.splits == 1;
+    a.last = p.own.parts == 0;
     a.merge = a.last ? a.part0 : 0u;
     if ((e = launch_pass<T, HD>(a, p.own, kv_heads, p.shared, st)) || a.last) return e;
     a.n_parts = p.parts;
-    return launch_ex(attn_join_kernel<T, HD>, dim3(cdiv((uint64_t)a.n_tokens * a.n_heads, 4)), dim3(128), 0, st, true, a);
+    return launch_ex(attn_join_kernel<T, HD>, dim3(cdiv((uint64_t)a.n_tokens * a.n_heads * (HD / 4), 128)), dim3(128), 0, st, true, a);
 }
 
 template <typename T>

@@ -54,6 +54,7 @@ struct PrefixArgs {
     uint32_t last;       // 1: writes out itself, after `merge` parts of the pass before it
     uint32_t merge;
     uint32_t n_parts;    // of the join
+    uint32_t cluster;    // attn_few_kernel: the splits are a cluster's
     uint32_t alternate;  // tcgen05 pass: one tile of vectors, even and odd row tiles
     uint32_t shared;     // 1: the prefix for all tokens; 0: per sequence
     uint32_t with_prefix;  // own pass: the prefix's rows come before the own ones
@@ -82,7 +83,7 @@ static constexpr uint32_t ATTN_MAX_PARTS = 128;
 template <typename T, int HD, int WM>
 constexpr size_t attn_rows_smem() {
     constexpr size_t ring = (size_t)AttnTraits<T>::STAGES * AttnTraits<T>::KT * HD * sizeof(T) * 2 + 16 * WM * HD * sizeof(T);
-    constexpr size_t join = 64 * (HD + 4 + 3) * 4 + 16 * WM * (2 + ATTN_MAX_PARTS + 1) * 4;
+    constexpr size_t join = 64 * (HD + 4 + 3) * 4 + 16 * WM * 2 * 4;
     return ring > join ? ring : join;
 }
 
@@ -271,19 +272,84 @@ __device__ __forceinline__ bool attn_item(const PrefixArgs& a, uint32_t item, ui
     return true;
 }
 
-// Offset of row r of the item (elements); false where its page is not one.
-__device__ __forceinline__ bool attn_row(const PrefixArgs& a, const AttnItem& w, uint32_t head, uint32_t r, uint64_t& off) {
+// The page that row r of the item lies in, as the table has it.
+__device__ __forceinline__ uint32_t attn_page(const PrefixArgs& a, const AttnItem& w, uint32_t r) {
     const bool pre = r < w.n_prefix;
-    const uint32_t i = pre ? r : r - w.n_prefix, pi = fast_div(i, a.page_rows);
-    const uint32_t pg = __ldg(pre ? a.prefix_pages + pi : a.pages + (size_t)w.seq * a.pages_per_seq + pi);
-    if (pg >= a.n_pages) {
-        qdev_fail(QDEV_BAD_ARG);
-        off = 0;
-        return false;
-    }
-    off = pg * a.page_stride + head * a.head_stride + (uint64_t)(i - pi * a.page_rows.d) * a.row_stride;
-    return true;
+    const uint32_t pi = fast_div(pre ? r : r - w.n_prefix, a.page_rows);
+    return __ldg(pre ? a.prefix_pages + pi : a.pages + (size_t)w.seq * a.pages_per_seq + pi);
 }
+// Offset of row r in its page (elements); ~0 where the page is not one.
+__device__ __forceinline__ uint64_t attn_offset(const PrefixArgs& a, const AttnItem& w, uint32_t head, uint32_t r, uint32_t page) {
+    if (page >= a.n_pages) {
+        qdev_fail(QDEV_BAD_ARG);
+        return ~0ull;
+    }
+    const uint32_t i = r < w.n_prefix ? r : r - w.n_prefix;
+    return page * a.page_stride + head * a.head_stride + (uint64_t)(i - fast_div(i, a.page_rows) * a.page_rows.d) * a.row_stride;
+}
+__device__ __forceinline__ bool attn_row(const PrefixArgs& a, const AttnItem& w, uint32_t head, uint32_t r, uint64_t& off) {
+    off = attn_offset(a, w, head, r, attn_page(a, w, r));
+    return off != ~0ull;
+}
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// Sum of parts (m, l, o) for four outputs of a vector.
+template <int HD>
+struct PartSum {
+    float M = -INFINITY, L = 0.0f;
+    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+    // Weights 2^(m - M); a part without a row (m = -inf, l = 0, o = 0) or
+    // with NaN sums is added as it is.
+    template <int N>
+    __device__ __forceinline__ void add(const float2 (&ml)[N], const float4 (&y)[N]) {
+        float top = M;
+#pragma unroll
+        for (int k = 0; k < N; ++k) top = fmaxf(top, ml[k].x);
+        const float f0 = M == top ? 1.0f : ex2(M - top);
+        M = top;
+        L *= f0;
+        x = make_float4(x.x * f0, x.y * f0, x.z * f0, x.w * f0);
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+            const float f = ml[k].x == top ? 1.0f : ex2(ml[k].x - top);
+            L = fmaf(ml[k].y, f, L);
+            x.x = fmaf(y[k].x, f, x.x);
+            x.y = fmaf(y[k].y, f, x.y);
+            x.z = fmaf(y[k].z, f, x.z);
+            x.w = fmaf(y[k].w, f, x.w);
+        }
+    }
+    // The workspace's first n parts of (token, head) id, twelve loads of each
+    // kind under way at once.
+    __device__ __forceinline__ void add_parts(const PrefixArgs& a, uint64_t id, uint32_t c, uint32_t n) {
+        constexpr int N = 12;
+        const uint64_t stride = (uint64_t)a.n_tokens * a.n_heads;
+        const float4* po = reinterpret_cast<const float4*>(a.part_o) + id * (HD / 4) + c;
+        for (uint32_t p = 0; p < n; p += N) {
+            float2 ml[N];
+            float4 y[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) {
+                const bool in = p + k < n;
+                ml[k] = in ? __ldcg(a.part_ml + (p + k) * stride + id) : make_float2(-INFINITY, 0.0f);
+                y[k] = in ? __ldcg(po + (p + k) * stride * (HD / 4)) : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+            }
+            add<N>(ml, y);
+        }
+    }
+    template <typename T>
+    __device__ __forceinline__ void store(const PrefixArgs& a, uint64_t tok, uint32_t h, uint32_t c) {
+        const float inv = L == 0.0f ? 0.0f : 1.0f / L;
+        float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
+        if (L == 0.0f) y[0] = y[1] = y[2] = y[3] = 0.0f;  // no row is seen
+        store_vec<T, 4>(reinterpret_cast<T*>(a.out) + tok * a.o_token + (uint64_t)h * a.o_head + c * 4, y);
+    }
+};
 
 template <typename T, int HD, int WM>
 __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_constant__ PrefixArgs a) {
@@ -621,41 +687,6 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
     consumers_sync();
     pdl_wait();  // what an earlier pass left is complete
 
-    // with the prefix's parts behind it this is the last pass: their weights go to shared memory
-    float* s_f = s_res + RV * 2;  // [RV][parts + 1], the own share's weight last
-    if (a.merge) {
-        const uint64_t stride = (uint64_t)a.n_tokens * a.n_heads;
-        for (uint32_t r = warp; r < w.n_vec; r += 4) {
-            const uint32_t i = fast_div(w.vec0 + r, a.by_group), h = head * a.group + (w.vec0 + r - i * a.group);
-            const uint64_t id = (uint64_t)(w.tok0 + i) * a.n_heads + h;
-            float pm[ATTN_MAX_PARTS / 32], pl[ATTN_MAX_PARTS / 32], M = s_res[r * 2];
-#pragma unroll
-            for (int k = 0; k < (int)ATTN_MAX_PARTS / 32; ++k) {
-                const uint32_t p = k * 32 + lane;
-                const float2 ml = p < a.merge ? __ldcg(a.part_ml + p * stride + id) : make_float2(-INFINITY, 0.0f);
-                pm[k] = ml.x;
-                pl[k] = ml.y;
-                M = fmaxf(M, ml.x);
-            }
-            M = warp_max(M);
-            const float own = s_res[r * 2] == -INFINITY ? 1.0f : exp2f(s_res[r * 2] - M);
-            float L = 0.0f;
-#pragma unroll
-            for (int k = 0; k < (int)ATTN_MAX_PARTS / 32; ++k) {
-                const uint32_t p = k * 32 + lane;
-                const float f = pm[k] == -INFINITY ? 1.0f : exp2f(pm[k] - M);
-                if (p < a.merge) s_f[r * (a.merge + 1) + p] = f;
-                L += pl[k] * f;
-            }
-            L = warp_sum(L) + s_res[r * 2 + 1] * own;
-            __syncwarp();
-            if (lane == 0) {
-                s_f[r * (a.merge + 1) + a.merge] = own;
-                s_res[r * 2 + 1] = L;
-            }
-        }
-        consumers_sync();
-    }
     for (uint32_t e = tid; e < w.n_vec * (HD / 4); e += ATTN_CONSUMERS) {
         const uint32_t r = e / (HD / 4), c = e % (HD / 4);
         const uint32_t i = fast_div(w.vec0 + r, a.by_group), h = head * a.group + (w.vec0 + r - i * a.group);
@@ -672,25 +703,12 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
         }
         const float L = s_res[r * 2 + 1];
         if (a.last) {
-            if (a.merge) {
-                const uint64_t stride = (uint64_t)a.n_tokens * a.n_heads * (HD / 4);
-                const float4* po = reinterpret_cast<const float4*>(a.part_o) + (tok * a.n_heads + h) * (HD / 4) + c;
-                const float* f = s_f + r * (a.merge + 1);
-                const float own = f[a.merge];
-                x = make_float4(x.x * own, x.y * own, x.z * own, x.w * own);
-#pragma unroll 4
-                for (uint32_t p = 0; p < a.merge; ++p) {
-                    const float4 y = __ldcg(po + p * stride);
-                    x.x = fmaf(y.x, f[p], x.x);
-                    x.y = fmaf(y.y, f[p], x.y);
-                    x.z = fmaf(y.z, f[p], x.z);
-                    x.w = fmaf(y.w, f[p], x.w);
-                }
-            }
-            const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-            float y[4] = {x.x * inv, x.y * inv, x.z * inv, x.w * inv};
-            if (L == 0.0f) y[0] = y[1] = y[2] = y[3] = 0.0f;
-            store_vec<T, 4>(reinterpret_cast<T*>(a.out) + tok * a.o_token + h * a.o_head + c * 4, y);
+            PartSum<HD> sum;
+            if (a.merge) sum.add_parts(a, tok * a.n_heads + h, c, a.merge);
+            const float2 ml[1] = {make_float2(s_res[r * 2], L)};
+            const float4 y[1] = {x};
+            sum.template add<1>(ml, y);
+            sum.template store<T>(a, tok, h, c);
         } else {
             const uint64_t at = ((uint64_t)(a.part0 + split) * a.n_tokens + tok) * a.n_heads + h;
             __stcg(reinterpret_cast<float4*>(a.part_o + at * HD) + c, x);
@@ -699,35 +717,18 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
     }
 }
 
-// One warp adds the parts of one (token, head), in part order.
+// A thread adds the parts of four outputs of one (token, head), in part order.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ PrefixArgs a) {
-    const uint32_t id = blockIdx.x * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31;
+    const uint64_t e = (uint64_t)blockIdx.x * 128 + threadIdx.x, stride = (uint64_t)a.n_tokens * a.n_heads;
     pdl_wait();
-    if (id >= a.n_tokens * a.n_heads) return;
-    const uint32_t tok = id / a.n_heads, h = id - tok * a.n_heads;
+    const uint64_t id = e / (HD / 4);
+    if (id >= stride) return;
+    const uint32_t c = (uint32_t)(e % (HD / 4)), tok = (uint32_t)(id / a.n_heads), h = (uint32_t)(id - (uint64_t)tok * a.n_heads);
     if (a.q_start && (tok < __ldg(a.q_start) || tok >= __ldg(a.q_start + a.n_seqs))) return;  // no sequence's token
-    const uint64_t stride = (uint64_t)a.n_tokens * a.n_heads;
-    float M = -INFINITY;
-    for (uint32_t p = lane; p < a.n_parts; p += 32) M = fmaxf(M, __ldcg(a.part_ml + p * stride + id).x);
-    M = warp_max(M);
-    float L = 0.0f, o[HD / 32];
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) o[i] = 0.0f;
-    for (uint32_t p = 0; p < a.n_parts; ++p) {
-        const float2 ml = __ldcg(a.part_ml + p * stride + id);
-        if (ml.y == 0.0f) continue;  // no row of this part is seen (a NaN sum is)
-        const float f = ml.x == -INFINITY ? 1.0f : exp2f(ml.x - M);
-        L += ml.y * f;
-#pragma unroll
-        for (int i = 0; i < HD / 32; ++i) o[i] = fmaf(__ldcg(a.part_o + (p * stride + id) * HD + i * 32 + lane), f, o[i]);
-    }
-    const float inv = L == 0.0f ? 0.0f : 1.0f / L;
-#pragma unroll
-    for (int i = 0; i < HD / 32; ++i) {
-        T* d = reinterpret_cast<T*>(a.out) + (uint64_t)tok * a.o_token + (uint64_t)h * a.o_head + i * 32 + lane;
-        *d = (T)(o[i] * inv);
-    }
+    PartSum<HD> sum;
+    sum.add_parts(a, id, c, a.n_parts);
+    sum.template store<T>(a, tok, h, c);
 }
 
 }  // namespace qb200

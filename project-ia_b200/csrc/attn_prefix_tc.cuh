@@ -73,12 +73,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
         : "memory");
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 template <typename T, int HD>
 __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __grid_constant__ PrefixArgs a) {
     using S = TcShape<HD>;
