@@ -217,8 +217,8 @@ q_error_code q_b200_gemv_f32(const float* d_w, uint32_t M, uint32_t K,
  *
  * Every pointer in the argument records is a device pointer of the current
  * device unless it is a plan (host); a pointer that is not is refused with
- * Q_ERR_INVALID_ARG.  Strides count elements.  Calls are asynchronous on
- * `stream`, allocate nothing, keep no state between calls and may be
+ * Q_ERR_INVALID_ARG.  Strides count elements and, but for page_stride, are
+ * below 2^32.  Calls are asynchronous on `stream`, allocate nothing, keep no state between calls and may be
  * captured in a CUDA graph; calls on different streams may overlap as long
  * as they share no output or workspace.  What the device alone can see to be
  * wrong (a page, sequence or token out of range, a length above its bound)

@@ -42,10 +42,18 @@ FastDiv fast_div_of(uint32_t d) {
     return {d, (uint32_t)(((1ull << 32) * ((1ull << s) - d)) / d + 1), s};
 }
 
+uint32_t cdiv(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
+
 uint64_t align_of(std::initializer_list<uint64_t> v) {  // largest power of two that divides all
     uint64_t all = 0;
     for (uint64_t x : v) all |= x;
     return all ? (all & (~all + 1)) : ~0ull;
+}
+// Strides that kernels keep in 32 bits.
+bool short_strides(std::initializer_list<uint64_t> v) {
+    for (uint64_t x : v)
+        if (x >> 32) return false;
+    return true;
 }
 uint64_t addr(const void* p) { return (uint64_t)(uintptr_t)p; }
 
@@ -54,7 +62,7 @@ q_error_code check_cache(const q_b200_paged_kv& kv) {
     if (!known(kv.dtype)) return Q_ERR_INVALID_DTYPE;
     if (kv.reserved) return Q_ERR_INVALID_ARG;
     if (kv.n_pages == 0 || kv.page_rows == 0 || kv.n_kv_heads == 0 || kv.head_dim == 0) return Q_ERR_INVALID_SIZE;
-    if (kv.page_rows > (1u << 30)) return Q_ERR_INVALID_SIZE;
+    if (kv.page_rows > (1u << 30) || !short_strides({kv.head_stride, kv.row_stride})) return Q_ERR_INVALID_SIZE;
     if (kv.row_stride < kv.head_dim && kv.page_rows > 1) return Q_ERR_INVALID_SIZE;
     if ((addr(kv.k) | addr(kv.v)) & (size_of(kv.dtype) - 1)) return Q_ERR_MISALIGNED;
     return Q_OK;
@@ -68,44 +76,38 @@ q_error_code check_plan(const q_b200_rope_plan* p, uint32_t head_dim) {
 
 // ---- rotation -------------------------------------------------------------------
 
+template <typename TI, typename TC, int E>
+cudaError_t launch_rotate_units(RotateArgs& a, cudaStream_t st) {
+    a.rot_units = a.rot / (2 * E);
+    const uint32_t U = a.rot_units + (a.head_dim - a.rot) / E;
+    a.heads = a.part[0].heads + a.part[1].heads + a.part[2].heads;
+    // Two units a thread where that fills the GPU, else one, for the shortest
+    // path through few tokens.
+    a.row_step = ROT_THREADS / U;  // U <= 256: head_dim is
+    const uint64_t all = (uint64_t)a.n_tokens * a.heads * U;
+    const uint32_t N = all >= 148ull * 8 * ROT_THREADS ? 2 : 1, room = N * a.row_step;
+    a.cta_heads = std::min(a.heads, room);
+    a.cta_tokens = std::min({a.n_tokens, std::max(1u, room / a.cta_heads), ROT_TOKENS, a.rot ? ROT_ANGLES / (a.rot / 2) : ROT_TOKENS});
+    a.by_units = fast_div_of(U);
+    a.by_heads = fast_div_of(a.cta_heads);
+    a.by_pairs = fast_div_of(std::max(1u, a.rot / 2));
+    const dim3 grid(cdiv(a.n_tokens, a.cta_tokens), cdiv(a.heads, a.cta_heads));
+    constexpr bool same = std::is_same<TI, TC>::value;
+    if (a.row || !same)
+        return launch_ex(N == 2 ? rotate_kernel<TI, TC, E, 2, true> : rotate_kernel<TI, TC, E, 1, true>, grid, dim3(ROT_THREADS), 0, st, false, a);
+    return launch_ex(N == 2 ? rotate_kernel<TI, TI, E, 2, false> : rotate_kernel<TI, TI, E, 1, false>, grid, dim3(ROT_THREADS), 0, st, false, a);
+}
+
 template <typename TI, typename TC>
-cudaError_t launch_rotate(RotateArgs& a, uint32_t E, uint32_t HB, cudaStream_t st) {
-    const uint32_t rot = a.rot;
-    a.rot_units = rot / (2 * E);
-    a.units = a.rot_units + (a.head_dim - rot) / E;
-    uint32_t chunks = 0;
-    for (RotateRows& p : a.part) {
-        p.chunks = (p.heads + HB - 1) / HB;
-        chunks += p.chunks;
-    }
-    if (chunks == 0) return cudaSuccess;
-    a.by_units = fast_div_of(a.units);
-    a.by_chunks = fast_div_of(chunks);
-    // the item index is 31 bits: longer inputs go in runs of tokens
-    const uint64_t per = (uint64_t)chunks * a.units;
-    const uint32_t run = (uint32_t)std::min<uint64_t>(a.n_tokens, (1ull << 30) / per + 1), all = a.n_tokens;
-    void (*kern)(const RotateArgs) = nullptr;
-    if (E == 8) kern = HB == 4 ? rotate_kernel<TI, TC, 8, 4> : rotate_kernel<TI, TC, 8, 1>;
-    else if (E == 4) kern = HB == 4 ? rotate_kernel<TI, TC, 4, 4> : rotate_kernel<TI, TC, 4, 1>;
-    else kern = HB == 4 ? rotate_kernel<TI, TC, 1, 4> : rotate_kernel<TI, TC, 1, 1>;
-    for (uint32_t t0 = 0; t0 < all; t0 += run) {
-        RotateArgs b = a;
-        b.n_tokens = std::min(run, all - t0);
-        b.n_items = per * b.n_tokens;
-        for (RotateRows& p : b.part) {
-            if (!p.heads) continue;
-            p.src = (const TI*)p.src + t0 * p.src_token;
-            if (!p.paged) p.dst = (TI*)p.dst + t0 * p.dst_token;
-        }
-        if (b.pos) b.pos += t0;
-        if (b.row) b.row += t0;
-        if (b.seq) b.seq += t0;
-        else if (b.row && t0) b.pages += (size_t)t0 * b.pages_per_seq, b.n_seqs -= std::min(t0, b.n_seqs);
-        const cudaError_t e = launch_ex(kern, dim3((uint32_t)((b.n_items + ROT_THREADS - 1) / ROT_THREADS)),
-                                        dim3(ROT_THREADS), 0, st, false, b);
-        if (e != cudaSuccess) return e;
-    }
-    return cudaSuccess;
+cudaError_t launch_rotate(RotateArgs& a, uint32_t E, cudaStream_t st) {
+    if constexpr (sizeof(TI) == 2 || sizeof(TC) == 2)
+        if (E == 8) return launch_rotate_units<TI, TC, 8>(a, st);
+    return E == 4 ? launch_rotate_units<TI, TC, 4>(a, st) : launch_rotate_units<TI, TC, 1>(a, st);
+}
+
+RotateRows rotate_rows(const void* src, void* dst, uint64_t st, uint64_t sh, uint64_t dt, uint64_t dh, uint32_t heads,
+                       bool rotate) {
+    return {src, dst, (uint32_t)st, (uint32_t)sh, (uint32_t)dt, (uint32_t)dh, heads, rotate ? 1u : 0u};
 }
 
 void set_plan(RotateArgs& a, const q_b200_rope_plan* plan, bool transpose) {
@@ -124,11 +126,6 @@ bool vectors_fit(uint32_t E, uint32_t es, uint64_t by, const RotateArgs& a) {
     const uint32_t pair = a.interleaved ? a.rot % (2 * E) : (a.rot / 2) % E;
     return pair == 0 && (a.head_dim - a.rot) % E == 0;
 }
-
-// Heads that a thread takes: four where that still leaves two full waves of
-// threads (the angle is formed once and four heads' loads are in flight),
-// else one, for the shortest path through few tokens.
-uint32_t heads_per_thread(uint64_t items_of_one) { return items_of_one / 4 >= 148ull * 2048 * 2 ? 4u : 1u; }
 
 }  // namespace
 
@@ -185,6 +182,7 @@ q_error_code q_b200_rope(const q_b200_rope_args* r, void* stream) {
     if (q_error_code rc = check_plan(r->plan, r->head_dim)) return rc;
     const uint32_t es = size_of(r->dtype);
     if (((addr(r->x) | addr(r->out)) & (es - 1)) || (addr(r->pos) & 3)) return Q_ERR_MISALIGNED;
+    if (!short_strides({r->x_token_stride, r->x_head_stride, r->out_token_stride, r->out_head_stride})) return Q_ERR_INVALID_SIZE;
     // in place means the same elements; another overlay would be read after it is written
     if (r->x == r->out && (r->x_token_stride != r->out_token_stride || r->x_head_stride != r->out_head_stride))
         return Q_ERR_ALIASING;
@@ -194,25 +192,17 @@ q_error_code q_b200_rope(const q_b200_rope_args* r, void* stream) {
     a.pos = r->pos;
     a.n_tokens = r->n_tokens;
     a.head_dim = r->head_dim;
-    RotateRows& p = a.part[2];
-    p.src = r->x;
-    p.dst = r->out;
-    p.src_token = r->x_token_stride;
-    p.src_head = r->x_head_stride;
-    p.dst_token = r->out_token_stride;
-    p.dst_head = r->out_head_stride;
-    p.heads = r->n_heads;
-    p.rotate = 1;
+    a.part[2] = rotate_rows(r->x, r->out, r->x_token_stride, r->x_head_stride, r->out_token_stride, r->out_head_stride,
+                            r->n_heads, true);
     const uint64_t by = align_of({addr(r->x), addr(r->out), r->x_token_stride * es, r->x_head_stride * es,
                                   r->out_token_stride * es, r->out_head_stride * es});
     uint32_t E = es == 4 ? 4 : 8;
     while (E > 1 && !vectors_fit(E, es, by, a)) E = E == 8 ? 4 : 1;
-    const uint32_t HB = heads_per_thread((uint64_t)r->n_tokens * r->n_heads * r->head_dim / (2 * E));
     cudaStream_t st = (cudaStream_t)stream;
     switch (r->dtype) {
-        case Q_B200_F32: Q_CUDA((launch_rotate<float, float>(a, E, HB, st))); break;
-        case Q_B200_F16: Q_CUDA((launch_rotate<__half, __half>(a, E, HB, st))); break;
-        default: Q_CUDA((launch_rotate<__nv_bfloat16, __nv_bfloat16>(a, E, HB, st))); break;
+        case Q_B200_F32: Q_CUDA((launch_rotate<float, float>(a, E, st))); break;
+        case Q_B200_F16: Q_CUDA((launch_rotate<__half, __half>(a, E, st))); break;
+        default: Q_CUDA((launch_rotate<__nv_bfloat16, __nv_bfloat16>(a, E, st))); break;
     }
     return Q_OK;
 }
@@ -230,6 +220,9 @@ q_error_code q_b200_kv_append(const q_b200_append_args* r, void* stream) {
     if (((addr(r->k) | addr(r->v) | addr(r->q) | addr(r->q_out)) & (es - 1)) ||
         ((addr(r->pages) | addr(r->seq) | addr(r->row) | addr(r->pos)) & 3))
         return Q_ERR_MISALIGNED;
+    if (!short_strides({r->k_token_stride, r->k_head_stride, r->v_token_stride, r->v_head_stride}) ||
+        (r->q && !short_strides({r->q_token_stride, r->q_head_stride, r->q_out_token_stride, r->q_out_head_stride})))
+        return Q_ERR_INVALID_SIZE;
     if (r->q && r->q == r->q_out && (r->q_token_stride != r->q_out_token_stride || r->q_head_stride != r->q_out_head_stride))
         return Q_ERR_ALIASING;
     if (!DevicePtrs()(r->kv.k)(r->kv.v)(r->k)(r->v)(r->q)(r->q ? r->q_out : nullptr)(r->pages)(r->seq)(r->row)(r->pos).ok)
@@ -241,7 +234,7 @@ q_error_code q_b200_kv_append(const q_b200_append_args* r, void* stream) {
     a.seq = r->seq;
     a.pages = r->pages;
     a.page_stride = r->kv.page_stride;
-    a.row_stride = r->kv.row_stride;
+    a.row_stride = (uint32_t)r->kv.row_stride;
     a.page_rows = fast_div_of(r->kv.page_rows);
     a.n_pages = r->kv.n_pages;
     a.pages_per_seq = r->pages_per_seq;
@@ -249,11 +242,12 @@ q_error_code q_b200_kv_append(const q_b200_append_args* r, void* stream) {
     a.n_tokens = r->n_tokens;
     a.head_dim = r->kv.head_dim;
     const uint64_t hs = r->kv.head_stride;
-    a.part[0] = {r->k, r->kv.k, r->k_token_stride, r->k_head_stride, 0, hs, r->kv.n_kv_heads, 0, r->plan ? 1u : 0u, 1u};
-    a.part[1] = {r->v, r->kv.v, r->v_token_stride, r->v_head_stride, 0, hs, r->kv.n_kv_heads, 0, 0u, 1u};
+    const bool rot = r->plan != nullptr;
+    a.part[0] = rotate_rows(r->k, r->kv.k, r->k_token_stride, r->k_head_stride, 0, hs, r->kv.n_kv_heads, rot);
+    a.part[1] = rotate_rows(r->v, r->kv.v, r->v_token_stride, r->v_head_stride, 0, hs, r->kv.n_kv_heads, false);
     if (r->q)
-        a.part[2] = {r->q, r->q_out, r->q_token_stride, r->q_head_stride, r->q_out_token_stride, r->q_out_head_stride,
-                     r->n_heads, 0, r->plan ? 1u : 0u, 0u};
+        a.part[2] = rotate_rows(r->q, r->q_out, r->q_token_stride, r->q_head_stride, r->q_out_token_stride,
+                                r->q_out_head_stride, r->n_heads, rot);
     uint64_t in = align_of({addr(r->k), addr(r->v), r->k_token_stride * es, r->k_head_stride * es, r->v_token_stride * es,
                             r->v_head_stride * es});
     if (r->q)
@@ -262,15 +256,13 @@ q_error_code q_b200_kv_append(const q_b200_append_args* r, void* stream) {
     const uint64_t to = align_of({addr(r->kv.k), addr(r->kv.v), r->kv.page_stride * ec, hs * ec, r->kv.row_stride * ec});
     uint32_t E = es == 4 && ec == 4 ? 4 : 8;
     while (E > 1 && !(vectors_fit(E, es, in, a) && vectors_fit(E, ec, to, a))) E = E == 8 ? 4 : 1;
-    const uint32_t heads = 2 * r->kv.n_kv_heads + (r->q ? r->n_heads : 0);
-    const uint32_t HB = heads_per_thread((uint64_t)r->n_tokens * heads * r->kv.head_dim / (2 * E));
     cudaStream_t st = (cudaStream_t)stream;
     auto go = [&](auto ti) -> cudaError_t {
         using TI = decltype(ti);
         switch (r->kv.dtype) {
-            case Q_B200_F32: return launch_rotate<TI, float>(a, E, HB, st);
-            case Q_B200_F16: return launch_rotate<TI, __half>(a, E, HB, st);
-            default: return launch_rotate<TI, __nv_bfloat16>(a, E, HB, st);
+            case Q_B200_F32: return launch_rotate<TI, float>(a, E, st);
+            case Q_B200_F16: return launch_rotate<TI, __half>(a, E, st);
+            default: return launch_rotate<TI, __nv_bfloat16>(a, E, st);
         }
     };
     switch (r->dtype) {
@@ -300,8 +292,6 @@ struct AttnPlan {
     AttnPass pre, own;
     uint32_t parts = 0;   // partial results in the workspace
 };
-
-uint32_t cdiv(uint64_t a, uint64_t b) { return (uint32_t)((a + b - 1) / b); }
 
 // A pass of attn_few_kernel (up to 32 vectors) or attn_rows_kernel: the rows
 // are cut until about two CTAs per SM have work, each with at least two

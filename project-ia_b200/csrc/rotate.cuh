@@ -9,17 +9,23 @@
 // the fraction in half turns, so nothing else is reduced.  Products and the
 // rotation are fp32; each output is rounded once to its type.
 //
-// Bound: bytes (3 flops for each element of 4 to 8 bytes moved).  One thread
-// takes one unit (E pairs: two vectors of E elements, E sized to 16-byte
-// accesses of the narrower type, or one pair where alignment allows no more)
-// of HB consecutive heads of one token: its cosines are computed once for
-// the HB heads, and the HB * 2 loads are in flight together.  Neighbouring
-// threads take neighbouring units of the same head, so every access is
-// coalesced.
+// Bound: bytes (3 flops for each element of 4 to 8 bytes moved), as long as
+// the angles do not cost more: a sine and cosine is about 50 instructions,
+// and every head of a token needs the same ones.  So a CTA takes whole tokens
+// (or a run of one token's heads), forms their cosines and sines once in
+// shared memory, and each thread then turns N units of E pairs (two vectors
+// of E elements, 16 bytes each where alignment allows).  The N units' loads
+// are issued before the angles are formed, so that they are under way
+// meanwhile.  Neighbouring threads take neighbouring units of a head: every
+// access is coalesced.  (Angles formed by every thread for its own unit took
+// 300 instructions a unit: 70 us against 26 us of bytes for 8191 x 40 x 128
+// bf16.)
 #pragma once
 
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
+
+#include <type_traits>
 
 #include "common.cuh"
 #include "qorus_b200.h"
@@ -28,49 +34,107 @@ namespace qb200 {
 
 static constexpr uint32_t ROT_THREADS = 256;
 
-// E consecutive elements to and from fp32; 4-, 8-, 16- or 32-byte accesses,
-// the address aligned to min(16, E * sizeof(T)).
-template <typename T, int E>
-__device__ __forceinline__ void load_vec(const T* p, float (&v)[E]) {
-    if constexpr (sizeof(T) * E >= 16) {
-#pragma unroll
-        for (int c = 0; c < (int)sizeof(T) * E / 16; ++c) {
-            const uint4 w = reinterpret_cast<const uint4*>(p)[c];
-            const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-            for (int i = 0; i < 16 / (int)sizeof(T); ++i) v[c * (16 / sizeof(T)) + i] = (float)e[i];
-        }
-    } else if constexpr (sizeof(T) * E == 8) {
-        const uint2 w = *reinterpret_cast<const uint2*>(p);
-        const T* e = reinterpret_cast<const T*>(&w);
-#pragma unroll
-        for (int i = 0; i < E; ++i) v[i] = (float)e[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) v[i] = (float)p[i];
-    }
+// Two 16-bit numbers in a word.
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <typename T>
+__device__ __forceinline__ float2 unpack2(uint32_t w);
+template <>
+__device__ __forceinline__ float2 unpack2<__half>(uint32_t w) {
+    return __half22float2(*reinterpret_cast<const __half2*>(&w));
+}
+template <>
+__device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
+    return __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w));
 }
 
+// E consecutive elements as they lie in memory, in 16-, 8- or single-element
+// accesses; the address is aligned to min(16, E * sizeof(T)).
 template <typename T, int E>
-__device__ __forceinline__ void store_vec(T* p, const float (&v)[E]) {
+struct alignas(sizeof(T) * E >= 16 ? 16 : sizeof(T) * E) Vec {
+    T e[E];
+};
+template <typename T, int E>
+__device__ __forceinline__ Vec<T, E> load_raw(const T* p) {
+    Vec<T, E> v;
     if constexpr (sizeof(T) * E >= 16) {
 #pragma unroll
-        for (int c = 0; c < (int)sizeof(T) * E / 16; ++c) {
-            uint4 w;
-            T* e = reinterpret_cast<T*>(&w);
-#pragma unroll
-            for (int i = 0; i < 16 / (int)sizeof(T); ++i) e[i] = (T)v[c * (16 / sizeof(T)) + i];
-            reinterpret_cast<uint4*>(p)[c] = w;
-        }
+        for (int c = 0; c < (int)sizeof(T) * E / 16; ++c) reinterpret_cast<uint4*>(&v)[c] = reinterpret_cast<const uint4*>(p)[c];
     } else if constexpr (sizeof(T) * E == 8) {
-        uint2 w;
-        T* e = reinterpret_cast<T*>(&w);
-#pragma unroll
-        for (int i = 0; i < E; ++i) e[i] = (T)v[i];
-        *reinterpret_cast<uint2*>(p) = w;
+        *reinterpret_cast<uint2*>(&v) = *reinterpret_cast<const uint2*>(p);
     } else {
 #pragma unroll
-        for (int i = 0; i < E; ++i) p[i] = (T)v[i];
+        for (int i = 0; i < E; ++i) v.e[i] = p[i];
+    }
+    return v;
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_raw(T* p, const Vec<T, E>& v) {
+    if constexpr (sizeof(T) * E >= 16) {
+#pragma unroll
+        for (int c = 0; c < (int)sizeof(T) * E / 16; ++c) reinterpret_cast<uint4*>(p)[c] = reinterpret_cast<const uint4*>(&v)[c];
+    } else if constexpr (sizeof(T) * E == 8) {
+        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(&v);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; ++i) p[i] = v.e[i];
+    }
+}
+// M elements from the i-th on, to fp32 and, rounded once, from fp32.
+template <int M, typename T, int E>
+__device__ __forceinline__ void get(const Vec<T, E>& v, int i, float (&y)[M]) {
+    if constexpr (sizeof(T) == 2 && M > 1) {
+#pragma unroll
+        for (int k = 0; k < M / 2; ++k) {
+            const float2 x = unpack2<T>(reinterpret_cast<const uint32_t*>(&v)[i / 2 + k]);
+            y[2 * k] = x.x;
+            y[2 * k + 1] = x.y;
+        }
+    } else {
+#pragma unroll
+        for (int k = 0; k < M; ++k) y[k] = (float)v.e[i + k];
+    }
+}
+template <int M, typename T, int E>
+__device__ __forceinline__ void put(Vec<T, E>& v, int i, const float (&y)[M]) {
+    if constexpr (sizeof(T) == 2 && M > 1) {
+#pragma unroll
+        for (int k = 0; k < M / 2; ++k) reinterpret_cast<uint32_t*>(&v)[i / 2 + k] = pack2<T>(y[2 * k], y[2 * k + 1]);
+    } else {
+#pragma unroll
+        for (int k = 0; k < M; ++k) v.e[i + k] = (T)y[k];
+    }
+}
+template <typename T, int E>
+__device__ __forceinline__ void to_float(const Vec<T, E>& v, float (&y)[E]) {
+    get<E>(v, 0, y);
+}
+template <typename T, int E>
+__device__ __forceinline__ void store_vec(T* p, const float (&y)[E]) {
+    Vec<T, E> v;
+    put<E>(v, 0, y);
+    store_raw(p, v);
+}
+template <int M>
+__device__ __forceinline__ void load_shared(const float* p, float (&y)[M]) {
+    if constexpr (M == 4) {
+        const float4 x = *reinterpret_cast<const float4*>(p);
+        y[0] = x.x, y[1] = x.y, y[2] = x.z, y[3] = x.w;
+    } else if constexpr (M == 2) {
+        const float2 x = *reinterpret_cast<const float2*>(p);
+        y[0] = x.x, y[1] = x.y;
+    } else {
+        y[0] = *p;
     }
 }
 
@@ -82,14 +146,16 @@ __device__ __forceinline__ uint32_t fast_div(uint32_t n, const FastDiv& f) {
     return (__umulhi(n, f.mul) + n) >> f.shift;
 }
 
-// One kind of head in a launch: rows of `heads` heads of every token.
+// One kind of head in a launch: `heads` heads of every token.
 struct RotateRows {
     const void* src;
     void* dst;  // the paged cache's base for keys and values
-    uint64_t src_token, src_head, dst_token, dst_head;
-    uint32_t heads, chunks;  // chunks of HB heads
-    uint32_t rotate, paged;
+    uint32_t src_token, src_head, dst_token, dst_head;
+    uint32_t heads, rotate;
 };
+
+static constexpr uint32_t ROT_ANGLES = 2048;  // cosines and sines of a CTA
+static constexpr uint32_t ROT_TOKENS = 32;    // tokens of a CTA
 
 struct RotateArgs {
     RotateRows part[3];    // append: keys, values, queries; rope: queries alone in part[2]
@@ -97,118 +163,171 @@ struct RotateArgs {
     const int32_t* row;    // append only: < 0 is padding
     const uint32_t* seq;
     const uint32_t* pages;
-    uint64_t page_stride, row_stride;
+    uint64_t page_stride;
+    uint32_t row_stride;
     FastDiv page_rows;
     uint32_t n_pages, pages_per_seq, n_seqs;
     uint32_t n_tokens, head_dim, rot, interleaved;
-    uint32_t units;        // units of a row: rot / (2E) rotating, the rest copied
-    uint32_t rot_units;
-    FastDiv by_units, by_chunks;
-    uint64_t n_items;      // threads with work: n_tokens * chunks * units
+    uint32_t rot_units;    // units of a row that rotate, rot / (2E); the rest is copied, E elements a unit
+    uint32_t cta_tokens, cta_heads, heads;  // a CTA's share; heads of all kinds
+    uint32_t row_step;     // rows that the CTA's threads take at once
+    FastDiv by_units, by_heads, by_pairs;   // units of a row, cta_heads, rot / 2
     float gain, sign;
     double turns[128];
 };
 
-template <typename TI, typename TO, int E, int HB>
-__device__ __forceinline__ void rotate_heads(const TI* src, uint64_t src_head, TO* dst, uint64_t dst_head, uint32_t n,
-                                             uint32_t ia, uint32_t ib, bool rot, bool inter, const float (&cs)[E],
-                                             const float (&sn)[E]) {
-    float a[HB][E], b[HB][E];
+// One unit: pairs (a_j, b_j) in the half layout, in the interleaved one the
+// pairs lie in a, then in b.  Four pairs at a time keep few numbers live.
+template <typename TI, typename TO, int E>
+__device__ __forceinline__ void turn_unit(const Vec<TI, E>& a, const Vec<TI, E>& b, const float* cs, const float* sn, bool inter,
+                                          Vec<TO, E>& oa, Vec<TO, E>& ob) {
+    constexpr int M = E >= 4 ? 4 : 1;
+    if (E > 1 && inter) {
+        constexpr int H = E > 1 ? E / 2 : 1;  // pairs of a, of b
 #pragma unroll
-    for (int h = 0; h < HB; ++h)
-        if (h < (int)n) {
-            load_vec<TI, E>(src + h * src_head + ia, a[h]);
-            if (ib != ~0u) load_vec<TI, E>(src + h * src_head + ib, b[h]);
-        }
+        for (int k = 0; k < 2; ++k) {
+            float x[E], c[H], s[H];
+            get<E>(k ? b : a, 0, x);
+            load_shared<H>(cs + k * H, c);
+            load_shared<H>(sn + k * H, s);
 #pragma unroll
-    for (int h = 0; h < HB; ++h) {
-        if (h >= (int)n) break;
-        if (rot) {
-            if (inter && E > 1) {  // (a0 a1)(a2 a3)... (b0 b1)...: pair j in elements 2j, 2j+1 of a then b
-#pragma unroll
-                for (int j = 0; j < E / 2; ++j) {
-                    const float x0 = a[h][2 * j], x1 = a[h][2 * j + 1], y0 = b[h][2 * j], y1 = b[h][2 * j + 1];
-                    a[h][2 * j] = x0 * cs[j] - x1 * sn[j];
-                    a[h][2 * j + 1] = x0 * sn[j] + x1 * cs[j];
-                    b[h][2 * j] = y0 * cs[E / 2 + j] - y1 * sn[E / 2 + j];
-                    b[h][2 * j + 1] = y0 * sn[E / 2 + j] + y1 * cs[E / 2 + j];
-                }
-            } else {
-#pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    const float x = a[h][j], y = b[h][j];
-                    a[h][j] = x * cs[j] - y * sn[j];
-                    b[h][j] = x * sn[j] + y * cs[j];
-                }
+            for (int j = 0; j < H; ++j) {
+                const float u = x[2 * j], v = x[2 * j + (E > 1)];
+                x[2 * j] = u * c[j] - v * s[j];
+                x[2 * j + (E > 1)] = u * s[j] + v * c[j];
             }
+            put<E>(k ? ob : oa, 0, x);
         }
-        store_vec<TO, E>(dst + h * dst_head + ia, a[h]);
-        if (ib != ~0u) store_vec<TO, E>(dst + h * dst_head + ib, b[h]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < E; i += M) {
+            float x[M], y[M], c[M], s[M];
+            get<M>(a, i, x);
+            get<M>(b, i, y);
+            load_shared<M>(cs + i, c);
+            load_shared<M>(sn + i, s);
+#pragma unroll
+            for (int j = 0; j < M; ++j) {
+                const float u = x[j], v = y[j];
+                x[j] = u * c[j] - v * s[j];
+                y[j] = u * s[j] + v * c[j];
+            }
+            put<M>(oa, i, x);
+            put<M>(ob, i, y);
+        }
+    }
+}
+template <typename TI, typename TO, int E>
+__device__ __forceinline__ Vec<TO, E> convert(const Vec<TI, E>& a) {
+    if constexpr (std::is_same<TI, TO>::value) {
+        return a;
+    } else {
+        Vec<TO, E> o;
+        float x[E];
+        get<E>(a, 0, x);
+        put<E>(o, 0, x);
+        return o;
     }
 }
 
-template <typename TI, typename TC, int E, int HB>
+template <typename TI, typename TC, int E, int N, bool APPEND>
 __global__ void __launch_bounds__(ROT_THREADS) rotate_kernel(const __grid_constant__ RotateArgs a) {
-    __shared__ double s_turns[128];
-    if (threadIdx.x < a.rot / 2) s_turns[threadIdx.x] = a.turns[threadIdx.x];
-    __syncthreads();
-    const uint64_t id = (uint64_t)blockIdx.x * ROT_THREADS + threadIdx.x;
-    if (id >= a.n_items) return;
-    const uint32_t n = (uint32_t)id;
-    const uint32_t rc = fast_div(n, a.by_units), u = n - rc * a.by_units.d;
-    const uint32_t t = fast_div(rc, a.by_chunks);
-    uint32_t c = rc - t * a.by_chunks.d;
-    int kind = 0;
-    while (kind < 2 && c >= a.part[kind].chunks) c -= a.part[kind++].chunks;
-    const RotateRows& p = a.part[kind];
-    uint64_t cache_off = 0;
-    int32_t pos;
-    if (a.row) {
+    __shared__ __align__(16) float s_cos[ROT_ANGLES], s_sin[ROT_ANGLES];
+    __shared__ uint64_t s_off[ROT_TOKENS];  // append: the token's row in the cache; ~0: none
+    const uint32_t tid = threadIdx.x, t0 = blockIdx.x * a.cta_tokens, h0 = blockIdx.y * a.cta_heads;
+    const uint32_t nt = min(a.cta_tokens, a.n_tokens - t0), nh = min(a.cta_heads, a.heads - h0);
+    // this thread's unit of every row that it takes: rows rsub, rsub + step, ... of the CTA's nt x nh
+    const uint32_t U = a.by_units.d, rsub = fast_div(tid, a.by_units), u = tid - rsub * U, step = a.row_step;
+    const bool turn = u < a.rot_units;
+    const uint32_t ia = turn ? (a.interleaved ? 2 * E * u : E * u) : a.rot + E * (u - a.rot_units);
+    const uint32_t ib = a.interleaved ? ia + E : ia + a.rot / 2;
+    struct Row {
+        uint32_t tok, kind, head;
+        bool in;
+    };
+    auto row_of = [&](int k) {
+        Row x;
+        const uint32_t r = rsub + k * step;
+        x.tok = fast_div(r, a.by_heads);
+        const uint32_t h = r - x.tok * a.cta_heads;
+        x.in = rsub < step && x.tok < nt && h < nh;
+        x.head = h0 + h;
+        x.kind = 2;
+        if (APPEND) {
+            const uint32_t kv = a.part[0].heads;
+            x.kind = x.head < kv ? 0 : x.head < 2 * kv ? 1 : 2;
+            x.head -= x.kind * kv;
+        }
+        return x;
+    };
+
+    Vec<TI, E> va[N], vb[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+        const Row x = row_of(k);
+        if (!x.in) continue;
+        const RotateRows& p = a.part[x.kind];
+        const TI* src = reinterpret_cast<const TI*>(p.src) + (uint64_t)(t0 + x.tok) * p.src_token + (uint64_t)x.head * p.src_head;
+        va[k] = load_raw<TI, E>(src + ia);
+        if (turn) vb[k] = load_raw<TI, E>(src + ib);
+    }
+    const uint32_t pairs = a.rot / 2;
+    // through a generic address: every lane reads another one, which the
+    // constant cache would serve one after another
+    const double* turns = a.turns;
+    asm volatile("" : "+l"(turns));
+    for (uint32_t e = tid; e < nt * pairs; e += ROT_THREADS) {
+        const uint32_t tok = fast_div(e, a.by_pairs), i = e - tok * pairs;
+        const int32_t pos = __ldg((APPEND && !a.pos ? a.row : a.pos) + t0 + tok);
+        double w = (double)pos * turns[i];
+        w -= rint(w);
+        float c, s;
+        sincospif((float)(w + w), &s, &c);
+        s_cos[e] = c * a.gain;
+        s_sin[e] = s * a.sign;
+    }
+    if (APPEND && tid < nt) {
+        const uint32_t t = t0 + tid;
         const int32_t row = __ldg(a.row + t);
-        if (row < 0) return;
-        pos = a.pos ? __ldg(a.pos + t) : row;
-        if (p.paged) {
+        uint64_t off = ~0ull;
+        if (row >= 0) {
             const uint32_t sq = a.seq ? __ldg(a.seq + t) : t, r = fast_div((uint32_t)row, a.page_rows);
             uint32_t pg = ~0u;
             if (sq < a.n_seqs && r < a.pages_per_seq) pg = __ldg(a.pages + (size_t)sq * a.pages_per_seq + r);
-            if (pg >= a.n_pages) {
-                qdev_fail(QDEV_BAD_ARG);
-                return;
-            }
-            cache_off = pg * a.page_stride + (uint64_t)((uint32_t)row - r * a.page_rows.d) * a.row_stride;
+            if (pg < a.n_pages) off = pg * a.page_stride + (uint64_t)((uint32_t)row - r * a.page_rows.d) * a.row_stride;
+            else qdev_fail(QDEV_BAD_ARG);
         }
-    } else {
-        pos = __ldg(a.pos + t);
+        s_off[tid] = off;
     }
-    const bool turning = u < a.rot_units;
-    const bool rot = p.rotate && turning;
-    uint32_t ia, ib;
-    if (turning) {
-        ia = a.interleaved ? 2 * E * u : E * u;
-        ib = a.interleaved ? ia + E : ia + a.rot / 2;
-    } else {
-        ia = a.rot + E * (u - a.rot_units);
-        ib = ~0u;
-    }
-    float cs[E], sn[E];
-    if (rot) {
+    __syncthreads();
 #pragma unroll
-        for (int j = 0; j < E; ++j) {
-            double w = (double)pos * s_turns[E * u + j];
-            w -= rint(w);
-            sincospif((float)(w + w), &sn[j], &cs[j]);
-            cs[j] *= a.gain;
-            sn[j] *= a.sign;
+    for (int k = 0; k < N; ++k) {
+        const Row x = row_of(k);
+        if (!x.in) continue;
+        const RotateRows& p = a.part[x.kind];
+        const float *cs = s_cos + x.tok * pairs + E * u, *sn = s_sin + x.tok * pairs + E * u;  // E divides both
+        auto finish = [&](auto* dst, auto to) {
+            using TO = decltype(to);
+            Vec<TO, E> oa, ob;
+            if (turn && p.rotate) {
+                turn_unit<TI, TO, E>(va[k], vb[k], cs, sn, a.interleaved, oa, ob);
+            } else {
+                oa = convert<TI, TO, E>(va[k]);
+                if (turn) ob = convert<TI, TO, E>(vb[k]);
+            }
+            store_raw(dst + ia, oa);
+            if (turn) store_raw(dst + ib, ob);
+        };
+        if (APPEND) {
+            const uint64_t off = s_off[x.tok];
+            if (off == ~0ull) continue;  // padding, or no page
+            if (x.kind < 2) {
+                finish(reinterpret_cast<TC*>(p.dst) + off + (uint64_t)x.head * p.dst_head, TC());
+                continue;
+            }
         }
+        finish(reinterpret_cast<TI*>(p.dst) + (uint64_t)(t0 + x.tok) * p.dst_token + (uint64_t)x.head * p.dst_head, TI());
     }
-    const uint32_t h0 = c * HB, nh = min((uint32_t)HB, p.heads - h0);
-    const TI* src = reinterpret_cast<const TI*>(p.src) + t * p.src_token + h0 * p.src_head;
-    if (p.paged)
-        rotate_heads<TI, TC, E, HB>(src, p.src_head, reinterpret_cast<TC*>(p.dst) + cache_off + h0 * p.dst_head,
-                                    p.dst_head, nh, ia, ib, rot, a.interleaved, cs, sn);
-    else
-        rotate_heads<TI, TI, E, HB>(src, p.src_head, reinterpret_cast<TI*>(p.dst) + t * p.dst_token + h0 * p.dst_head,
-                                    p.dst_head, nh, ia, ib, rot, a.interleaved, cs, sn);
 }
 
 }  // namespace qb200

@@ -53,7 +53,7 @@ struct VerifyArgs {
 template <typename T, int E>
 __device__ __forceinline__ void load_row(const T* row, uint32_t i, uint32_t end, bool vec, float none, float (&v)[E]) {
     if (vec && i + E <= end) {
-        load_vec<T, E>(row + i, v);
+        to_float(load_raw<T, E>(row + i), v);
     } else {
 #pragma unroll
         for (int j = 0; j < E; ++j) v[j] = i + j < end ? (float)row[i + j] : none;
