@@ -585,15 +585,18 @@ q_error_code q_b200_verify_draft(const q_b200_verify_args* r, void* stream) {
     a.vocab = r->vocab;
     uint64_t by = align_of({addr(r->target), a.t_seq * es, a.t_row * es});
     if (a.draft) by = std::min(by, align_of({addr(r->draft), a.d_seq * es, a.d_row * es}));
-    a.vec = by >= 16;
+    a.vec = by >= 16 && r->vocab >= 8;
     const int kind = r->kind == Q_B200_PROBS ? VER_PROBS : r->temperature < 1e-6f ? VER_GREEDY : VER_LOGITS;
     if (kind == VER_LOGITS) {
         a.cd = 1.44269504088896340736 / (double)r->temperature;
         a.c = (float)a.cd;
     }
-    // CTAs of a sequence: as many as fill the GPU, but each with 2048 entries
-    uint32_t CL = VER_MAX_CL;
-    while (CL > 1 && ((uint64_t)r->n_seqs * CL > 148 || (uint64_t)CL * 2048 > r->vocab)) CL /= 2;
+    // CTAs of a sequence: as many as run at once (two on an SM), but a warp's
+    // segment fills a lane's vectors at least once; 16 of them, which not
+    // every part of the GPU has room for twice, only for a few sequences
+    const uint32_t once = VER_VECS * 32 * (16 / es) * VER_WARPS;
+    uint32_t CL = r->n_seqs <= 4 ? 16 : 8;
+    while (CL > 1 && ((uint64_t)r->n_seqs * CL > 2 * 148 || (uint64_t)(CL / 2) * once >= r->vocab)) CL /= 2;
     a.seg = (cdiv(r->vocab, (uint64_t)CL * VER_WARPS) + 7) & ~7u;
     cudaStream_t st = (cudaStream_t)stream;
     switch (r->dtype) {

@@ -269,12 +269,6 @@ __device__ __forceinline__ bool attn_row(const PrefixArgs& a, const AttnItem& w,
     return off != ~0ull;
 }
 
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // Sum of parts (m, l, o) for four outputs of a vector.
 template <int HD>
 struct PartSum {

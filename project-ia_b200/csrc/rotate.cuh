@@ -34,6 +34,12 @@ namespace qb200 {
 
 static constexpr uint32_t ROT_THREADS = 256;
 
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
 // Two 16-bit numbers in a word.
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -59,60 +65,74 @@ __device__ __forceinline__ float2 unpack2<__nv_bfloat16>(uint32_t w) {
 }
 
 // E consecutive elements as they lie in memory, in 16-, 8- or single-element
-// accesses; the address is aligned to min(16, E * sizeof(T)).
+// accesses; the address is aligned to min(16, E * sizeof(T)).  They are kept
+// as whole words: an array of 16-bit elements is taken apart right behind its
+// load, which then waits, and the loads after it with it.
 template <typename T, int E>
-struct alignas(sizeof(T) * E >= 16 ? 16 : sizeof(T) * E) Vec {
-    T e[E];
+struct Vec {
+    static constexpr int WORDS = sizeof(T) * E / 4;
+    uint32_t w[WORDS];
+};
+template <typename T>
+struct Vec<T, 1> {
+    T e;
 };
 template <typename T, int E>
 __device__ __forceinline__ Vec<T, E> load_raw(const T* p) {
     Vec<T, E> v;
-    if constexpr (sizeof(T) * E >= 16) {
+    if constexpr (E == 1) {
+        v.e = *p;
+    } else if constexpr (sizeof(T) * E >= 16) {
 #pragma unroll
-        for (int c = 0; c < (int)sizeof(T) * E / 16; ++c) reinterpret_cast<uint4*>(&v)[c] = reinterpret_cast<const uint4*>(p)[c];
-    } else if constexpr (sizeof(T) * E == 8) {
-        *reinterpret_cast<uint2*>(&v) = *reinterpret_cast<const uint2*>(p);
+        for (int c = 0; c < Vec<T, E>::WORDS / 4; ++c) {
+            const uint4 x = reinterpret_cast<const uint4*>(p)[c];
+            v.w[4 * c] = x.x, v.w[4 * c + 1] = x.y, v.w[4 * c + 2] = x.z, v.w[4 * c + 3] = x.w;
+        }
     } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) v.e[i] = p[i];
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        v.w[0] = x.x, v.w[1] = x.y;
     }
     return v;
 }
 template <typename T, int E>
 __device__ __forceinline__ void store_raw(T* p, const Vec<T, E>& v) {
-    if constexpr (sizeof(T) * E >= 16) {
+    if constexpr (E == 1) {
+        *p = v.e;
+    } else if constexpr (sizeof(T) * E >= 16) {
 #pragma unroll
-        for (int c = 0; c < (int)sizeof(T) * E / 16; ++c) reinterpret_cast<uint4*>(p)[c] = reinterpret_cast<const uint4*>(&v)[c];
-    } else if constexpr (sizeof(T) * E == 8) {
-        *reinterpret_cast<uint2*>(p) = *reinterpret_cast<const uint2*>(&v);
+        for (int c = 0; c < Vec<T, E>::WORDS / 4; ++c)
+            reinterpret_cast<uint4*>(p)[c] = make_uint4(v.w[4 * c], v.w[4 * c + 1], v.w[4 * c + 2], v.w[4 * c + 3]);
     } else {
-#pragma unroll
-        for (int i = 0; i < E; ++i) p[i] = v.e[i];
+        *reinterpret_cast<uint2*>(p) = make_uint2(v.w[0], v.w[1]);
     }
 }
 // M elements from the i-th on, to fp32 and, rounded once, from fp32.
 template <int M, typename T, int E>
 __device__ __forceinline__ void get(const Vec<T, E>& v, int i, float (&y)[M]) {
-    if constexpr (sizeof(T) == 2 && M > 1) {
+    if constexpr (E == 1) {
+        y[0] = (float)v.e;
+    } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
         for (int k = 0; k < M / 2; ++k) {
-            const float2 x = unpack2<T>(reinterpret_cast<const uint32_t*>(&v)[i / 2 + k]);
+            const float2 x = unpack2<T>(v.w[i / 2 + k]);
             y[2 * k] = x.x;
             y[2 * k + 1] = x.y;
         }
     } else {
 #pragma unroll
-        for (int k = 0; k < M; ++k) y[k] = (float)v.e[i + k];
+        for (int k = 0; k < M; ++k) y[k] = __uint_as_float(v.w[i + k]);
     }
 }
 template <int M, typename T, int E>
 __device__ __forceinline__ void put(Vec<T, E>& v, int i, const float (&y)[M]) {
-    if constexpr (sizeof(T) == 2 && M > 1) {
+    if constexpr (E == 1) {
+        v.e = (T)y[0];
+    } else if constexpr (sizeof(T) == 2) {
 #pragma unroll
-        for (int k = 0; k < M / 2; ++k) reinterpret_cast<uint32_t*>(&v)[i / 2 + k] = pack2<T>(y[2 * k], y[2 * k + 1]);
+        for (int k = 0; k < M / 2; ++k) v.w[i / 2 + k] = pack2<T>(y[2 * k], y[2 * k + 1]);
     } else {
 #pragma unroll
-        for (int k = 0; k < M; ++k) v.e[i + k] = (T)y[k];
+        for (int k = 0; k < M; ++k) v.w[i + k] = __float_as_uint(y[k]);
     }
 }
 template <typename T, int E>

@@ -18,7 +18,8 @@
 // order, so a result does not depend on the launch.  Every row that the test
 // needs is read from HBM once.  Bound: bytes for a batch; for one sequence
 // the dependent steps (draft id -> its probabilities -> the row -> the
-// search), which is why the row's work is spread over up to 16 CTAs.
+// search, about 10 us), which is why the row's work is spread over up to 16
+// CTAs, and a batch over as many as run at once.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -27,10 +28,13 @@
 
 namespace qb200 {
 
-static constexpr uint32_t VER_THREADS = 512;
+static constexpr uint32_t VER_THREADS = 512;  // two CTAs on an SM: 64 registers a thread
 static constexpr uint32_t VER_WARPS = VER_THREADS / 32;
 static constexpr uint32_t VER_MAX_CL = 16;
 static constexpr uint32_t VER_MAX_DRAFT = 31;
+static constexpr uint32_t VER_CHUNKS = 16;  // sums that a warp keeps of its segment's chunks, the last one of all behind
+
+static constexpr int VER_VECS = 2;  // vectors of a row that a lane has under way
 
 enum : int { VER_PROBS = 0, VER_LOGITS = 1, VER_GREEDY = 2 };
 
@@ -49,26 +53,112 @@ struct VerifyArgs {
     double cd;
 };
 
-// E entries from index i of a row, `none` past its end.
+// A lane's share of VER_VECS * 32 E consecutive entries of a row from i0 on:
+// 16-byte vectors of E, 32 E apart; `none` past the end.  A vector past the
+// end is loaded from the row's start instead and replaced, so that all loads
+// are issued before the first is looked at.
 template <typename T, int E>
-__device__ __forceinline__ void load_row(const T* row, uint32_t i, uint32_t end, bool vec, float none, float (&v)[E]) {
-    if (vec && i + E <= end) {
-        to_float(load_raw<T, E>(row + i), v);
-    } else {
+struct RowPart {
+    Vec<T, E> v[VER_VECS];
+    __device__ __forceinline__ void load(const T* row, uint32_t i0, uint32_t end, bool vec, float none) {
+        const uint32_t i = i0 + (threadIdx.x & 31) * E;
+        const uint32_t fill = sizeof(T) == 4 ? __float_as_uint(none) : word<T>(none, none);
+        if (vec) {
 #pragma unroll
-        for (int j = 0; j < E; ++j) v[j] = i + j < end ? (float)row[i + j] : none;
+            for (int k = 0; k < VER_VECS; ++k) v[k] = load_raw<T, E>(row + (i + k * 32 * E + E <= end ? i + k * 32 * E : 0u));
+#pragma unroll
+            for (int k = 0; k < VER_VECS; ++k)
+                if (i + k * 32 * E + E > end)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) v[k].w[j] = fill;
+            if (i0 + VER_VECS * 32 * E <= end || end % E == 0) return;
+        }
+#pragma unroll
+        for (int k = 0; k < VER_VECS; ++k) {  // entry by entry: rows that are not aligned, the last vector of others
+            const uint32_t at = i + k * 32 * E;
+            if (vec && (at + E <= end || at >= end)) continue;
+            float x[E];
+#pragma unroll
+            for (int j = 0; j < E; ++j) x[j] = at + j < end ? (float)row[at + j] : none;
+            put<E>(v[k], 0, x);
+        }
     }
-}
+    template <typename U>
+    static __device__ __forceinline__ uint32_t word(float a, float b) {
+        if constexpr (sizeof(U) == 2) return pack2<U>(a, b);
+        else return 0u;
+    }
+};
 
-// 2^y for y <= 0 to about 1e-13: y = k/256 + r, a table of 2^(j/256) and the
-// series of e^(r ln 2) to the third power (|r ln 2| < 1.4e-3).
+// 2^y for -1010 < y <= 1 to about 1e-13: y = k/256 + r, a table of 2^(j/256)
+// and the series of e^(r ln 2) to the third power (|r ln 2| < 1.4e-3).  k
+// comes out of the low word of y * 256 + 1.5 * 2^52, which rounds there.
 __device__ __forceinline__ double exp2_table(double y, const double* table) {
-    if (!(y > -1000.0)) return 0.0;
-    const double k = rint(y * 256.0);
-    const double r = fma(k, -1.0 / 256.0, y) * 0.69314718055994530942;
-    const int ki = (int)k;
+    const double big = 6755399441055744.0;
+    const double t = fma(y, 256.0, big);
+    const int ki = __double2loint(t);
+    const double r = fma(t - big, -1.0 / 256.0, y) * 0.69314718055994530942;
     const double p = fma(r, fma(r, fma(r, 1.0 / 6.0, 0.5), 1.0), 1.0) * table[ki & 255];
     return __hiloint2double(__double2hiint(p) + ((ki >> 8) << 20), __double2loint(p));
+}
+// 2^((v - m) c) for a logit v; exactly zero far below m (v <= low), and for NaN.
+__device__ __forceinline__ double logit_weight(float v, float low, double c, double mc, const double* table) {
+    const double w = exp2_table(fma((double)fmaxf(v, low), c, -mc), table);
+    return v > low ? w : 0.0;
+}
+
+// Two fp32 numbers, added and multiplied side by side.
+struct F2 {
+    unsigned long long w;
+    __device__ __forceinline__ F2() : w(0ull) {}
+    __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(w) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(w)); }
+};
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.w) : "l"(a.w), "l"(b.w));
+    return d;
+}
+__device__ __forceinline__ F2 sub2(F2 a, F2 b) {  // a - b, rounded once
+    F2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.w) : "l"(b.w), "l"(F2(-1.0f, -1.0f).w), "l"(a.w));
+    return d;
+}
+
+// Sum of max(p - q, 0) over a lane's E entries of each of four vectors, in
+// fp32 pairs (s, c) whose s + c is exact to 2^-48: the difference of p >= q
+// >= 0 is hi + lo without error, and so is each addition's own error.  On
+// fp64 units the two conversions of each entry alone would take 4 us for a
+// batch of 64 on 128 K entries.
+template <typename T, int E>
+__device__ __forceinline__ double rest_sum(const RowPart<T, E>& xp, const RowPart<T, E>& xq, bool two) {
+    static_assert(E % 2 == 0, "pairs");
+    F2 s, c;
+#pragma unroll
+    for (int k = 0; k < VER_VECS; ++k) {
+        float p[E], q[E];
+        to_float(xp.v[k], p);
+        if (two) to_float(xq.v[k], q);
+#pragma unroll
+        for (int j = 0; j < E; j += 2) {
+            const float p0 = fmaxf(p[j], 0.0f), p1 = fmaxf(p[j + 1], 0.0f);  // NaN too
+            F2 hi(p0, p1), lo;
+            if (two) {  // q clipped into [0, p]: the difference is not below zero
+                const F2 P = hi, Q(fminf(fmaxf(q[j], 0.0f), p0), fminf(fmaxf(q[j + 1], 0.0f), p1));
+                hi = sub2(P, Q);
+                lo = sub2(sub2(P, hi), Q);
+            }
+            const F2 t = add2(s, hi), z = sub2(t, s);
+            const F2 err = add2(sub2(s, sub2(t, z)), sub2(hi, z));
+            s = t;
+            c = add2(c, err);
+            if (two) c = add2(c, lo);
+        }
+    }
+    float s0, s1, c0, c1;
+    s.get(s0, s1);
+    c.get(c0, c1);
+    return ((double)s0 + (double)c0) + ((double)s1 + (double)c1);
 }
 
 __device__ __forceinline__ double warp_sum_f64(double v) {
@@ -86,7 +176,7 @@ __device__ __forceinline__ unsigned long long argmax_key64(float v, uint32_t i) 
 }
 
 template <typename T, int KIND>
-__global__ void __launch_bounds__(VER_THREADS) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs a) {
     namespace cg = cooperative_groups;
     constexpr int E = 16 / sizeof(T);
     cg::cluster_group cluster = cg::this_cluster();
@@ -98,8 +188,9 @@ __global__ void __launch_bounds__(VER_THREADS) verify_kernel(const VerifyArgs a)
     __shared__ unsigned long long s_part[ROWS * VER_WARPS];       // phase A: this CTA's parts of each row
     __shared__ unsigned long long s_stat[ROWS * VER_MAX_CL];      // phase A: every CTA's share of each row
     __shared__ double s_sum[2][VER_MAX_CL * VER_WARPS];           // segment sums of target and draft
-    __shared__ float s_max[2][VER_MAX_CL * VER_WARPS];
+    __shared__ float s_max[VER_MAX_CL * VER_WARPS];
     __shared__ double s_rest[2][VER_MAX_CL * VER_WARPS];          // segment sums of what is drawn from
+    __shared__ double s_chunk[VER_WARPS][VER_CHUNKS];             // this CTA's chunk sums
     __shared__ double s_table[256];
     __shared__ double s_z[2], s_thr;
     __shared__ float s_m[2];
@@ -107,7 +198,7 @@ __global__ void __launch_bounds__(VER_THREADS) verify_kernel(const VerifyArgs a)
 
     const T* target = reinterpret_cast<const T*>(a.target) + b * a.t_seq;
     const T* draft = a.draft && KIND != VER_GREEDY ? reinterpret_cast<const T*>(a.draft) + b * a.d_seq : nullptr;
-    cluster.sync();  // every CTA of the cluster runs before its shared memory is written to
+    cluster.barrier_arrive();  // every CTA of the cluster runs before its shared memory is written to
 
     // lane i of the first warp keeps draft i
     uint32_t x = 0, len = 0;
@@ -132,11 +223,13 @@ __global__ void __launch_bounds__(VER_THREADS) verify_kernel(const VerifyArgs a)
     if (KIND == VER_LOGITS)
         if (tid < 256) s_table[tid] = exp2((double)tid / 256.0);
 
+    uint32_t Rt = 0;  // rows of the target among those that phase A sums
     // ---- phase A: what the accepting tests need of whole rows ----------------------
     if (KIND != VER_PROBS) {
         __syncthreads();
         len = s_len;
-        const uint32_t Rt = KIND == VER_GREEDY ? len + 1 : len, R = Rt + (draft ? len : 0);
+        Rt = KIND == VER_GREEDY ? len + 1 : len;
+        const uint32_t R = Rt + (draft ? len : 0);
         const uint32_t P = R ? max(1u, VER_WARPS / R) : 1u;  // warps on one row
         const uint32_t share = (((V + CL - 1) / CL) + 7) & ~7u, c0 = min(rank * share, V), c1 = min(c0 + share, V);
         const uint32_t psz = (((c1 - c0 + P - 1) / P) + 7) & ~7u;
@@ -145,13 +238,18 @@ __global__ void __launch_bounds__(VER_THREADS) verify_kernel(const VerifyArgs a)
             const T* row = r < Rt ? target + r * a.t_row : draft + (r - Rt) * a.d_row;
             if (KIND == VER_GREEDY) {
                 unsigned long long best = 0;
-                for (uint32_t i = p0 + lane * E; i < p1; i += 32 * E) {
-                    float v[E];
-                    load_row<T, E>(row, i, p1, a.vec, __int_as_float(0x7fffffff), v);
+                for (uint32_t i0 = p0; i0 < p1; i0 += VER_VECS * 32 * E) {
+                    RowPart<T, E> x;
+                    x.load(row, i0, p1, a.vec, __int_as_float(0x7fffffff));
 #pragma unroll
-                    for (int j = 0; j < E; ++j) {
-                        const unsigned long long k = argmax_key64(v[j], i + j);
-                        best = k > best ? k : best;
+                    for (int k = 0; k < VER_VECS; ++k) {
+                        float v[E];
+                        to_float(x.v[k], v);
+#pragma unroll
+                        for (int j = 0; j < E; ++j) {
+                            const unsigned long long key = argmax_key64(v[j], i0 + (k * 32 + lane) * E + j);
+                            best = key > best ? key : best;
+                        }
                     }
                 }
 #pragma unroll
@@ -161,36 +259,41 @@ __global__ void __launch_bounds__(VER_THREADS) verify_kernel(const VerifyArgs a)
                 }
                 if (lane == 0) s_part[it] = best;
             } else {
-                float m = -INFINITY, s = 0.0f;  // of y = logit * c, the softmax in powers of two
-                for (uint32_t i = p0 + lane * E; i < p1; i += 32 * E) {
-                    float v[E], mx = m;
-                    load_row<T, E>(row, i, p1, a.vec, -INFINITY, v);
+                float m = -INFINITY, s = 0.0f;  // sum of 2^((logit - m) c)
+                for (uint32_t i0 = p0; i0 < p1; i0 += VER_VECS * 32 * E) {
+                    RowPart<T, E> x;
+                    x.load(row, i0, p1, a.vec, -INFINITY);
+                    float mx = m, add = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < E; ++j) {
-                        v[j] *= a.c;
-                        mx = fmaxf(mx, v[j]);
+                    for (int k = 0; k < VER_VECS; ++k) {
+                        float v[E];
+                        to_float(x.v[k], v);
+#pragma unroll
+                        for (int j = 0; j < E; ++j) mx = fmaxf(mx, v[j]);
                     }
                     if (mx == -INFINITY) continue;
-                    float add = 0.0f;
 #pragma unroll
-                    for (int j = 0; j < E; ++j) {
-                        const float e = exp2f(v[j] - mx);
-                        add += e > 0.0f ? e : 0.0f;  // NaN counts as zero
+                    for (int k = 0; k < VER_VECS; ++k) {
+                        float v[E];
+                        to_float(x.v[k], v);
+#pragma unroll
+                        for (int j = 0; j < E; ++j) add += ex2((fmaxf(v[j], -INFINITY) - mx) * a.c);  // NaN counts as zero
                     }
-                    s = s * exp2f(m - mx) + add;
+                    s = s * ex2((m - mx) * a.c) + add;
                     m = mx;
                 }
 #pragma unroll
                 for (int o = 16; o > 0; o >>= 1) {
                     const float m2 = __shfl_xor_sync(0xffffffffu, m, o), s2 = __shfl_xor_sync(0xffffffffu, s, o);
                     const float mm = fmaxf(m, m2);
-                    if (mm != -INFINITY) s = s * exp2f(m - mm) + s2 * exp2f(m2 - mm);
+                    if (mm != -INFINITY) s = s * ex2((m - mm) * a.c) + s2 * ex2((m2 - mm) * a.c);
                     m = mm;
                 }
                 if (lane == 0) s_part[it] = ((unsigned long long)__float_as_uint(m) << 32) | __float_as_uint(s);
             }
         }
         __syncthreads();
+        cluster.barrier_wait();
         for (uint32_t e = tid; e < R * CL; e += VER_THREADS) {  // row e / CL to CTA e % CL
             const uint32_t r = e / CL, to = e - r * CL;
             unsigned long long w = s_part[r * P];
@@ -202,7 +305,7 @@ __global__ void __launch_bounds__(VER_THREADS) verify_kernel(const VerifyArgs a)
                     const float m = __uint_as_float((uint32_t)(w >> 32)), m2 = __uint_as_float((uint32_t)(w2 >> 32));
                     float s = __uint_as_float((uint32_t)w);
                     const float mm = fmaxf(m, m2);
-                    if (mm != -INFINITY) s = s * exp2f(m - mm) + __uint_as_float((uint32_t)w2) * exp2f(m2 - mm);
+                    if (mm != -INFINITY) s = s * ex2((m - mm) * a.c) + __uint_as_float((uint32_t)w2) * ex2((m2 - mm) * a.c);
                     w = ((unsigned long long)__float_as_uint(mm) << 32) | __float_as_uint(s);
                 }
             }
@@ -235,9 +338,9 @@ __global__ void __launch_bounds__(VER_THREADS) verify_kernel(const VerifyArgs a)
                     for (uint32_t k = 0; k < CL; ++k) {
                         const unsigned long long w = s_stat[r * VER_MAX_CL + k];
                         const float mk = __uint_as_float((uint32_t)(w >> 32));
-                        if (mk != -INFINITY) s += (double)__uint_as_float((uint32_t)w) * (double)exp2f(mk - m);
+                        if (mk != -INFINITY) s += (double)__uint_as_float((uint32_t)w) * (double)ex2((mk - m) * a.c);
                     }
-                    const double e = exp2((double)logit * a.cd - (double)m);
+                    const double e = exp2(((double)logit - (double)m) * a.cd);
                     return s > 0.0 && e > 0.0 ? e / s : 0.0;
                 };
                 bool ok = false;
@@ -271,66 +374,82 @@ __global__ void __launch_bounds__(VER_THREADS) verify_kernel(const VerifyArgs a)
     const uint32_t g = rank * VER_WARPS + warp, segs = CL * VER_WARPS;
     const uint32_t g0 = min(g * a.seg, V), g1 = min(g0 + a.seg, V);
 
-    if (KIND == VER_LOGITS) {  // the two rows' maxima and sums, in fp64
+    if (KIND == VER_LOGITS) {  // the two rows' sums, in fp64
+        float m[2];
+        for (int k = 0; k < 2; ++k) {  // any reference near the maximum does
+            m[k] = -INFINITY;
+            const uint32_t r = k ? Rt + n : n;
+            if (n < len && (k == 0 || qrow))
+                for (uint32_t c = 0; c < CL; ++c) m[k] = fmaxf(m[k], __uint_as_float((uint32_t)(s_stat[r * VER_MAX_CL + c] >> 32)));
+        }
+        if (n >= len) {  // a row that no test has looked at
+            float top = -INFINITY;
+            for (uint32_t i0 = g0; i0 < g1; i0 += VER_VECS * 32 * E) {
+                RowPart<T, E> x;
+                x.load(prow, i0, g1, a.vec, -INFINITY);
+#pragma unroll
+                for (int k = 0; k < VER_VECS; ++k) {
+                    float v[E];
+                    to_float(x.v[k], v);
+#pragma unroll
+                    for (int j = 0; j < E; ++j) top = fmaxf(top, v[j]);
+                }
+            }
+            top = warp_max(top);
+            if (lane < CL) *cluster.map_shared_rank(&s_max[g], lane) = top;
+            cluster.sync();
+            for (uint32_t i = lane; i < segs; i += 32) m[0] = fmaxf(m[0], s_max[i]);
+            m[0] = warp_max(m[0]);
+        }
         for (int k = 0; k < 2; ++k) {
             const T* row = k ? qrow : prow;
-            float m = -INFINITY;
+            const double mc = (double)m[k] * a.cd;
+            const float low = m[k] - 1000.0f / a.c;
             double s = 0.0;
-            if (row) {
-                for (uint32_t i = g0 + lane * E; i < g1; i += 32 * E) {
-                    float v[E];
-                    load_row<T, E>(row, i, g1, a.vec, -INFINITY, v);
+            if (row && m[k] > -INFINITY && m[k] < INFINITY)
+                for (uint32_t i0 = g0; i0 < g1; i0 += VER_VECS * 32 * E) {
+                    RowPart<T, E> x;
+                    x.load(row, i0, g1, a.vec, -INFINITY);
 #pragma unroll
-                    for (int j = 0; j < E; ++j) m = fmaxf(m, v[j]);
-                }
-                m = warp_max(m);
-                if (m > -INFINITY && m < INFINITY)
-                    for (uint32_t i = g0 + lane * E; i < g1; i += 32 * E) {
+                    for (int q = 0; q < VER_VECS; ++q) {
                         float v[E];
-                        load_row<T, E>(row, i, g1, a.vec, -INFINITY, v);
+                        to_float(x.v[q], v);
 #pragma unroll
-                        for (int j = 0; j < E; ++j) s += exp2_table(((double)v[j] - (double)m) * a.cd, s_table);
+                        for (int j = 0; j < E; ++j) s += logit_weight(v[j], low, a.cd, mc, s_table);
                     }
-                s = warp_sum_f64(s);
-            }
-            if (lane < CL) {
-                *cluster.map_shared_rank(&s_max[k][g], lane) = m;
-                *cluster.map_shared_rank(&s_sum[k][g], lane) = s;
-            }
+                }
+            s = warp_sum_f64(s);
+            if (lane < CL) *cluster.map_shared_rank(&s_sum[k][g], lane) = s;
+            if (tid == 0) s_m[k] = m[k];
         }
         cluster.sync();
         if (warp < 2) {
-            float m = -INFINITY;
-            for (uint32_t i = lane; i < segs; i += 32) m = fmaxf(m, s_max[warp][i]);
-            m = warp_max(m);
             double z = 0.0;
-            for (uint32_t i = lane; i < segs; i += 32)
-                z += s_sum[warp][i] * exp2_table(((double)s_max[warp][i] - (double)m) * a.cd, s_table);
+            for (uint32_t i = lane; i < segs; i += 32) z += s_sum[warp][i];
             z = warp_sum_f64(z);
-            if (lane == 0) {
-                s_m[warp] = m;
-                s_z[warp] = z > 0.0 ? 1.0 / z : 0.0;
-            }
+            if (lane == 0) s_z[warp] = z > 0.0 ? 1.0 / z : 0.0;
         }
         __syncthreads();
     }
-    const double mp = KIND == VER_LOGITS ? (double)s_m[0] : 0.0, mq = KIND == VER_LOGITS ? (double)s_m[1] : 0.0;
+    const double mp = KIND == VER_LOGITS ? (double)s_m[0] * a.cd : 0.0, mq = KIND == VER_LOGITS ? (double)s_m[1] * a.cd : 0.0;
+    const float lp = KIND == VER_LOGITS ? s_m[0] - 1000.0f / a.c : 0.0f, lq = KIND == VER_LOGITS ? s_m[1] - 1000.0f / a.c : 0.0f;
     const double zp = KIND == VER_LOGITS ? s_z[0] : 1.0, zq = KIND == VER_LOGITS ? s_z[1] : 1.0;
-    // weights of entries i.. in fp64; past the end and NaN: zero
-    auto weights = [&](uint32_t i, bool rest, double (&w)[E]) {
+    // weights in fp64 of E entries from index i on; past the end and NaN: zero
+    const float none = KIND == VER_LOGITS ? -INFINITY : 0.0f;
+    auto weights = [&](const Vec<T, E>& vp, const Vec<T, E>& vq, uint32_t i, bool rest, double (&w)[E]) {
         float p[E], q[E];
-        load_row<T, E>(prow, i, g1, a.vec, KIND == VER_LOGITS ? -INFINITY : 0.0f, p);
+        to_float(vp, p);
         const bool two = rest && qrow;
-        if (two) load_row<T, E>(qrow, i, g1, a.vec, KIND == VER_LOGITS ? -INFINITY : 0.0f, q);
+        if (two) to_float(vq, q);
 #pragma unroll
         for (int j = 0; j < E; ++j) {
             double d;
             if (KIND == VER_LOGITS) {
-                d = exp2_table(((double)p[j] - mp) * a.cd, s_table) * zp;
-                if (two) d -= exp2_table(((double)q[j] - mq) * a.cd, s_table) * zq;
+                d = logit_weight(p[j], lp, a.cd, mp, s_table) * zp;
+                if (two) d -= logit_weight(q[j], lq, a.cd, mq, s_table) * zq;
             } else {
                 d = (double)p[j];
-                if (two && q[j] > 0.0f) d -= (double)q[j];
+                if (two) d -= (double)fmaxf(q[j], 0.0f);  // also where q is no number
             }
             w[j] = d > 0.0 && !(rest && i + j == gone) ? d : 0.0;
         }
@@ -338,14 +457,33 @@ __global__ void __launch_bounds__(VER_THREADS) verify_kernel(const VerifyArgs a)
 
     bool rest = n < len;
     for (int round = 0; round < 2; ++round) {
+        // chunk after chunk; their sums show the search where to begin
+        if (lane < VER_CHUNKS) s_chunk[warp][lane] = 0.0;
+        __syncwarp();
+        const bool two = rest && qrow;
         double sum = 0.0;
-        for (uint32_t i = g0 + lane * E; i < g1; i += 32 * E) {
-            double w[E];
-            weights(i, rest, w);
+        for (uint32_t i0 = g0, chunk = 0; i0 < g1; i0 += VER_VECS * 32 * E, ++chunk) {
+            RowPart<T, E> xp, xq;
+            xp.load(prow, i0, g1, a.vec, none);
+            if (two) xq.load(qrow, i0, g1, a.vec, none);
+            double part = 0.0;
+            if (KIND == VER_PROBS && !(rest && gone - i0 < VER_VECS * 32 * E)) {
+                part = rest_sum(xp, xq, two);
+            } else {
 #pragma unroll
-            for (int j = 0; j < E; ++j) sum += w[j];
+                for (int k = 0; k < VER_VECS; ++k) {
+                    double w[E];
+                    weights(xp.v[k], xq.v[k], i0 + (k * 32 + lane) * E, rest, w);
+#pragma unroll
+                    for (int j = 0; j < E; ++j) part += w[j];
+                }
+            }
+            part = warp_sum_f64(part);
+            if (lane == 0) s_chunk[warp][min(chunk, VER_CHUNKS - 1)] += part;
+            sum += part;
         }
-        sum = warp_sum_f64(sum);
+        __syncwarp();
+        if (KIND == VER_PROBS && round == 0) cluster.barrier_wait();
         if (lane < CL) *cluster.map_shared_rank(&s_rest[round][g], lane) = sum;
         cluster.sync();
         if (warp == 0) {  // lane l adds segments 8l.., then the lanes in order
@@ -400,44 +538,58 @@ __global__ void __launch_bounds__(VER_THREADS) verify_kernel(const VerifyArgs a)
     if (owner) {
         const double thr = s_thr;
         double at = 0.0;
+        uint32_t c0 = g0;
+        for (uint32_t k = 0; k + 1 < VER_CHUNKS && c0 + VER_VECS * 32 * E < g1 && !(at + s_chunk[warp][k] > thr); ++k) {
+            at += s_chunk[warp][k];
+            c0 += VER_VECS * 32 * E;
+        }
         bool found = false;
-        for (uint32_t i0 = g0; i0 < g1 && !found; i0 += 32 * E) {
-            double w[E], run = 0.0;
-            weights(i0 + lane * E, rest, w);
-            uint32_t last = 0;
+        for (uint32_t pass = 0; pass < 2 && !found; ++pass) {
+            // the second pass, for a border that rounding hid: the segment's last weight
+            if (pass) c0 = g0, at = -INFINITY;
+            for (; c0 < g1 && !found; c0 += VER_VECS * 32 * E) {
+                RowPart<T, E> xp, xq;
+                xp.load(prow, c0, g1, a.vec, none);
+                if (rest && qrow) xq.load(qrow, c0, g1, a.vec, none);
+#pragma unroll 1
+                for (int k = 0; k < VER_VECS && !found; ++k) {
+                    Vec<T, E> vp = xp.v[0], vq = xq.v[0];
 #pragma unroll
-            for (int j = 0; j < E; ++j) {
-                run += w[j];
-                if (w[j] > 0.0) last = i0 + lane * E + j + 1;
-            }
-            double incl = run;
+                    for (int q = 1; q < VER_VECS; ++q)
+                        if (k == q) vp = xp.v[q], vq = xq.v[q];
+                    const uint32_t i = c0 + (k * 32 + lane) * E;
+                    double w[E], run = 0.0;
+                    weights(vp, vq, i, rest, w);
 #pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const double t = __shfl_up_sync(0xffffffffu, incl, o);
-                if (lane >= (uint32_t)o) incl += t;
-            }
-            double before = __shfl_up_sync(0xffffffffu, incl, 1);
-            if (lane == 0) before = 0.0;
-            const uint32_t vote = __ballot_sync(0xffffffffu, run > 0.0 && at + incl > thr);
-            const uint32_t lasts = __reduce_max_sync(0xffffffffu, last);
-            if (lasts) token = lasts - 1;  // stays where no border is met
-            if (vote) {
-                const uint32_t from = __ffs(vote) - 1;
-                uint32_t mine = last ? last - 1 : 0;
-                double c = at + before;
-                bool met = false;
+                    for (int j = 0; j < E; ++j) run += w[j];
+                    double incl = run;
 #pragma unroll
-                for (int j = 0; j < E; ++j) {
-                    c += w[j];
-                    if (!met && w[j] > 0.0 && c > thr) {
-                        mine = i0 + lane * E + j;
-                        met = true;
+                    for (int o = 1; o < 32; o <<= 1) {
+                        const double t = __shfl_up_sync(0xffffffffu, incl, o);
+                        if (lane >= (uint32_t)o) incl += t;
                     }
+                    const uint32_t has = __ballot_sync(0xffffffffu, run > 0.0);
+                    const uint32_t vote = __ballot_sync(0xffffffffu, run > 0.0 && at + incl > thr);
+                    if (has) {  // the lane with the border; without one, the last that has weight
+                        const uint32_t from = vote ? __ffs(vote) - 1 : 31 - __clz(has);
+                        double c = __shfl_up_sync(0xffffffffu, incl, 1);
+                        c = at + (lane == 0 ? 0.0 : c);
+                        uint32_t mine = 0;
+                        bool met = false;
+#pragma unroll
+                        for (int j = 0; j < E; ++j) {
+                            c += w[j];
+                            if (!met && w[j] > 0.0) {
+                                mine = i + j;
+                                met = c > thr;
+                            }
+                        }
+                        token = __shfl_sync(0xffffffffu, mine, from);
+                        found = vote != 0;
+                    }
+                    at += __shfl_sync(0xffffffffu, incl, 31);
                 }
-                token = __shfl_sync(0xffffffffu, mine, from);
-                found = true;
             }
-            at += __shfl_sync(0xffffffffu, incl, 31);
         }
         if (lane == 0) a.tokens[(size_t)b * (K + 1) + n] = token;
     }
