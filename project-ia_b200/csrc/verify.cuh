@@ -34,7 +34,8 @@ static constexpr uint32_t VER_MAX_CL = 16;
 static constexpr uint32_t VER_MAX_DRAFT = 31;
 static constexpr uint32_t VER_CHUNKS = 16;  // sums that a warp keeps of its segment's chunks, the last one of all behind
 
-static constexpr int VER_VECS = 2;  // vectors of a row that a lane has under way
+static constexpr int VER_VECS = 2;  // vectors of each of two rows that a lane has under way
+static constexpr int VER_SUMS = 8;  // of one row, where whole rows are summed
 
 enum : int { VER_PROBS = 0, VER_LOGITS = 1, VER_GREEDY = 2 };
 
@@ -53,28 +54,28 @@ struct VerifyArgs {
     double cd;
 };
 
-// A lane's share of VER_VECS * 32 E consecutive entries of a row from i0 on:
+// A lane's share of NV * 32 E consecutive entries of a row from i0 on:
 // 16-byte vectors of E, 32 E apart; `none` past the end.  A vector past the
 // end is loaded from the row's start instead and replaced, so that all loads
 // are issued before the first is looked at.
-template <typename T, int E>
+template <typename T, int E, int NV = VER_VECS>
 struct RowPart {
-    Vec<T, E> v[VER_VECS];
+    Vec<T, E> v[NV];
     __device__ __forceinline__ void load(const T* row, uint32_t i0, uint32_t end, bool vec, float none) {
         const uint32_t i = i0 + (threadIdx.x & 31) * E;
         const uint32_t fill = sizeof(T) == 4 ? __float_as_uint(none) : word<T>(none, none);
         if (vec) {
 #pragma unroll
-            for (int k = 0; k < VER_VECS; ++k) v[k] = load_raw<T, E>(row + (i + k * 32 * E + E <= end ? i + k * 32 * E : 0u));
+            for (int k = 0; k < NV; ++k) v[k] = load_raw<T, E>(row + (i + k * 32 * E + E <= end ? i + k * 32 * E : 0u));
 #pragma unroll
-            for (int k = 0; k < VER_VECS; ++k)
+            for (int k = 0; k < NV; ++k)
                 if (i + k * 32 * E + E > end)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) v[k].w[j] = fill;
-            if (i0 + VER_VECS * 32 * E <= end || end % E == 0) return;
+            if (i0 + NV * 32 * E <= end || end % E == 0) return;
         }
 #pragma unroll
-        for (int k = 0; k < VER_VECS; ++k) {  // entry by entry: rows that are not aligned, the last vector of others
+        for (int k = 0; k < NV; ++k) {  // entry by entry: rows that are not aligned, the last vector of others
             const uint32_t at = i + k * 32 * E;
             if (vec && (at + E <= end || at >= end)) continue;
             float x[E];
@@ -90,18 +91,21 @@ struct RowPart {
     }
 };
 
-// 2^y for -1010 < y <= 1 to about 1e-13: y = k/256 + r, a table of 2^(j/256)
-// and the series of e^(r ln 2) to the third power (|r ln 2| < 1.4e-3).  k
-// comes out of the low word of y * 256 + 1.5 * 2^52, which rounds there.
+// 2^(y / 1024) for -1010 < y / 1024 <= 1 to about 1e-11: y = k + r, a table
+// of 2^(j/1024) and the series of e^(r ln 2 / 1024) to the second power
+// (its argument is below 3.4e-4).  k comes out of the low word of
+// y + 1.5 * 2^52, which rounds there.
+static constexpr uint32_t VER_TABLE = 1024;
 __device__ __forceinline__ double exp2_table(double y, const double* table) {
     const double big = 6755399441055744.0;
-    const double t = fma(y, 256.0, big);
+    const double t = y + big, r = y - (t - big);
     const int ki = __double2loint(t);
-    const double r = fma(t - big, -1.0 / 256.0, y) * 0.69314718055994530942;
-    const double p = fma(r, fma(r, fma(r, 1.0 / 6.0, 0.5), 1.0), 1.0) * table[ki & 255];
-    return __hiloint2double(__double2hiint(p) + ((ki >> 8) << 20), __double2loint(p));
+    constexpr double c1 = 0.69314718055994530942 / VER_TABLE, c2 = c1 * c1 / 2.0;
+    const double p = fma(r, fma(r, c2, c1), 1.0) * table[ki & (VER_TABLE - 1)];
+    return __hiloint2double(__double2hiint(p) + ((ki >> 10) << 20), __double2loint(p));
 }
-// 2^((v - m) c) for a logit v; exactly zero far below m (v <= low), and for NaN.
+// 2^((v - m) c) for a logit v, with c and m c times 1024; exactly zero far
+// below m (v <= low), and for NaN.
 __device__ __forceinline__ double logit_weight(float v, float low, double c, double mc, const double* table) {
     const double w = exp2_table(fma((double)fmaxf(v, low), c, -mc), table);
     return v > low ? w : 0.0;
@@ -191,7 +195,7 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
     __shared__ float s_max[VER_MAX_CL * VER_WARPS];
     __shared__ double s_rest[2][VER_MAX_CL * VER_WARPS];          // segment sums of what is drawn from
     __shared__ double s_chunk[VER_WARPS][VER_CHUNKS];             // this CTA's chunk sums
-    __shared__ double s_table[256];
+    __shared__ double s_table[KIND == VER_LOGITS ? VER_TABLE : 1];
     __shared__ double s_z[2], s_thr;
     __shared__ float s_m[2];
     __shared__ uint32_t s_n, s_owner, s_len;
@@ -221,7 +225,7 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
         }
     }
     if (KIND == VER_LOGITS)
-        if (tid < 256) s_table[tid] = exp2((double)tid / 256.0);
+        for (uint32_t i = tid; i < VER_TABLE; i += VER_THREADS) s_table[i] = exp2((double)i / VER_TABLE);
 
     uint32_t Rt = 0;  // rows of the target among those that phase A sums
     // ---- phase A: what the accepting tests need of whole rows ----------------------
@@ -238,11 +242,11 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
             const T* row = r < Rt ? target + r * a.t_row : draft + (r - Rt) * a.d_row;
             if (KIND == VER_GREEDY) {
                 unsigned long long best = 0;
-                for (uint32_t i0 = p0; i0 < p1; i0 += VER_VECS * 32 * E) {
-                    RowPart<T, E> x;
+                for (uint32_t i0 = p0; i0 < p1; i0 += VER_SUMS * 32 * E) {
+                    RowPart<T, E, VER_SUMS> x;
                     x.load(row, i0, p1, a.vec, __int_as_float(0x7fffffff));
 #pragma unroll
-                    for (int k = 0; k < VER_VECS; ++k) {
+                    for (int k = 0; k < VER_SUMS; ++k) {
                         float v[E];
                         to_float(x.v[k], v);
 #pragma unroll
@@ -260,12 +264,12 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
                 if (lane == 0) s_part[it] = best;
             } else {
                 float m = -INFINITY, s = 0.0f;  // sum of 2^((logit - m) c)
-                for (uint32_t i0 = p0; i0 < p1; i0 += VER_VECS * 32 * E) {
-                    RowPart<T, E> x;
+                for (uint32_t i0 = p0; i0 < p1; i0 += VER_SUMS * 32 * E) {
+                    RowPart<T, E, VER_SUMS> x;
                     x.load(row, i0, p1, a.vec, -INFINITY);
                     float mx = m, add = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < VER_VECS; ++k) {
+                    for (int k = 0; k < VER_SUMS; ++k) {
                         float v[E];
                         to_float(x.v[k], v);
 #pragma unroll
@@ -273,7 +277,7 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
                     }
                     if (mx == -INFINITY) continue;
 #pragma unroll
-                    for (int k = 0; k < VER_VECS; ++k) {
+                    for (int k = 0; k < VER_SUMS; ++k) {
                         float v[E];
                         to_float(x.v[k], v);
 #pragma unroll
@@ -371,6 +375,7 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
     const T* qrow = draft && n < len ? draft + n * a.d_row : nullptr;
     // a draft without probabilities takes its own token out of the row
     const uint32_t gone = !draft && n < len ? __ldg(a.draft_tokens + (size_t)b * K + n) : ~0u;
+    const double ct = a.cd * VER_TABLE;
     const uint32_t g = rank * VER_WARPS + warp, segs = CL * VER_WARPS;
     const uint32_t g0 = min(g * a.seg, V), g1 = min(g0 + a.seg, V);
 
@@ -403,7 +408,7 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
         }
         for (int k = 0; k < 2; ++k) {
             const T* row = k ? qrow : prow;
-            const double mc = (double)m[k] * a.cd;
+            const double mc = (double)m[k] * ct;
             const float low = m[k] - 1000.0f / a.c;
             double s = 0.0;
             if (row && m[k] > -INFINITY && m[k] < INFINITY)
@@ -415,7 +420,7 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
                         float v[E];
                         to_float(x.v[q], v);
 #pragma unroll
-                        for (int j = 0; j < E; ++j) s += logit_weight(v[j], low, a.cd, mc, s_table);
+                        for (int j = 0; j < E; ++j) s += logit_weight(v[j], low, ct, mc, s_table);
                     }
                 }
             s = warp_sum_f64(s);
@@ -431,7 +436,7 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
         }
         __syncthreads();
     }
-    const double mp = KIND == VER_LOGITS ? (double)s_m[0] * a.cd : 0.0, mq = KIND == VER_LOGITS ? (double)s_m[1] * a.cd : 0.0;
+    const double mp = KIND == VER_LOGITS ? (double)s_m[0] * ct : 0.0, mq = KIND == VER_LOGITS ? (double)s_m[1] * ct : 0.0;
     const float lp = KIND == VER_LOGITS ? s_m[0] - 1000.0f / a.c : 0.0f, lq = KIND == VER_LOGITS ? s_m[1] - 1000.0f / a.c : 0.0f;
     const double zp = KIND == VER_LOGITS ? s_z[0] : 1.0, zq = KIND == VER_LOGITS ? s_z[1] : 1.0;
     // weights in fp64 of E entries from index i on; past the end and NaN: zero
@@ -445,8 +450,8 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
         for (int j = 0; j < E; ++j) {
             double d;
             if (KIND == VER_LOGITS) {
-                d = logit_weight(p[j], lp, a.cd, mp, s_table) * zp;
-                if (two) d -= logit_weight(q[j], lq, a.cd, mq, s_table) * zq;
+                d = logit_weight(p[j], lp, ct, mp, s_table) * zp;
+                if (two) d -= logit_weight(q[j], lq, ct, mq, s_table) * zq;
             } else {
                 d = (double)p[j];
                 if (two) d -= (double)fmaxf(q[j], 0.0f);  // also where q is no number
