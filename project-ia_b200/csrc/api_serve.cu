@@ -326,8 +326,8 @@ AttnPass plan_tc(uint32_t vecs, uint32_t kv_heads, uint32_t rows) {
     p.alternate = vecs <= 128;
     p.tiles = p.items = cdiv(vecs, p.alternate ? 128 : 256);
     const uint32_t ctas = p.items * kv_heads;
-    p.splits = std::min({std::max(1u, 148 / ctas), std::max(1u, cdiv(rows, 2 * TC_ROWS)), ATTN_MAX_PARTS / 2});
-    p.parts = p.alternate ? 2 * p.splits : p.splits;
+    p.splits = std::min({std::max(1u, 148 / ctas), std::max(1u, cdiv(rows, 2 * TC_ROWS)), ATTN_MAX_PARTS});
+    p.parts = p.splits;
     return p;
 }
 

@@ -4,11 +4,15 @@
 // All new tokens' query vectors of a KV head (tokens x G heads) meet the same
 // rows, so the pass is a matrix product: S = Q K^T and O += P V with 128
 // query vectors as the MMA's M, 128 rows of the cache as one tile.  One CTA
-// runs two streams, each with scores and an output of its own in TMEM
-// (columns [0,128) and [128,256): S0, S1; [256,..) and [384,..): O0, O1):
+// runs two streams, each with scores and an output of its own in TMEM:
 //   two tiles of vectors, the same rows (more than 128 vectors), or
-//   one tile of vectors, even and odd row tiles (up to 128),
-// so that one stream's products run while the other's exponentials do.
+//   one tile of vectors, even and odd row tiles (up to 128; joined at the end),
+// and each stream takes a row tile in two halves of 64 rows with a score
+// buffer each, so that the products for one half run while the exponentials
+// of the other do (columns: S[stream][half] at 128 stream + 64 half, O at 256
+// + 128 stream).  With one buffer of 128 rows a stream, products and
+// exponentials of a stream took turns: 105 us where this takes 50 (512
+// vectors x 32768 rows x 8 KV heads, head_dim 128).
 //
 // Roles: warps 0-3 and 4-7 are the streams' softmax, a thread per vector
 // (its row of S lies in its own TMEM lane, so maximum and sum need no
@@ -18,14 +22,13 @@
 // in 16 bits (the operand type) and is the A operand of P V from there; V is
 // used as it lies in the cache, [row][dim], as an MN-major B operand.
 //
-// The running maximum moves only when a row tile exceeds it by 2^8: then the
+// The running maximum moves only when a half tile exceeds it by 2^8: then the
 // output is rescaled in TMEM; until then exponentials may reach 256, which
 // fp16 holds, and the quotient o / l is the same.
 //
 // Bound: for up to 128 vectors the bytes of K and V; beyond, the tensor pipe
-// (4 x 128 x 128 x head_dim flops a tile) beside the exponentials (128 x 128
-// of them a tile on 16 lanes of the special function unit: as long as the
-// products at head_dim 128).
+// and, at head_dim 128 nearly as long, the exponentials (128 x 128 of them a
+// tile and stream on 16 lanes of the special function unit).
 #pragma once
 
 #include "attn_prefix.cuh"
@@ -34,7 +37,7 @@
 namespace qb200 {
 
 static constexpr uint32_t TC_THREADS = 416;
-static constexpr uint32_t TC_ROWS = 128;
+static constexpr uint32_t TC_ROWS = 128, TC_HALF = 64;
 
 template <int HD>
 struct TcShape {
@@ -73,13 +76,46 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&v)[16
         : "memory");
 }
 
+// True in one lane of the warp, always the same one.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
+
+// 16 and 64 consecutive columns of this warp's 32 TMEM lanes.
+__device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+          "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+        : "r"(taddr)
+        : "memory");
+}
+#define TC_R16(b) \
+    "=r"(r[b]), "=r"(r[b + 1]), "=r"(r[b + 2]), "=r"(r[b + 3]), "=r"(r[b + 4]), "=r"(r[b + 5]), "=r"(r[b + 6]), "=r"(r[b + 7]), \
+        "=r"(r[b + 8]), "=r"(r[b + 9]), "=r"(r[b + 10]), "=r"(r[b + 11]), "=r"(r[b + 12]), "=r"(r[b + 13]), "=r"(r[b + 14]), "=r"(r[b + 15])
+__device__ __forceinline__ void tmem_ld64(uint32_t taddr, uint32_t (&r)[64]) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,"
+        "%62,%63}, [%64];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : TC_R16(0), TC_R16(16), TC_R16(32), TC_R16(48)
+        : "r"(taddr)
+        : "memory");
+}
+#undef TC_R16
+
 template <typename T, int HD>
 __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __grid_constant__ PrefixArgs a) {
     using S = TcShape<HD>;
     constexpr uint32_t NS = S::SLOTS, CH = HD / 8;
     constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : 1u;
     // D fp32; A and B of the cache's type; K-major A; N and M in the upper fields
-    constexpr uint32_t ID_QK = (1u << 4) | (FMT << 7) | (FMT << 10) | ((TC_ROWS >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t ID_QK = (1u << 4) | (FMT << 7) | (FMT << 10) | ((TC_HALF >> 3) << 17) | ((128u >> 4) << 24);
     constexpr uint32_t ID_PV = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((HD >> 3) << 17) | ((128u >> 4) << 24);
     extern __shared__ uint8_t tc_smem_raw[];
     const uint32_t base = (smem_u32(tc_smem_raw) + 1023u) & ~1023u;
@@ -87,14 +123,14 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
     const uint32_t s_q = base, s_kv = base + 2 * S::TILE;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + (2 + NS) * S::TILE);
     uint64_t* empty = full + NS;
-    uint64_t* s_full = empty + NS;  // a stream's scores are there
-    uint64_t* p_full = s_full + 2;  // its exponentials are
-    uint64_t* o_full = p_full + 2;  // its output is complete
-    uint64_t* q_full = o_full + 2;
+    uint64_t* s_full = empty + NS;  // [stream][half]: scores are there
+    uint64_t* p_full = s_full + 4;  // [stream][half]: exponentials are
+    uint64_t* o_done = p_full + 4;  // [stream]: a half's product with V is done
+    uint64_t* q_full = o_done + 2;
     uint64_t* drain = q_full + 1;   // every product is done
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
 
-    const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, head = blockIdx.z, split = blockIdx.x;
+    const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, head = blockIdx.z, split = blockIdx.x;
     pdl_trigger();  // the pass over the own rows may start beside this one
     const bool pair = !a.alternate;  // two tiles of vectors
 
@@ -103,14 +139,15 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
     const uint32_t n_tiles = any ? (w.r1 - w.r0 + TC_ROWS - 1) / TC_ROWS : 0;
     if (tid == 0) {
         for (uint32_t i = 0; i < NS; ++i) {
-            mbar_init(&full[i], 4);
+            mbar_init(&full[i], 128);  // each copying thread's copies
             mbar_init(&empty[i], 1);
         }
-        for (int t = 0; t < 2; ++t) {
+        for (int t = 0; t < 4; ++t) {
             mbar_init(&s_full[t], 1);
             mbar_init(&p_full[t], 4);
-            mbar_init(&o_full[t], 1);
         }
+        mbar_init(&o_done[0], 1);
+        mbar_init(&o_done[1], 1);
         mbar_init(q_full, 8);
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -128,7 +165,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
     if (warp < 8) {
         // ---- softmax ----------------------------------------------------------------------
         const uint32_t t = warp >> 2, row = tid & 127;
-        const uint32_t lanes = tmem + (((warp & 3) * 32u) << 16), ts = lanes + t * 128, to = lanes + 256 + t * 128;
+        const uint32_t lanes = tmem + (((warp & 3) * 32u) << 16), to = lanes + 256 + t * 128;
         {  // Q, one tile a stream, or the one tile by halves
             const uint32_t nv = any ? w.n_vec : 0, v0 = pair ? t * 128 : 0, r0 = pair ? 0 : t * 64, r1 = pair ? 128 : r0 + 64;
             const uint32_t dst = s_q + (pair ? t * S::TILE : 0);
@@ -147,93 +184,132 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
             if (lane == 0) mbar_arrive(q_full);
         }
         const uint32_t mine = pair ? n_tiles : (n_tiles + 1 - t) / 2;
-        float m = -INFINITY, l = 0.0f;
+        const F2 c2(a.c, a.c);
+        float m = -INFINITY;
+        F2 sum;  // of even and odd columns
         bool alive = true;
-        for (uint32_t j = 0; j < mine && alive; ++j) {
-            const uint32_t tile = pair ? j : 2 * j + t;
-            alive = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, QDEV_WAIT_FULL_TIMEOUT));
+        for (uint32_t u = 0; u < 2 * mine && alive; ++u) {  // half tiles
+            const uint32_t j = u >> 1, h = u & 1, ts = lanes + t * 128 + h * TC_HALF;
+            alive = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + h], j & 1, QDEV_WAIT_FULL_TIMEOUT));
             if (!alive) break;
             tc_fence_after();
-            const uint32_t cols = min(TC_ROWS, w.r1 - w.r0 - tile * TC_ROWS);  // rows past the end score nothing
-            float mx = -INFINITY;
+            uint32_t v[64];
+            tmem_ld64(ts, v);
+            const int32_t cols = (int32_t)(w.r1 - w.r0) - (int32_t)((pair ? j : 2 * j + t) * TC_ROWS + h * TC_HALF);
+            if (cols < (int32_t)TC_HALF) {  // rows past the end score nothing
 #pragma unroll
-            for (uint32_t c = 0; c < 4; ++c) {
-                float v[32];
-                tmem_ld32(ts + c * 32, v);
-                if (cols < TC_ROWS) {
-#pragma unroll
-                    for (uint32_t i = 0; i < 32; ++i)
-                        if (c * 32 + i >= cols) v[i] = -INFINITY;
-                }
-#pragma unroll
-                for (int i = 0; i < 32; ++i) mx = fmaxf(mx, v[i]);
+                for (int i = 0; i < 64; ++i)
+                    if (i >= cols) v[i] = 0xff800000u;
             }
-            mx *= a.c;  // c > 0
+            float mx = -INFINITY, my = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 64; i += 4) {
+                mx = fmaxf(fmaxf(mx, __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
+                my = fmaxf(fmaxf(my, __uint_as_float(v[i + 2])), __uint_as_float(v[i + 3]));
+            }
+            mx = fmaxf(mx, my) * a.c;  // c > 0
             const bool move = mx > m + 8.0f;  // also from -infinity
             if (__any_sync(0xffffffffu, move)) {
                 const float f = move ? (m == -INFINITY ? 0.0f : ex2(m - mx)) : 1.0f;
-                if (move) {
-                    m = mx;
-                    l *= f;
-                }
-                if (j > 0) {
+                if (move) m = mx;
+                float s0, s1;
+                sum.get(s0, s1);
+                sum = F2(s0 * f, s1 * f);
+                if (u > 0) {  // the product before this one is done before its output is touched
+                    alive = __all_sync(0xffffffffu, mbar_wait(&o_done[t], (u - 1) & 1, QDEV_WAIT_FULL_TIMEOUT));
+                    if (!alive) break;
+                    tc_fence_after();
 #pragma unroll 1
-                    for (uint32_t c = 0; c < HD / 32; ++c) {
-                        float v[32];
-                        tmem_ld32(to + c * 32, v);
+                    for (uint32_t c = 0; c < HD / 16; ++c) {
+                        uint32_t o[16];
+                        tmem_ld16(to + c * 16, o);
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] *= f;
-                        tmem_st32(to + c * 32, v);
+                        for (int i = 0; i < 16; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                        tmem_st16(to + c * 16, o);
                     }
+                    asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
                 }
             }
             const float sub = m == -INFINITY ? 0.0f : -m;
+            const F2 sub2f(sub, sub);
 #pragma unroll
-            for (uint32_t c = 0; c < 4; ++c) {
-                float v[32];
-                tmem_ld32(ts + c * 32, v);
+            for (int k = 0; k < 2; ++k) {
                 uint32_t p[16];
 #pragma unroll
-                for (int i = 0; i < 32; ++i) {
-                    v[i] = ex2(fmaf(v[i], a.c, sub));
-                    if (cols < TC_ROWS && c * 32 + i >= cols) v[i] = 0.0f;
-                    l += v[i];
+                for (int i = 0; i < 16; ++i) {
+                    float x, y;
+                    fma2(F2(__uint_as_float(v[32 * k + 2 * i]), __uint_as_float(v[32 * k + 2 * i + 1])), c2, sub2f).get(x, y);
+                    x = ex2(x);
+                    y = ex2(y);
+                    sum = add2(sum, F2(x, y));
+                    p[i] = pack2<T>(x, y);
                 }
-#pragma unroll
-                for (int i = 0; i < 16; ++i) p[i] = pack2<T>(v[2 * i], v[2 * i + 1]);
-                tmem_st16(ts + c * 16, p);
+                tmem_st16(ts + k * 16, p);
             }
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&p_full[t]);
+            if (lane == 0) mbar_arrive(&p_full[2 * t + h]);
         }
+        float l, l1;
+        sum.get(l, l1);
+        l += l1;
         // ---- this stream's part ----
-        bool ok = alive;
-        if (mine && alive) ok = __all_sync(0xffffffffu, mbar_wait(&o_full[t], 0, QDEV_WAIT_FULL_TIMEOUT));
+        bool ok = alive && mine;
+        // the last two products may be under way: a wait tells a phase from the next one only
+        for (uint32_t u = 0; u < 2 && ok; ++u) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], u, QDEV_WAIT_FULL_TIMEOUT));
         tc_fence_after();
+        if (!ok) m = -INFINITY, l = 0.0f;
         const uint32_t v = (pair ? t * 128 : 0) + row;
         const bool valid = any && v < w.n_vec;
-        uint64_t at = 0;
-        if (valid) {
-            const uint32_t i = fast_div(w.vec0 + v, a.by_group), h = head * a.group + (w.vec0 + v - i * a.group);
-            const uint32_t part = pair ? split : 2 * split + t;
-            at = ((uint64_t)part * a.n_tokens + i) * a.n_heads + h;
-            __stcg(a.part_ml + at, mine ? make_float2(m, l) : make_float2(-INFINITY, 0.0f));
-        }
+        float* s_o = reinterpret_cast<float*>(smem + 2 * S::TILE);  // [128][HD + 1], in the ring's place
+        float* s_ml = s_o + 128 * (HD + 1);                         // [128][2]
+        float f0 = 1.0f, f1 = 0.0f;
+        if (!pair) {  // the second stream's share goes through shared memory to the first
+            // (both streams' products are done: each has waited for its own last one)
+            asm volatile("bar.sync 2, 256;" ::: "memory");
+            if (t == 1) {
 #pragma unroll 1
-        for (uint32_t c = 0; c < HD / 32; ++c) {
-            float o[32];
-            if (mine && ok) {
-                tmem_ld32(to + c * 32, o);
-            } else {
+                for (uint32_t c = 0; c < HD / 16; ++c) {
+                    uint32_t o[16];
+                    if (ok) tmem_ld16(to + c * 16, o);
 #pragma unroll
-                for (int i = 0; i < 32; ++i) o[i] = 0.0f;
+                    for (int i = 0; i < 16; ++i) s_o[row * (HD + 1) + c * 16 + i] = ok ? __uint_as_float(o[i]) : 0.0f;
+                }
+                s_ml[row * 2] = m;
+                s_ml[row * 2 + 1] = l;
             }
+            asm volatile("bar.sync 2, 256;" ::: "memory");
+            if (t == 0) {
+                const float m1 = s_ml[row * 2], l2 = s_ml[row * 2 + 1], M = fmaxf(m, m1);
+                f0 = m == M ? 1.0f : ex2(m - M);
+                f1 = m1 == M ? 1.0f : ex2(m1 - M);
+                m = M;
+                l = l * f0 + l2 * f1;
+            }
+        }
+        if (pair || t == 0) {
+            uint64_t at = 0;
             if (valid) {
-                float4* d = reinterpret_cast<float4*>(a.part_o + at * HD + c * 32);
+                const uint32_t i = fast_div(w.vec0 + v, a.by_group), h = head * a.group + (w.vec0 + v - i * a.group);
+                at = ((uint64_t)split * a.n_tokens + i) * a.n_heads + h;
+                __stcg(a.part_ml + at, make_float2(m, l));
+            }
+#pragma unroll 1
+            for (uint32_t c = 0; c < HD / 16; ++c) {
+                uint32_t o[16];
+                if (ok) tmem_ld16(to + c * 16, o);
+                float x[16];
 #pragma unroll
-                for (int i = 0; i < 8; ++i) __stcg(d + i, make_float4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]));
+                for (int i = 0; i < 16; ++i) {
+                    x[i] = ok ? __uint_as_float(o[i]) : 0.0f;
+                    if (!pair) x[i] = x[i] * f0 + s_o[row * (HD + 1) + c * 16 + i] * f1;
+                }
+                if (valid) {
+                    float4* d = reinterpret_cast<float4*>(a.part_o + at * HD + c * 16);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) __stcg(d + i, make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
+                }
             }
         }
     } else if (warp < 12) {
@@ -241,17 +317,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
         const uint32_t lw = warp - 8;
         constexpr uint32_t RP = 32 / CH;       // rows of one instruction
         constexpr uint32_t N = 32 / RP;        // instructions for the warp's 32 rows
-        constexpr uint32_t AHEAD = NS - 2;     // slots under way before the oldest is waited for
         const uint32_t lr = lane / CH, lc = lane % CH;
         const T* bases[2] = {reinterpret_cast<const T*>(a.k), reinterpret_cast<const T*>(a.v)};
         bool alive = true;
-        uint32_t fill = 0, done = 0;
-        auto finish = [&] {  // the oldest slot's copies are visible to the tensor core
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&full[done % NS]);
-            ++done;
-        };
+        uint32_t fill = 0;
         for (uint32_t tile = 0; tile < n_tiles && alive; ++tile) {
             const uint32_t row = w.r0 + tile * TC_ROWS + lw * 32 + lane;
             uint64_t off;
@@ -271,92 +340,90 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
                     const uint32_t at = st + (lc >> 3) * S::PANEL + r * 128 + (((lc & 7) ^ (r & 7)) << 4);
                     cp_async16(at, bases[kv] + (o == ~0ull ? 0ull : o) + lc * 8, o == ~0ull ? 0u : 16u);
                 }
-                cp_async_commit();
-                if (fill - done >= AHEAD) {
-                    cp_async_wait<AHEAD>();
-                    finish();
-                }
+                cp_async_arrive(&full[slot]);
             }
         }
         cp_async_wait_all();
-        while (done < fill && alive) finish();
-    } else if (lane == 0) {
+    } else {
         // ---- products ---------------------------------------------------------------------------
+        // The whole warp takes these steps and one elected lane issues: what a product needs (addresses,
+        // descriptors) is then the same in all lanes and stays in uniform registers, where the
+        // instruction reads it.  Formed by a single lane in a branch of its own, the 48 products of a
+        // tile took 5100 clocks to issue.
         bool alive = true;
+        const uint32_t tiles = __shfl_sync(0xffffffffu, n_tiles, 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
         auto wait = [&](uint64_t* bar, uint32_t parity) {
-            if (alive) alive = mbar_wait(bar, parity, QDEV_WAIT_FULL_TIMEOUT);
+            if (alive) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, QDEV_WAIT_FULL_TIMEOUT));
             tc_fence_after();
         };
-        auto qk = [&](uint32_t t, uint32_t tile) {
-            const uint32_t q = s_q + (pair ? t * S::TILE : 0), k = s_kv + ((2 * tile) % NS) * S::TILE;
-#pragma unroll
-            for (uint32_t j = 0; j < HD / 16; ++j) {
-                const uint32_t at = (j >> 2) * S::PANEL + (j & 3) * 32;
-                umma_f16(tmem + t * 128, umma_desc_sw128(q + at), umma_desc_sw128(k + at), j != 0, ID_QK);
-            }
-            umma_commit(&s_full[t]);
+        auto commit_one = [&](uint64_t* bar) {
+            if (elect_one()) umma_commit(bar);
+            __syncwarp();
         };
-        auto pv = [&](uint32_t t, uint32_t tile, bool first) {
-            const uint32_t v = s_kv + ((2 * tile + 1) % NS) * S::TILE;
+        auto qk = [&](uint32_t t, uint32_t tile, uint32_t h) {
+            const uint32_t q = s_q + (pair ? t * S::TILE : 0), k = s_kv + ((2 * tile) % NS) * S::TILE + h * TC_HALF * 128;
+            const uint64_t dq = umma_desc_sw128(q), dk = umma_desc_sw128(k);
+            const uint32_t d = tm + t * 128 + h * TC_HALF;
+            if (elect_one()) {
 #pragma unroll
-            for (uint32_t j = 0; j < TC_ROWS / 16; ++j)
-                umma_f16_ta(tmem + 256 + t * 128, tmem + t * 128 + j * 8, umma_desc_sw128_mn(v + j * 2048, S::PANEL), !(first && j == 0), ID_PV);
+                for (uint32_t j = 0; j < HD / 16; ++j) {
+                    const uint32_t at = ((j >> 2) * S::PANEL + (j & 3) * 32) >> 4;  // added to the address field
+                    umma_f16(d, dq + at, dk + at, j != 0, ID_QK);
+                }
+                umma_commit(&s_full[2 * t + h]);
+            }
+            __syncwarp();
         };
-        auto k_full = [&](uint32_t tile) { wait(&full[(2 * tile) % NS], (2 * tile / NS) & 1); };
-        auto v_full = [&](uint32_t tile) { wait(&full[(2 * tile + 1) % NS], ((2 * tile + 1) / NS) & 1); };
-        auto k_free = [&](uint32_t tile) { umma_commit(&empty[(2 * tile) % NS]); };
-        auto v_free = [&](uint32_t tile) { umma_commit(&empty[(2 * tile + 1) % NS]); };
-        if (n_tiles) wait(q_full, 0);
-        if (pair) {
-            if (n_tiles) {
-                k_full(0);
-                if (alive) {
-                    qk(0, 0);
-                    qk(1, 0);
-                    k_free(0);
-                }
+        auto pv = [&](uint32_t t, uint32_t tile, uint32_t h, bool first) {
+            const uint32_t v = s_kv + ((2 * tile + 1) % NS) * S::TILE + h * TC_HALF * 128;
+            const uint64_t dv = umma_desc_sw128_mn(v, S::PANEL);
+            const uint32_t d = tm + 256 + t * 128, p = tm + t * 128 + h * TC_HALF;
+            if (elect_one()) {
+#pragma unroll
+                for (uint32_t j = 0; j < TC_HALF / 16; ++j) umma_f16_ta(d, p + j * 8, dv + j * (2048 >> 4), !(first && j == 0), ID_PV);
+                umma_commit(&o_done[t]);
             }
-            for (uint32_t i = 0; i < n_tiles && alive; ++i) {
-                const bool more = i + 1 < n_tiles;
-                v_full(i);
-                if (more) k_full(i + 1);
-                for (uint32_t t = 0; t < 2; ++t) {
-                    wait(&p_full[t], i & 1);
+            __syncwarp();
+        };
+        // The copies are generic-proxy writes of other threads: after the barrier that their arrival
+        // completes, this fence orders them before the tensor core's reads.
+        auto landed = [&](uint32_t fill) {
+            wait(&full[fill % NS], (fill / NS) & 1);
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        };
+        auto k_full = [&](uint32_t tile) { landed(2 * tile); };
+        auto v_full = [&](uint32_t tile) { landed(2 * tile + 1); };
+        auto k_free = [&](uint32_t tile) { commit_one(&empty[(2 * tile) % NS]); };
+        auto v_free = [&](uint32_t tile) { commit_one(&empty[(2 * tile + 1) % NS]); };
+        // Tile i's two halves; a half's buffer takes the next tile's scores as soon as its product with V is issued.
+        const uint32_t step = pair ? 1 : 2;  // from a stream's tile to its next
+        if (tiles) wait(q_full, 0);
+        for (uint32_t i = 0; i < step && i < tiles && alive; ++i) {
+            k_full(i);
+            if (!alive) break;
+            for (uint32_t h = 0; h < 2; ++h)
+                for (uint32_t t = pair ? 0 : i; t < (pair ? 2 : i + 1); ++t) qk(t, i, h);
+            k_free(i);
+        }
+        for (uint32_t i = 0; i < tiles && alive; ++i) {
+            const uint32_t next = i + step, par = (i / step) & 1;
+            v_full(i);
+            for (uint32_t h = 0; h < 2 && alive; ++h) {
+                if (h == 0 && next < tiles) k_full(next);
+                for (uint32_t t = pair ? 0 : i & 1; t < (pair ? 2 : (i & 1) + 1); ++t) {
+                    wait(&p_full[2 * t + h], par);
                     if (!alive) break;
-                    pv(t, i, i == 0);
-                    if (t) v_free(i);
-                    if (more) qk(t, i + 1);
-                    else umma_commit(&o_full[t]);
-                    if (more && t) k_free(i + 1);
+                    pv(t, i, h, i < step && h == 0);
+                    if (next < tiles) qk(t, next, h);
                 }
             }
-        } else {
-            for (uint32_t t = 0; t < 2 && t < n_tiles; ++t) {
-                k_full(t);
-                if (!alive) break;
-                qk(t, t);
-                k_free(t);
-            }
-            for (uint32_t i = 0; i < n_tiles && alive; ++i) {
-                const uint32_t t = i & 1;
-                v_full(i);
-                wait(&p_full[t], (i >> 1) & 1);
-                if (!alive) break;
-                pv(t, i, i < 2);
-                v_free(i);
-                if (i + 2 < n_tiles) {
-                    k_full(i + 2);
-                    if (!alive) break;
-                    qk(t, i + 2);
-                    k_free(i + 2);
-                } else {
-                    umma_commit(&o_full[t]);
-                }
-            }
+            if (!alive) break;
+            v_free(i);
+            if (next < tiles) k_free(next);
         }
         // every product issued has finished before TMEM is freed
-        if (n_tiles) {
-            umma_commit(drain);
+        if (tiles) {
+            commit_one(drain);
             mbar_wait(drain, 0, QDEV_WAIT_FULL_TIMEOUT);
         }
     }

@@ -40,6 +40,29 @@ __device__ __forceinline__ float ex2(float x) {
     return y;
 }
 
+// Two fp32 numbers, added and multiplied side by side.
+struct F2 {
+    unsigned long long w;
+    __device__ __forceinline__ F2() : w(0ull) {}
+    __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(w) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(w)); }
+};
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+    F2 d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d.w) : "l"(a.w), "l"(b.w));
+    return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.w) : "l"(a.w), "l"(b.w), "l"(c.w));
+    return d;
+}
+__device__ __forceinline__ F2 sub2(F2 a, F2 b) {  // a - b, rounded once
+    F2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.w) : "l"(b.w), "l"(F2(-1.0f, -1.0f).w), "l"(a.w));
+    return d;
+}
+
 // Two 16-bit numbers in a word.
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
