@@ -7,20 +7,27 @@
 // runs two streams, each with scores and an output of its own in TMEM:
 //   two tiles of vectors, the same rows (more than 128 vectors), or
 //   one tile of vectors, even and odd row tiles (up to 128; joined at the end),
-// and each stream takes a row tile in two halves of 64 rows with a score
-// buffer each, so that the products for one half run while the exponentials
-// of the other do (columns: S[stream][half] at 128 stream + 64 half, O at 256
-// + 128 stream).  With one buffer of 128 rows a stream, products and
-// exponentials of a stream took turns: 105 us where this takes 50 (512
-// vectors x 32768 rows x 8 KV heads, head_dim 128).
+// so that one stream's products run while the other's exponentials do
+// (columns: S at 128 stream, O at 256 + 128 stream).  A stream's exponentials
+// come in two halves of 64 rows, so that the first half's product with V runs
+// beside the second half's exponentials.
 //
 // Roles: warps 0-3 and 4-7 are the streams' softmax, a thread per vector
 // (its row of S lies in its own TMEM lane, so maximum and sum need no
 // exchange); warps 8-11 copy rows of K and V (16-byte cp.async into the
 // 128-byte swizzle that the MMA's descriptors name; a row's page is looked up
-// by one lane); one lane of warp 12 issues the MMAs.  P overwrites S in TMEM
-// in 16 bits (the operand type) and is the A operand of P V from there; V is
-// used as it lies in the cache, [row][dim], as an MN-major B operand.
+// by one lane); warp 13 hands landed tiles over to the tensor core's proxy;
+// warp 12 issues the products.  P overwrites S
+// in TMEM in 16 bits (the operand type) and is the A operand of P V from
+// there; V is used as it lies in the cache, [row][dim], as an MN-major B
+// operand.
+//
+// What it took (512 vectors x 32768 rows x 8 KV heads, head_dim 128, 29 tiles
+// a CTA): scores of 64 rows with two buffers a stream instead of 128 with
+// one keep the streams apart from their own products, but a product of
+// 64 columns takes 53 clocks and not 32 (its operands come from shared memory
+// at 128 bytes a clock); the fence between the copies and the products cost
+// the issuing warp 500 clocks a tile.
 //
 // The running maximum moves only when a half tile exceeds it by 2^8: then the
 // output is rescaled in TMEM; until then exponentials may reach 256, which
@@ -36,7 +43,7 @@
 
 namespace qb200 {
 
-static constexpr uint32_t TC_THREADS = 416;
+static constexpr uint32_t TC_THREADS = 448;
 static constexpr uint32_t TC_ROWS = 128, TC_HALF = 64;
 
 template <int HD>
@@ -44,7 +51,7 @@ struct TcShape {
     static constexpr uint32_t SLOTS = HD == 128 ? 5 : 9;        // K and V tiles in the ring
     static constexpr uint32_t TILE = TC_ROWS * HD * 2;          // one K or V tile, one tile of Q
     static constexpr uint32_t PANEL = TC_ROWS * 128;            // 64 columns of it
-    static constexpr size_t SMEM = (size_t)(2 + SLOTS) * TILE + 1024 + 256;
+    static constexpr size_t SMEM = (size_t)(2 + SLOTS) * TILE + 1024 + 512;
 };
 
 // Descriptor of an MN-major operand in the 128-byte swizzle: 64 contiguous
@@ -115,16 +122,17 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
     constexpr uint32_t NS = S::SLOTS, CH = HD / 8;
     constexpr uint32_t FMT = std::is_same<T, __half>::value ? 0u : 1u;
     // D fp32; A and B of the cache's type; K-major A; N and M in the upper fields
-    constexpr uint32_t ID_QK = (1u << 4) | (FMT << 7) | (FMT << 10) | ((TC_HALF >> 3) << 17) | ((128u >> 4) << 24);
+    constexpr uint32_t ID_QK = (1u << 4) | (FMT << 7) | (FMT << 10) | ((TC_ROWS >> 3) << 17) | ((128u >> 4) << 24);
     constexpr uint32_t ID_PV = (1u << 4) | (FMT << 7) | (FMT << 10) | (1u << 16) | ((HD >> 3) << 17) | ((128u >> 4) << 24);
     extern __shared__ uint8_t tc_smem_raw[];
     const uint32_t base = (smem_u32(tc_smem_raw) + 1023u) & ~1023u;
     uint8_t* smem = tc_smem_raw + (base - smem_u32(tc_smem_raw));
     const uint32_t s_q = base, s_kv = base + 2 * S::TILE;
     uint64_t* full = reinterpret_cast<uint64_t*>(smem + (2 + NS) * S::TILE);
-    uint64_t* empty = full + NS;
-    uint64_t* s_full = empty + NS;  // [stream][half]: scores are there
-    uint64_t* p_full = s_full + 4;  // [stream][half]: exponentials are
+    uint64_t* landed = full + NS;
+    uint64_t* empty = landed + NS;
+    uint64_t* s_full = empty + NS;  // [stream]: scores are there
+    uint64_t* p_full = s_full + 2;  // [stream][half]: exponentials are
     uint64_t* o_done = p_full + 4;  // [stream]: a half's product with V is done
     uint64_t* q_full = o_done + 2;
     uint64_t* drain = q_full + 1;   // every product is done
@@ -139,13 +147,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
     const uint32_t n_tiles = any ? (w.r1 - w.r0 + TC_ROWS - 1) / TC_ROWS : 0;
     if (tid == 0) {
         for (uint32_t i = 0; i < NS; ++i) {
-            mbar_init(&full[i], 128);  // each copying thread's copies
+            mbar_init(&landed[i], 128);  // each copying thread's copies
+            mbar_init(&full[i], 1);
             mbar_init(&empty[i], 1);
         }
-        for (int t = 0; t < 4; ++t) {
-            mbar_init(&s_full[t], 1);
-            mbar_init(&p_full[t], 4);
-        }
+        for (int t = 0; t < 4; ++t) mbar_init(&p_full[t], 4);
+        mbar_init(&s_full[0], 1);
+        mbar_init(&s_full[1], 1);
         mbar_init(&o_done[0], 1);
         mbar_init(&o_done[1], 1);
         mbar_init(q_full, 8);
@@ -190,9 +198,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
         bool alive = true;
         for (uint32_t u = 0; u < 2 * mine && alive; ++u) {  // half tiles
             const uint32_t j = u >> 1, h = u & 1, ts = lanes + t * 128 + h * TC_HALF;
-            alive = __all_sync(0xffffffffu, mbar_wait(&s_full[2 * t + h], j & 1, QDEV_WAIT_FULL_TIMEOUT));
-            if (!alive) break;
-            tc_fence_after();
+            if (h == 0) {
+                alive = __all_sync(0xffffffffu, mbar_wait(&s_full[t], j & 1, QDEV_WAIT_FULL_TIMEOUT));
+                if (!alive) break;
+                tc_fence_after();
+            }
             uint32_t v[64];
             tmem_ld64(ts, v);
             const int32_t cols = (int32_t)(w.r1 - w.r0) - (int32_t)((pair ? j : 2 * j + t) * TC_ROWS + h * TC_HALF);
@@ -340,90 +350,128 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
                     const uint32_t at = st + (lc >> 3) * S::PANEL + r * 128 + (((lc & 7) ^ (r & 7)) << 4);
                     cp_async16(at, bases[kv] + (o == ~0ull ? 0ull : o) + lc * 8, o == ~0ull ? 0u : 16u);
                 }
-                cp_async_arrive(&full[slot]);
+                cp_async_arrive(&landed[slot]);
             }
         }
         cp_async_wait_all();
+    } else if (warp == 13) {
+        // ---- landed copies, generic-proxy writes of other threads, to the tensor core's proxy ----------
+        bool alive = true;
+        for (uint32_t f = 0; f < 2 * n_tiles && alive; ++f) {
+            alive = __all_sync(0xffffffffu, mbar_wait(&landed[f % NS], (f / NS) & 1, QDEV_WAIT_FULL_TIMEOUT));
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            if (alive && lane == 0) mbar_arrive(&full[f % NS]);
+        }
     } else {
         // ---- products ---------------------------------------------------------------------------
         // The whole warp takes these steps and one elected lane issues: what a product needs (addresses,
         // descriptors) is then the same in all lanes and stays in uniform registers, where the
         // instruction reads it.  Formed by a single lane in a branch of its own, the 48 products of a
         // tile took 5100 clocks to issue.
+        // Every instruction here is on the streams' way (a state machine that polled both streams took
+        // 3000 clocks a tile), so slots are counted, not divided.
         bool alive = true;
         const uint32_t tiles = __shfl_sync(0xffffffffu, n_tiles, 0), tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t hi = umma_desc_sw128(0) & ~0xffffffffull;  // of every descriptor here
+        const uint32_t lo_k = (uint32_t)umma_desc_sw128(0), lo_mn = (uint32_t)umma_desc_sw128_mn(0, S::PANEL);
+        struct Slot {  // of the K or V tile that is used next
+            uint32_t at, phase;
+            __device__ __forceinline__ void next(uint32_t by) {
+                at += by;
+                if (at >= NS) {
+                    at -= NS;
+                    phase ^= 1;
+                }
+            }
+        };
         auto wait = [&](uint64_t* bar, uint32_t parity) {
             if (alive) alive = __all_sync(0xffffffffu, mbar_wait(bar, parity, QDEV_WAIT_FULL_TIMEOUT));
             tc_fence_after();
         };
-        auto commit_one = [&](uint64_t* bar) {
-            if (elect_one()) umma_commit(bar);
-            __syncwarp();
-        };
-        auto qk = [&](uint32_t t, uint32_t tile, uint32_t h) {
-            const uint32_t q = s_q + (pair ? t * S::TILE : 0), k = s_kv + ((2 * tile) % NS) * S::TILE + h * TC_HALF * 128;
-            const uint64_t dq = umma_desc_sw128(q), dk = umma_desc_sw128(k);
-            const uint32_t d = tm + t * 128 + h * TC_HALF;
+        auto qk = [&](uint32_t t, uint32_t slot, uint64_t* free_k) {
+            const uint32_t lq = lo_k + ((s_q + (pair ? t * S::TILE : 0)) >> 4), lk = lo_k + ((s_kv + slot * S::TILE) >> 4);
+            const uint32_t d = tm + t * 128;
             if (elect_one()) {
 #pragma unroll
                 for (uint32_t j = 0; j < HD / 16; ++j) {
                     const uint32_t at = ((j >> 2) * S::PANEL + (j & 3) * 32) >> 4;  // added to the address field
-                    umma_f16(d, dq + at, dk + at, j != 0, ID_QK);
+                    umma_f16(d, hi | (lq + at), hi | (lk + at), j != 0, ID_QK);
                 }
-                umma_commit(&s_full[2 * t + h]);
+                umma_commit(&s_full[t]);
+                if (free_k) umma_commit(free_k);
             }
             __syncwarp();
         };
-        auto pv = [&](uint32_t t, uint32_t tile, uint32_t h, bool first) {
-            const uint32_t v = s_kv + ((2 * tile + 1) % NS) * S::TILE + h * TC_HALF * 128;
-            const uint64_t dv = umma_desc_sw128_mn(v, S::PANEL);
+        auto pv = [&](uint32_t t, uint32_t slot, uint32_t h, bool first, uint64_t* free_v) {
+            const uint32_t lv = lo_mn + ((s_kv + slot * S::TILE + h * TC_HALF * 128) >> 4);
             const uint32_t d = tm + 256 + t * 128, p = tm + t * 128 + h * TC_HALF;
             if (elect_one()) {
 #pragma unroll
-                for (uint32_t j = 0; j < TC_HALF / 16; ++j) umma_f16_ta(d, p + j * 8, dv + j * (2048 >> 4), !(first && j == 0), ID_PV);
+                for (uint32_t j = 0; j < TC_HALF / 16; ++j) umma_f16_ta(d, p + j * 8, hi | (lv + j * (2048 >> 4)), !(first && j == 0), ID_PV);
                 umma_commit(&o_done[t]);
+                if (free_v) umma_commit(free_v);
             }
             __syncwarp();
         };
-        // The copies are generic-proxy writes of other threads: after the barrier that their arrival
-        // completes, this fence orders them before the tensor core's reads.
-        auto landed = [&](uint32_t fill) {
-            wait(&full[fill % NS], (fill / NS) & 1);
-            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        };
-        auto k_full = [&](uint32_t tile) { landed(2 * tile); };
-        auto v_full = [&](uint32_t tile) { landed(2 * tile + 1); };
-        auto k_free = [&](uint32_t tile) { commit_one(&empty[(2 * tile) % NS]); };
-        auto v_free = [&](uint32_t tile) { commit_one(&empty[(2 * tile + 1) % NS]); };
-        // Tile i's two halves; a half's buffer takes the next tile's scores as soon as its product with V is issued.
-        const uint32_t step = pair ? 1 : 2;  // from a stream's tile to its next
+        Slot k = {0, 0}, v = {1, 0};
         if (tiles) wait(q_full, 0);
-        for (uint32_t i = 0; i < step && i < tiles && alive; ++i) {
-            k_full(i);
-            if (!alive) break;
-            for (uint32_t h = 0; h < 2; ++h)
-                for (uint32_t t = pair ? 0 : i; t < (pair ? 2 : i + 1); ++t) qk(t, i, h);
-            k_free(i);
-        }
-        for (uint32_t i = 0; i < tiles && alive; ++i) {
-            const uint32_t next = i + step, par = (i / step) & 1;
-            v_full(i);
-            for (uint32_t h = 0; h < 2 && alive; ++h) {
-                if (h == 0 && next < tiles) k_full(next);
-                for (uint32_t t = pair ? 0 : i & 1; t < (pair ? 2 : (i & 1) + 1); ++t) {
-                    wait(&p_full[2 * t + h], par);
-                    if (!alive) break;
-                    pv(t, i, h, i < step && h == 0);
-                    if (next < tiles) qk(t, next, h);
+        if (pair) {
+            if (tiles) {
+                wait(&full[k.at], k.phase);
+                if (alive) {
+                    qk(0, k.at, nullptr);
+                    qk(1, k.at, &empty[k.at]);
                 }
             }
-            if (!alive) break;
-            v_free(i);
-            if (next < tiles) k_free(next);
+            for (uint32_t i = 0; i < tiles && alive; ++i) {
+                const bool more = i + 1 < tiles;
+                k.next(2);
+                wait(&full[v.at], v.phase);
+                wait(&p_full[0], i & 1);
+                if (!alive) break;
+                pv(0, v.at, 0, i == 0, nullptr);
+                wait(&p_full[2], i & 1);
+                if (!alive) break;
+                pv(1, v.at, 0, i == 0, nullptr);
+                if (more) wait(&full[k.at], k.phase);
+                wait(&p_full[1], i & 1);
+                if (!alive) break;
+                pv(0, v.at, 1, false, nullptr);
+                if (more) qk(0, k.at, nullptr);
+                wait(&p_full[3], i & 1);
+                if (!alive) break;
+                pv(1, v.at, 1, false, &empty[v.at]);
+                if (more) qk(1, k.at, &empty[k.at]);
+                v.next(2);
+            }
+        } else {
+            for (uint32_t t = 0; t < 2 && t < tiles && alive; ++t) {
+                wait(&full[k.at], k.phase);
+                if (alive) qk(t, k.at, &empty[k.at]);
+                k.next(2);
+            }
+            for (uint32_t i = 0; i < tiles && alive; ++i) {
+                const uint32_t t = i & 1, par = (i >> 1) & 1;
+                wait(&full[v.at], v.phase);
+                wait(&p_full[2 * t], par);
+                if (!alive) break;
+                pv(t, v.at, 0, i < 2, nullptr);
+                wait(&p_full[2 * t + 1], par);
+                if (!alive) break;
+                pv(t, v.at, 1, false, &empty[v.at]);
+                v.next(2);
+                if (i + 2 < tiles) {
+                    wait(&full[k.at], k.phase);
+                    if (!alive) break;
+                    qk(t, k.at, &empty[k.at]);
+                    k.next(2);
+                }
+            }
         }
         // every product issued has finished before TMEM is freed
         if (tiles) {
-            commit_one(drain);
+            if (elect_one()) umma_commit(drain);
+            __syncwarp();
             mbar_wait(drain, 0, QDEV_WAIT_FULL_TIMEOUT);
         }
     }
