@@ -134,7 +134,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
     uint64_t* s_full = empty + NS;  // [stream]: scores are there
     uint64_t* p_full = s_full + 2;  // [stream][half]: exponentials are
     uint64_t* o_done = p_full + 4;  // [stream]: a half's product with V is done
-    uint64_t* q_full = o_done + 2;
+    uint64_t* o_last = o_done + 2;  // [stream]: the last one is
+    uint64_t* q_full = o_last + 2;
     uint64_t* drain = q_full + 1;   // every product is done
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
 
@@ -154,8 +155,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
         for (int t = 0; t < 4; ++t) mbar_init(&p_full[t], 4);
         mbar_init(&s_full[0], 1);
         mbar_init(&s_full[1], 1);
-        mbar_init(&o_done[0], 1);
-        mbar_init(&o_done[1], 1);
+        for (int t = 0; t < 2; ++t) {
+            mbar_init(&o_done[t], 1);
+            mbar_init(&o_last[t], 1);
+        }
         mbar_init(q_full, 8);
         mbar_init(drain, 1);
         fence_mbar_init();
@@ -266,8 +269,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
         l += l1;
         // ---- this stream's part ----
         bool ok = alive && mine;
-        // the last two products may be under way: a wait tells a phase from the next one only
-        for (uint32_t u = 0; u < 2 && ok; ++u) ok = __all_sync(0xffffffffu, mbar_wait(&o_done[t], u, QDEV_WAIT_FULL_TIMEOUT));
+        // (a barrier of its own: o_done may be one phase back or two by now, which a parity cannot tell)
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&o_last[t], 0, QDEV_WAIT_FULL_TIMEOUT));
         tc_fence_after();
         if (!ok) m = -INFINITY, l = 0.0f;
         const uint32_t v = (pair ? t * 128 : 0) + row;
@@ -402,13 +405,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
             }
             __syncwarp();
         };
-        auto pv = [&](uint32_t t, uint32_t slot, uint32_t h, bool first, uint64_t* free_v) {
+        auto pv = [&](uint32_t t, uint32_t slot, uint32_t h, bool first, bool last, uint64_t* free_v) {
             const uint32_t lv = lo_mn + ((s_kv + slot * S::TILE + h * TC_HALF * 128) >> 4);
             const uint32_t d = tm + 256 + t * 128, p = tm + t * 128 + h * TC_HALF;
             if (elect_one()) {
 #pragma unroll
                 for (uint32_t j = 0; j < TC_HALF / 16; ++j) umma_f16_ta(d, p + j * 8, hi | (lv + j * (2048 >> 4)), !(first && j == 0), ID_PV);
-                umma_commit(&o_done[t]);
+                umma_commit(last ? &o_last[t] : &o_done[t]);
                 if (free_v) umma_commit(free_v);
             }
             __syncwarp();
@@ -429,18 +432,18 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
                 wait(&full[v.at], v.phase);
                 wait(&p_full[0], i & 1);
                 if (!alive) break;
-                pv(0, v.at, 0, i == 0, nullptr);
+                pv(0, v.at, 0, i == 0, false, nullptr);
                 wait(&p_full[2], i & 1);
                 if (!alive) break;
-                pv(1, v.at, 0, i == 0, nullptr);
+                pv(1, v.at, 0, i == 0, false, nullptr);
                 if (more) wait(&full[k.at], k.phase);
                 wait(&p_full[1], i & 1);
                 if (!alive) break;
-                pv(0, v.at, 1, false, nullptr);
+                pv(0, v.at, 1, false, !more, nullptr);
                 if (more) qk(0, k.at, nullptr);
                 wait(&p_full[3], i & 1);
                 if (!alive) break;
-                pv(1, v.at, 1, false, &empty[v.at]);
+                pv(1, v.at, 1, false, !more, &empty[v.at]);
                 if (more) qk(1, k.at, &empty[k.at]);
                 v.next(2);
             }
@@ -455,10 +458,10 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
                 wait(&full[v.at], v.phase);
                 wait(&p_full[2 * t], par);
                 if (!alive) break;
-                pv(t, v.at, 0, i < 2, nullptr);
+                pv(t, v.at, 0, i < 2, false, nullptr);
                 wait(&p_full[2 * t + 1], par);
                 if (!alive) break;
-                pv(t, v.at, 1, false, &empty[v.at]);
+                pv(t, v.at, 1, false, i + 2 >= tiles, &empty[v.at]);
                 v.next(2);
                 if (i + 2 < tiles) {
                     wait(&full[k.at], k.phase);
