@@ -294,7 +294,7 @@ struct AttnPlan {
 };
 
 // A pass of attn_few_kernel (up to 32 vectors) or attn_rows_kernel: the rows
-// are cut until about two CTAs per SM have work, each with at least two
+// are cut until as many CTAs as run at once have work, each with at least two
 // tiles.  Up to 8 cuts of the own rows are one cluster's and leave nothing
 // in the workspace.
 AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t rows, uint32_t step, bool own) {
@@ -305,28 +305,27 @@ AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t row
     p.items = p.tiles * seqs;
     const uint64_t ctas = (uint64_t)p.items * kv_heads;
     const uint32_t most = std::max(1u, cdiv(rows, 2 * step));
-    p.splits = (uint32_t)std::min<uint64_t>({std::max<uint64_t>(1, 2 * 148 / ctas), most, 64});
+    const uint32_t per_sm = p.kern == ATTN_FEW && p.mb == 1 ? 3 : 2;
+    p.splits = (uint32_t)std::min<uint64_t>({std::max<uint64_t>(1, per_sm * 148 / ctas), most, 64});
     if (p.kern == ATTN_FEW && own && p.splits > 1) {
         p.cluster = p.splits <= 8 || rows <= 8 * 4 * step;
-        if (p.cluster) {
-            uint32_t c = 1;
-            while (c * 2 <= std::min(p.splits, 8u)) c *= 2;
-            p.splits = c;
-        }
+        if (p.cluster) p.splits = std::min(p.splits, 8u);
     }
     p.parts = own && (p.cluster || p.splits == 1) ? 0 : p.splits;
     return p;
 }
 
 // The prefix on tcgen05: a tile of 128 vectors (two where there are more)
-// per CTA, one CTA per SM, the rows cut so that all SMs have one.
+// per CTA, one CTA per SM, the rows cut so that all SMs have one, but each
+// four tiles: a shorter part costs as much to begin, and to add later, as to
+// compute, and the own rows' pass takes the SMs that are left.
 AttnPass plan_tc(uint32_t vecs, uint32_t kv_heads, uint32_t rows) {
     AttnPass p;
     p.kern = ATTN_TC;
     p.alternate = vecs <= 128;
     p.tiles = p.items = cdiv(vecs, p.alternate ? 128 : 256);
     const uint32_t ctas = p.items * kv_heads;
-    p.splits = std::min({std::max(1u, 148 / ctas), std::max(1u, cdiv(rows, 2 * TC_ROWS)), ATTN_MAX_PARTS});
+    p.splits = std::min({std::max(1u, 148 / ctas), std::max(1u, rows / (4 * TC_ROWS)), ATTN_MAX_PARTS});
     p.parts = p.splits;
     return p;
 }

@@ -15,7 +15,7 @@
 // the outputs from all CTAs' shared memory, in part order.  The prefix's
 // parts (from the pass before) are added there too.
 //
-// Bound: bytes of K and V; two CTAs on an SM keep 128 to 192 KB under way.
+// Bound: bytes of K and V; three CTAs on an SM keep 96 to 192 KB under way.
 #pragma once
 
 #include <cooperative_groups.h>
@@ -30,7 +30,7 @@ template <typename T, int HD>
 struct FewShape {
     static constexpr int KT = sizeof(T) == 4 ? 8 : 16;  // rows of a chunk
     static constexpr uint32_t TILE = KT * HD * sizeof(T);
-    static constexpr uint32_t STAGES = HD == 128 ? 3 : 4;
+    static constexpr uint32_t STAGES = HD == 128 ? 2 : 3;
     static constexpr uint32_t RING = STAGES * 2 * TILE;  // of one warp
     static constexpr __host__ __device__ uint32_t q_bytes(int mb) { return 16 * mb * HD * sizeof(T); }
     // a warp's output takes its ring's place (or more than that)
@@ -41,7 +41,7 @@ struct FewShape {
 };
 
 template <typename T, int HD, int MB>
-__global__ void __launch_bounds__(FEW_THREADS, 2) attn_few_kernel(const __grid_constant__ PrefixArgs a) {
+__global__ void __launch_bounds__(FEW_THREADS, MB == 1 ? 3 : 2) attn_few_kernel(const __grid_constant__ PrefixArgs a) {
     namespace cg = cooperative_groups;
     constexpr bool F32 = sizeof(T) == 4;
     using S = FewShape<T, HD>;
@@ -77,19 +77,36 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) attn_few_kernel(const __grid_c
         const uint32_t row = row_of(i) + lane;
         if (lane < KT && i < mine && row < w.r1) page = attn_page(a, w, row);
     };
+    // Pages of a multiple of KT rows hold a chunk's rows one behind the other (rows begin at a multiple
+    // of KT: parts do, and so does the own part without a prefix before it).
+    const bool run = a.page_rows.d % KT == 0 && (w.n_prefix % KT == 0 || a.shared);
     uint32_t slot_in = 0;
     auto copy = [&](uint32_t i) {
         if (i < mine) {
-            const uint32_t st = s_kv + slot_in * 2 * S::TILE, row = row_of(i) + lane;
-            const uint64_t off = lane < KT && row < w.r1 ? attn_offset(a, w, head, row, page) : ~0ull;
+            const uint32_t st = s_kv + slot_in * 2 * S::TILE, row0 = row_of(i);
+            if (run && row0 + KT <= w.r1) {
+                const uint64_t o = attn_offset(a, w, head, row0, __shfl_sync(0xffffffffu, page, 0));
+                const uint32_t n = o == ~0ull ? 0u : 16u;
+                const T* src = kb + (o == ~0ull ? 0ull : o + lr * a.row_stride) + lc * E16;
+                const uint64_t by = o == ~0ull ? 0ull : RP * a.row_stride;
 #pragma unroll
-            for (int p = 0; p < KT / RP; ++p) {
-                const uint32_t r = p * RP + lr;
-                const uint64_t o = __shfl_sync(0xffffffffu, off, r);
-                const uint32_t n = o == ~0ull ? 0u : 16u;  // nothing read, zeros written
-                const T* src = kb + (o == ~0ull ? 0ull : o) + lc * E16;
-                cp_async16(st + tile_off<T, HD>(r, lc), src, n);
-                cp_async16(st + S::TILE + vt_off<T, HD>(r, lc), (const uint8_t*)src + v_from_k, n);
+                for (int p = 0; p < KT / RP; ++p) {
+                    cp_async16(st + tile_off<T, HD>(p * RP + lr, lc), src, n);
+                    cp_async16(st + S::TILE + vt_off<T, HD>(p * RP + lr, lc), (const uint8_t*)src + v_from_k, n);
+                    src += by;
+                }
+            } else {
+                const uint32_t row = row0 + lane;
+                const uint64_t off = lane < KT && row < w.r1 ? attn_offset(a, w, head, row, page) : ~0ull;
+#pragma unroll
+                for (int p = 0; p < KT / RP; ++p) {
+                    const uint32_t r = p * RP + lr;
+                    const uint64_t o = __shfl_sync(0xffffffffu, off, r);
+                    const uint32_t n = o == ~0ull ? 0u : 16u;  // nothing read, zeros written
+                    const T* src = kb + (o == ~0ull ? 0ull : o) + lc * E16;
+                    cp_async16(st + tile_off<T, HD>(r, lc), src, n);
+                    cp_async16(st + S::TILE + vt_off<T, HD>(r, lc), (const uint8_t*)src + v_from_k, n);
+                }
             }
             slot_in = slot_in + 1 == ST ? 0 : slot_in + 1;
         }
@@ -151,6 +168,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) attn_few_kernel(const __grid_c
 #pragma unroll
             for (int n = 0; n < NT; ++n) s[b][n][0] = s[b][n][1] = s[b][n][2] = s[b][n][3] = 0.0f;
         if constexpr (!F32) {
+            float s2[MB][NT][4];  // two chains of products instead of one
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+#pragma unroll
+                for (int n = 0; n < NT; ++n) s2[b][n][0] = s2[b][n][1] = s2[b][n][2] = s2[b][n][3] = 0.0f;
 #pragma unroll
             for (int j = 0; j < HD / 32; ++j) {
                 uint32_t q[MB][2][4];
@@ -167,16 +189,22 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) attn_few_kernel(const __grid_c
                     ldsm4(sk + tile_off<T, HD>(n * 8 + (lane & 7), 4 * j + (lane >> 3)), k);
                     if constexpr (QREG) {
                         mma16(s[0][n], qf[2 * j], k[0], k[1], T());
-                        mma16(s[0][n], qf[2 * j + 1], k[2], k[3], T());
+                        mma16(s2[0][n], qf[2 * j + 1], k[2], k[3], T());
                     } else {
 #pragma unroll
                         for (int b = 0; b < MB; ++b) {
                             mma16(s[b][n], q[b][0], k[0], k[1], T());
-                            mma16(s[b][n], q[b][1], k[2], k[3], T());
+                            mma16(s2[b][n], q[b][1], k[2], k[3], T());
                         }
                     }
                 }
             }
+#pragma unroll
+            for (int b = 0; b < MB; ++b)
+#pragma unroll
+                for (int n = 0; n < NT; ++n)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) s[b][n][i] += s2[b][n][i];
         } else {
             float sl[MB][4];
 #pragma unroll
@@ -216,7 +244,7 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) attn_few_kernel(const __grid_c
         uint32_t pf[F32 ? 1 : MB][F32 ? 1 : NT][2];
 #pragma unroll
         for (int b = 0; b < MB; ++b) {
-            float mx[2] = {m[b][0], m[b][1]};
+            float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
             for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -233,9 +261,11 @@ __global__ void __launch_bounds__(FEW_THREADS, 2) attn_few_kernel(const __grid_c
             for (int h = 0; h < 2; ++h) {
                 mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
                 mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-                const float base = mx[h] == -INFINITY ? 0.0f : mx[h];  // nothing seen yet: 2^-inf = 0
-                corr[b][h] = ex2(m[b][h] - base);
-                m[b][h] = mx[h];
+                // the maximum moves only past 2^8 times the old one (fp16 holds that): few outputs are rescaled
+                const float M = mx[h] > m[b][h] + 8.0f ? mx[h] : m[b][h];
+                const float base = M == -INFINITY ? 0.0f : M;  // nothing seen yet: 2^-inf = 0
+                corr[b][h] = M == m[b][h] ? 1.0f : ex2(m[b][h] - base);
+                m[b][h] = M;
                 l[b][h] *= corr[b][h];
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {

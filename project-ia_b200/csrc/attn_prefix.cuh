@@ -203,40 +203,31 @@ struct AttnItem {
 
 __device__ __forceinline__ bool attn_item(const PrefixArgs& a, uint32_t item, uint32_t split, uint32_t vecs, uint32_t step,
                                           AttnItem& w) {
-    uint32_t P = 0, L = 0;
-    if ((a.shared || a.with_prefix) && a.prefix_pages) {
-        P = __ldg(a.prefix_len);
-        if (P > a.max_prefix) {
-            qdev_fail(QDEV_BAD_ARG);
-            P = a.max_prefix;
-        }
-    }
-    uint32_t tile = item;
+    // all loads first: they are the start of every CTA's chain
+    uint32_t tile = item, P = 0, L = 0, s0 = 0, s1 = 0;
     w.seq = 0;
-    if (a.shared) {
-        w.tok0 = 0;
-        w.n_tok = a.n_tokens;
-        w.see0 = 0x40000000;
-    } else {
+    if ((a.shared || a.with_prefix) && a.prefix_pages) P = __ldg(a.prefix_len);
+    if (!a.shared) {
         w.seq = item / a.tiles;
         tile = item - w.seq * a.tiles;
-        if (a.q_start) {
-            const uint32_t s0 = __ldg(a.q_start + w.seq), s1 = __ldg(a.q_start + w.seq + 1);
-            const bool bad = s0 > s1 || s1 > a.n_tokens || s1 - s0 > a.max_q;
-            if (bad) qdev_fail(QDEV_BAD_ARG);
-            w.tok0 = s0;
-            w.n_tok = bad ? 0 : s1 - s0;
-        } else {
-            w.tok0 = w.seq;
-            w.n_tok = 1;
-        }
         L = __ldg(a.lens + w.seq);
-        if (L > a.max_len) {
-            qdev_fail(QDEV_BAD_ARG);
-            L = a.max_len;
+        if (a.q_start) {
+            s0 = __ldg(a.q_start + w.seq);
+            s1 = __ldg(a.q_start + w.seq + 1);
+        } else {
+            s0 = w.seq;
+            s1 = s0 + 1;
         }
-        w.see0 = (int32_t)(P + L) - (int32_t)w.n_tok + 1;
     }
+    const bool bad = s0 > s1 || s1 > a.n_tokens || s1 - s0 > a.max_q;
+    if (P > a.max_prefix || L > a.max_len || bad) {
+        qdev_fail(QDEV_BAD_ARG);
+        P = min(P, a.max_prefix);
+        L = min(L, a.max_len);
+    }
+    w.tok0 = a.shared ? 0 : s0;
+    w.n_tok = a.shared ? a.n_tokens : bad ? 0 : s1 - s0;
+    w.see0 = a.shared ? 0x40000000 : (int32_t)(P + L) - (int32_t)w.n_tok + 1;
     w.n_prefix = P;
     w.n_rows = P + L;
     w.vec0 = tile * vecs;
