@@ -81,21 +81,30 @@ cudaError_t launch_rotate_units(RotateArgs& a, cudaStream_t st) {
     a.rot_units = a.rot / (2 * E);
     const uint32_t U = a.rot_units + (a.head_dim - a.rot) / E;
     a.heads = a.part[0].heads + a.part[1].heads + a.part[2].heads;
-    // Two units a thread where that fills the GPU, else one, for the shortest
-    // path through few tokens.
+    // Two or three units a thread, whichever whole tokens fill better, where
+    // that fills the GPU; else one, for the shortest path through few tokens.
     a.row_step = ROT_THREADS / U;  // U <= 256: head_dim is
     const uint64_t all = (uint64_t)a.n_tokens * a.heads * U;
-    const uint32_t N = all >= 148ull * 8 * ROT_THREADS ? 2 : 1, room = N * a.row_step;
-    a.cta_heads = std::min(a.heads, room);
-    a.cta_tokens = std::min({a.n_tokens, std::max(1u, room / a.cta_heads), ROT_TOKENS, a.rot ? ROT_ANGLES / (a.rot / 2) : ROT_TOKENS});
+    const uint32_t most = a.rot ? std::min(ROT_TOKENS, ROT_ANGLES / (a.rot / 2)) : ROT_TOKENS;
+    uint32_t N = 0, filled = 0;
+    for (uint32_t n = all >= 148ull * 8 * ROT_THREADS ? 2 : 1, last = n == 1 ? 1 : 3; n <= last; ++n) {
+        const uint32_t room = n * a.row_step, h = std::min(a.heads, room), t = std::min({a.n_tokens, std::max(1u, room / h), most});
+        if (N && h * t * 1000 / room <= filled) continue;
+        N = n;
+        filled = h * t * 1000 / room;
+        a.cta_heads = h;
+        a.cta_tokens = t;
+    }
     a.by_units = fast_div_of(U);
     a.by_heads = fast_div_of(a.cta_heads);
     a.by_pairs = fast_div_of(std::max(1u, a.rot / 2));
     const dim3 grid(cdiv(a.n_tokens, a.cta_tokens), cdiv(a.heads, a.cta_heads));
     constexpr bool same = std::is_same<TI, TC>::value;
     if (a.row || !same)
-        return launch_ex(N == 2 ? rotate_kernel<TI, TC, E, 2, true> : rotate_kernel<TI, TC, E, 1, true>, grid, dim3(ROT_THREADS), 0, st, false, a);
-    return launch_ex(N == 2 ? rotate_kernel<TI, TI, E, 2, false> : rotate_kernel<TI, TI, E, 1, false>, grid, dim3(ROT_THREADS), 0, st, false, a);
+        return launch_ex(N == 3 ? rotate_kernel<TI, TC, E, 3, true> : N == 2 ? rotate_kernel<TI, TC, E, 2, true> : rotate_kernel<TI, TC, E, 1, true>,
+                         grid, dim3(ROT_THREADS), 0, st, false, a);
+    return launch_ex(N == 3 ? rotate_kernel<TI, TI, E, 3, false> : N == 2 ? rotate_kernel<TI, TI, E, 2, false> : rotate_kernel<TI, TI, E, 1, false>,
+                     grid, dim3(ROT_THREADS), 0, st, false, a);
 }
 
 template <typename TI, typename TC>
