@@ -52,6 +52,7 @@ struct TcShape {
     static constexpr uint32_t TILE = TC_ROWS * HD * 2;          // one K or V tile, one tile of Q
     static constexpr uint32_t PANEL = TC_ROWS * 128;            // 64 columns of it
     static constexpr size_t SMEM = (size_t)(2 + SLOTS) * TILE + 1024 + 512;
+    static_assert(SLOTS * TILE >= 256 * (HD + 4) * 4 + 1024, "the outputs fit into the ring");
 };
 
 // Descriptor of an MN-major operand in the 128-byte swizzle: 64 contiguous
@@ -300,55 +301,54 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
         if (!ok) m = -INFINITY, l = 0.0f;
         const uint32_t v = (pair ? t * 128 : 0) + row;
         const bool valid = any && v < w.n_vec;
-        float* s_o = reinterpret_cast<float*>(smem + 2 * S::TILE);  // [128][HD + 1], in the ring's place
-        float* s_ml = s_o + 128 * (HD + 1);                         // [128][2]
-        float f0 = 1.0f, f1 = 0.0f;
-        if (!pair) {  // the second stream's share goes through shared memory to the first
-            // (both streams' products are done: each has waited for its own last one)
-            asm volatile("bar.sync 2, 256;" ::: "memory");
-            if (t == 1) {
+        // Both streams' products are done behind this barrier, so the ring's place takes the outputs, a
+        // row of HD + 4 floats per vector (16-byte accesses of neighbouring rows meet different banks),
+        // which one bulk copy each takes to the workspace (rows of 16-byte stores from TMEM took 5 us).
+        asm volatile("bar.sync 2, 256;" ::: "memory");
+        constexpr uint32_t OP = HD + 4;
+        float* s_o = reinterpret_cast<float*>(smem + 2 * S::TILE);  // [2][128][OP]
+        float* mine_o = s_o + (t * 128 + row) * OP;
+        float* s_ml = s_o + 256 * OP;                               // [128][2]
+        auto stage = [&](float f0, const float* other, float f1) {
 #pragma unroll 1
-                for (uint32_t c = 0; c < HD / 16; ++c) {
-                    uint32_t o[16];
-                    if (ok) tmem_ld16(to + c * 16, o);
+            for (uint32_t c = 0; c < HD / 16; ++c) {
+                uint32_t o[16];
+                if (ok) tmem_ld16(to + c * 16, o);
 #pragma unroll
-                    for (int i = 0; i < 16; ++i) s_o[row * (HD + 1) + c * 16 + i] = ok ? __uint_as_float(o[i]) : 0.0f;
+                for (int i = 0; i < 4; ++i) {
+                    float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+                    if (ok) x = make_float4(__uint_as_float(o[4 * i]), __uint_as_float(o[4 * i + 1]), __uint_as_float(o[4 * i + 2]), __uint_as_float(o[4 * i + 3]));
+                    if (other) {
+                        const float4 y = *reinterpret_cast<const float4*>(other + c * 16 + 4 * i);
+                        x = make_float4(x.x * f0 + y.x * f1, x.y * f0 + y.y * f1, x.z * f0 + y.z * f1, x.w * f0 + y.w * f1);
+                    }
+                    *reinterpret_cast<float4*>(mine_o + c * 16 + 4 * i) = x;
                 }
+            }
+        };
+        if (pair || t == 1) stage(1.0f, nullptr, 0.0f);
+        if (!pair) {  // the second stream's share goes through shared memory to the first
+            if (t == 1) {
                 s_ml[row * 2] = m;
                 s_ml[row * 2 + 1] = l;
             }
             asm volatile("bar.sync 2, 256;" ::: "memory");
             if (t == 0) {
                 const float m1 = s_ml[row * 2], l2 = s_ml[row * 2 + 1], M = fmaxf(m, m1);
-                f0 = m == M ? 1.0f : ex2(m - M);
-                f1 = m1 == M ? 1.0f : ex2(m1 - M);
+                const float f0 = m == M ? 1.0f : ex2(m - M), f1 = m1 == M ? 1.0f : ex2(m1 - M);
                 m = M;
                 l = l * f0 + l2 * f1;
+                stage(f0, s_o + (128 + row) * OP, f1);
             }
         }
-        if (pair || t == 0) {
-            uint64_t at = 0;
-            if (valid) {
-                const uint32_t i = fast_div(w.vec0 + v, a.by_group), h = head * a.group + (w.vec0 + v - i * a.group);
-                at = ((uint64_t)split * a.n_tokens + i) * a.n_heads + h;
-                __stcg(a.part_ml + at, make_float2(m, l));
-            }
-#pragma unroll 1
-            for (uint32_t c = 0; c < HD / 16; ++c) {
-                uint32_t o[16];
-                if (ok) tmem_ld16(to + c * 16, o);
-                float x[16];
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    x[i] = ok ? __uint_as_float(o[i]) : 0.0f;
-                    if (!pair) x[i] = x[i] * f0 + s_o[row * (HD + 1) + c * 16 + i] * f1;
-                }
-                if (valid) {
-                    float4* d = reinterpret_cast<float4*>(a.part_o + at * HD + c * 16);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) __stcg(d + i, make_float4(x[4 * i], x[4 * i + 1], x[4 * i + 2], x[4 * i + 3]));
-                }
-            }
+        if (valid && (pair || t == 0)) {
+            const uint32_t i = fast_div(w.vec0 + v, a.by_group), h = head * a.group + (w.vec0 + v - i * a.group);
+            const uint64_t at = ((uint64_t)split * a.n_tokens + i) * a.n_heads + h;
+            __stcg(a.part_ml + at, make_float2(m, l));
+            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+            asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(a.part_o + at * HD), "r"(smem_u32(mine_o)), "r"(HD * 4) : "memory");
+            asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+            asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
         }
     } else if (warp < 12) {
         // ---- copies: slots take K0 V0 K1 V1 ...; a warp brings 32 rows of each -----------------
