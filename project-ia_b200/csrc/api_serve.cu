@@ -599,12 +599,12 @@ q_error_code q_b200_verify_draft(const q_b200_verify_args* r, void* stream) {
         a.cd = 1.44269504088896340736 / (double)r->temperature;
         a.c = (float)a.cd;
     }
-    // CTAs of a sequence: as many as run at once (two on an SM), but a warp's
-    // segment fills a lane's vectors at least once; 16 of them, which not
-    // every part of the GPU has room for twice, only for a few sequences
-    const uint32_t once = VER_VECS * 32 * (16 / es) * VER_WARPS;
+    // CTAs of a sequence: as many as run at once, but a warp's segment fills a
+    // lane's vectors at least once; 16 of them, which not every part of the
+    // GPU has room for, only for a few sequences
+    const uint32_t once = ver_vecs(kind) * 32 * (16 / es) * VER_WARPS;
     uint32_t CL = r->n_seqs <= 4 ? 16 : 8;
-    while (CL > 1 && ((uint64_t)r->n_seqs * CL > 2 * 148 || (uint64_t)(CL / 2) * once >= r->vocab)) CL /= 2;
+    while (CL > 1 && ((uint64_t)r->n_seqs * CL > 148u * ver_ctas(kind) || (uint64_t)(CL / 2) * once >= r->vocab)) CL /= 2;
     a.seg = (cdiv(r->vocab, (uint64_t)CL * VER_WARPS) + 7) & ~7u;
     cudaStream_t st = (cudaStream_t)stream;
     switch (r->dtype) {

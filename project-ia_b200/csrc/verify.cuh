@@ -28,13 +28,17 @@
 
 namespace qb200 {
 
-static constexpr uint32_t VER_THREADS = 512;  // two CTAs on an SM: 64 registers a thread
+static constexpr uint32_t VER_THREADS = 512;
 static constexpr uint32_t VER_WARPS = VER_THREADS / 32;
 static constexpr uint32_t VER_MAX_CL = 16;
 static constexpr uint32_t VER_MAX_DRAFT = 31;
 static constexpr uint32_t VER_CHUNKS = 16;  // sums that a warp keeps of its segment's chunks, the last one of all behind
 
-static constexpr int VER_VECS = 2;  // vectors of each of two rows that a lane has under way
+// CTAs that share an SM, and vectors of each of two rows that a lane has under
+// way: probabilities take 128 registers and four vectors; logits, whose
+// clusters of 8 would not all find room one CTA to an SM, half of both.
+constexpr __host__ __device__ int ver_ctas(int kind) { return kind == 0 ? 1 : 2; }
+constexpr __host__ __device__ int ver_vecs(int kind) { return kind == 0 ? 4 : 2; }
 static constexpr int VER_SUMS = 8;  // of one row, where whole rows are summed
 
 enum : int { VER_PROBS = 0, VER_LOGITS = 1, VER_GREEDY = 2 };
@@ -58,7 +62,7 @@ struct VerifyArgs {
 // 16-byte vectors of E, 32 E apart; `none` past the end.  A vector past the
 // end is loaded from the row's start instead and replaced, so that all loads
 // are issued before the first is looked at.
-template <typename T, int E, int NV = VER_VECS>
+template <typename T, int E, int NV>
 struct RowPart {
     Vec<T, E> v[NV];
     __device__ __forceinline__ void load(const T* row, uint32_t i0, uint32_t end, bool vec, float none) {
@@ -116,12 +120,12 @@ __device__ __forceinline__ double logit_weight(float v, float low, double c, dou
 // >= 0 is hi + lo without error, and so is each addition's own error.  On
 // fp64 units the two conversions of each entry alone would take 4 us for a
 // batch of 64 on 128 K entries.
-template <typename T, int E>
-__device__ __forceinline__ double rest_sum(const RowPart<T, E>& xp, const RowPart<T, E>& xq, bool two) {
+template <typename T, int E, int NV>
+__device__ __forceinline__ double rest_sum(const RowPart<T, E, NV>& xp, const RowPart<T, E, NV>& xq, bool two) {
     static_assert(E % 2 == 0, "pairs");
     F2 s, c;
 #pragma unroll
-    for (int k = 0; k < VER_VECS; ++k) {
+    for (int k = 0; k < NV; ++k) {
         float p[E], q[E];
         to_float(xp.v[k], p);
         if (two) to_float(xq.v[k], q);
@@ -162,9 +166,9 @@ __device__ __forceinline__ unsigned long long argmax_key64(float v, uint32_t i) 
 }
 
 template <typename T, int KIND>
-__global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs a) {
+__global__ void __launch_bounds__(VER_THREADS, ver_ctas(KIND)) verify_kernel(const VerifyArgs a) {
     namespace cg = cooperative_groups;
-    constexpr int E = 16 / sizeof(T);
+    constexpr int E = 16 / sizeof(T), VER_VECS = ver_vecs(KIND);
     cg::cluster_group cluster = cg::this_cluster();
     const uint32_t CL = cluster.num_blocks(), rank = cluster.block_rank();
     const uint32_t b = blockIdx.x / CL, tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -178,6 +182,7 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
     __shared__ double s_rest[2][VER_MAX_CL * VER_WARPS];          // segment sums of what is drawn from
     __shared__ double s_chunk[VER_WARPS][VER_CHUNKS];             // this CTA's chunk sums
     __shared__ double s_table[KIND == VER_LOGITS ? VER_TABLE : 1];
+    __shared__ float2 s_row[KIND == VER_LOGITS ? ROWS : 1];       // (maximum, sum) of each row
     __shared__ double s_z[2], s_thr;
     __shared__ float s_m[2];
     __shared__ uint32_t s_n, s_owner, s_len;
@@ -298,6 +303,19 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
             *cluster.map_shared_rank(&s_stat[r * VER_MAX_CL + rank], to) = w;
         }
         cluster.sync();
+        if (KIND == VER_LOGITS) {  // a lane adds a row's shares
+            if (tid < R) {
+                float m = -INFINITY, s = 0.0f;
+                for (uint32_t k = 0; k < CL; ++k) m = fmaxf(m, __uint_as_float((uint32_t)(s_stat[tid * VER_MAX_CL + k] >> 32)));
+                for (uint32_t k = 0; k < CL; ++k) {
+                    const unsigned long long w = s_stat[tid * VER_MAX_CL + k];
+                    const float mk = __uint_as_float((uint32_t)(w >> 32));
+                    if (mk != -INFINITY) s = fmaf(__uint_as_float((uint32_t)w), ex2((mk - m) * a.c), s);
+                }
+                s_row[tid] = make_float2(m, s);
+            }
+            __syncthreads();
+        }
         if (warp == 0) {
             if (KIND == VER_GREEDY) {
                 unsigned long long best = 0;
@@ -317,17 +335,9 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
                 }
             } else {
                 auto law = [&](uint32_t r, float logit) -> double {  // softmax at one entry
-                    float m = -INFINITY;
-                    for (uint32_t k = 0; k < CL; ++k)
-                        m = fmaxf(m, __uint_as_float((uint32_t)(s_stat[r * VER_MAX_CL + k] >> 32)));
-                    double s = 0.0;
-                    for (uint32_t k = 0; k < CL; ++k) {
-                        const unsigned long long w = s_stat[r * VER_MAX_CL + k];
-                        const float mk = __uint_as_float((uint32_t)(w >> 32));
-                        if (mk != -INFINITY) s += (double)__uint_as_float((uint32_t)w) * (double)ex2((mk - m) * a.c);
-                    }
-                    const double e = exp2(((double)logit - (double)m) * a.cd);
-                    return s > 0.0 && e > 0.0 ? e / s : 0.0;
+                    const float2 row = s_row[r];
+                    const double e = exp2(((double)logit - (double)row.x) * a.cd);
+                    return row.y > 0.0f && e > 0.0 ? e / (double)row.y : 0.0;
                 };
                 bool ok = false;
                 if (live) {
@@ -366,13 +376,12 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
         for (int k = 0; k < 2; ++k) {  // any reference near the maximum does
             m[k] = -INFINITY;
             const uint32_t r = k ? Rt + n : n;
-            if (n < len && (k == 0 || qrow))
-                for (uint32_t c = 0; c < CL; ++c) m[k] = fmaxf(m[k], __uint_as_float((uint32_t)(s_stat[r * VER_MAX_CL + c] >> 32)));
+            if (n < len && (k == 0 || qrow)) m[k] = s_row[r].x;
         }
         if (n >= len) {  // a row that no test has looked at
             float top = -INFINITY;
             for (uint32_t i0 = g0; i0 < g1; i0 += VER_VECS * 32 * E) {
-                RowPart<T, E> x;
+                RowPart<T, E, VER_VECS> x;
                 x.load(prow, i0, g1, a.vec, -INFINITY);
 #pragma unroll
                 for (int k = 0; k < VER_VECS; ++k) {
@@ -395,7 +404,7 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
             double s = 0.0;
             if (row && m[k] > -INFINITY && m[k] < INFINITY)
                 for (uint32_t i0 = g0; i0 < g1; i0 += VER_VECS * 32 * E) {
-                    RowPart<T, E> x;
+                    RowPart<T, E, VER_VECS> x;
                     x.load(row, i0, g1, a.vec, -INFINITY);
 #pragma unroll
                     for (int q = 0; q < VER_VECS; ++q) {
@@ -450,7 +459,7 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
         const bool two = rest && qrow;
         double sum = 0.0;
         for (uint32_t i0 = g0, chunk = 0; i0 < g1; i0 += VER_VECS * 32 * E, ++chunk) {
-            RowPart<T, E> xp, xq;
+            RowPart<T, E, VER_VECS> xp, xq;
             xp.load(prow, i0, g1, a.vec, none);
             if (two) xq.load(qrow, i0, g1, a.vec, none);
             double part = 0.0;
@@ -535,7 +544,7 @@ __global__ void __launch_bounds__(VER_THREADS, 2) verify_kernel(const VerifyArgs
             // the second pass, for a border that rounding hid: the segment's last weight
             if (pass) c0 = g0, at = -INFINITY;
             for (; c0 < g1 && !found; c0 += VER_VECS * 32 * E) {
-                RowPart<T, E> xp, xq;
+                RowPart<T, E, VER_VECS> xp, xq;
                 xp.load(prow, c0, g1, a.vec, none);
                 if (rest && qrow) xq.load(qrow, c0, g1, a.vec, none);
 #pragma unroll 1
