@@ -1,7 +1,9 @@
 // api_serve.cu — the serving operators' entry points: argument checks, plans
 // and launches (kernels: rotate.cuh, attn_prefix.cuh, verify.cuh).
 //
-// Nothing is allocated and nothing is kept between calls; checks that need
+// Every launch is a programmatic dependent one: a kernel's CTAs may be set up
+// beside the tail of the work before it, and wait for that work's end before
+// they read or write.  Nothing is allocated and nothing is kept between calls; checks that need
 // no device come first, so that a refusal is the same with and without one.
 #include <cmath>
 
@@ -102,9 +104,9 @@ cudaError_t launch_rotate_units(RotateArgs& a, cudaStream_t st) {
     constexpr bool same = std::is_same<TI, TC>::value;
     if (a.row || !same)
         return launch_ex(N == 3 ? rotate_kernel<TI, TC, E, 3, true> : N == 2 ? rotate_kernel<TI, TC, E, 2, true> : rotate_kernel<TI, TC, E, 1, true>,
-                         grid, dim3(ROT_THREADS), 0, st, false, a);
+                         grid, dim3(ROT_THREADS), 0, st, true, a);
     return launch_ex(N == 3 ? rotate_kernel<TI, TI, E, 3, false> : N == 2 ? rotate_kernel<TI, TI, E, 2, false> : rotate_kernel<TI, TI, E, 1, false>,
-                     grid, dim3(ROT_THREADS), 0, st, false, a);
+                     grid, dim3(ROT_THREADS), 0, st, true, a);
 }
 
 template <typename TI, typename TC>
@@ -376,7 +378,7 @@ size_t attn_bytes(const q_b200_attn_args* r, const AttnPlan& p) {
 }
 
 template <typename T, int HD, int MB>
-cudaError_t launch_few(PrefixArgs& a, const AttnPass& p, uint32_t kv_heads, bool pdl, cudaStream_t st) {
+cudaError_t launch_few(PrefixArgs& a, const AttnPass& p, uint32_t kv_heads, cudaStream_t st) {
     using S = FewShape<T, HD>;
     constexpr uint32_t smem = S::smem(MB);
     if (cudaError_t e = ensure_smem_attr((const void*)attn_few_kernel<T, HD, MB>, smem)) return e;
@@ -394,11 +396,9 @@ cudaError_t launch_few(PrefixArgs& a, const AttnPass& p, uint32_t kv_heads, bool
         attr[n].val.clusterDim.y = attr[n].val.clusterDim.z = 1;
         ++n;
     }
-    if (pdl) {
-        attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-        attr[n].val.programmaticStreamSerializationAllowed = 1;
-        ++n;
-    }
+    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[n].val.programmaticStreamSerializationAllowed = 1;
+    ++n;
     cfg.attrs = attr;
     cfg.numAttrs = n;
     g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
@@ -406,7 +406,7 @@ cudaError_t launch_few(PrefixArgs& a, const AttnPass& p, uint32_t kv_heads, bool
 }
 
 template <typename T, int HD>
-cudaError_t launch_pass(PrefixArgs a, const AttnPass& p, uint32_t kv_heads, bool pdl, cudaStream_t st) {
+cudaError_t launch_pass(PrefixArgs a, const AttnPass& p, uint32_t kv_heads, cudaStream_t st) {
     a.tiles = p.tiles;
     a.splits = p.splits;
     if constexpr (sizeof(T) == 2 && HD >= 64) {
@@ -414,33 +414,34 @@ cudaError_t launch_pass(PrefixArgs a, const AttnPass& p, uint32_t kv_heads, bool
             a.alternate = p.alternate;
             if (cudaError_t e = ensure_smem_attr((const void*)attn_prefix_tc_kernel<T, HD>, (int)TcShape<HD>::SMEM)) return e;
             return launch_ex(attn_prefix_tc_kernel<T, HD>, dim3(p.splits, p.items, kv_heads), dim3(TC_THREADS),
-                             TcShape<HD>::SMEM, st, pdl, a);
+                             TcShape<HD>::SMEM, st, true, a);
         }
     }
     if (p.kern == ATTN_FEW)
-        return p.mb == 1 ? launch_few<T, HD, 1>(a, p, kv_heads, pdl, st) : launch_few<T, HD, 2>(a, p, kv_heads, pdl, st);
+        return p.mb == 1 ? launch_few<T, HD, 1>(a, p, kv_heads, st) : launch_few<T, HD, 2>(a, p, kv_heads, st);
     const size_t smem = attn_rows_smem<T, HD, 4>();
     if (cudaError_t e = ensure_smem_attr((const void*)attn_rows_kernel<T, HD, 4>, (int)smem)) return e;
-    return launch_ex(attn_rows_kernel<T, HD, 4>, dim3(p.splits, p.items, kv_heads), dim3(ATTN_THREADS), smem, st, pdl, a);
+    return launch_ex(attn_rows_kernel<T, HD, 4>, dim3(p.splits, p.items, kv_heads), dim3(ATTN_THREADS), smem, st, true, a);
 }
 
 // The prefix's pass, then the own rows' beside its tail (programmatic
-// dependent launch: a pass waits for the one before it only when its own
-// rows are done), which adds the prefix's parts itself unless its rows are
+// dependent launch: a pass that is not the call's first waits for the one
+// before it only when its own rows are done), which adds the prefix's parts itself unless its rows are
 // in parts too: then the join adds all of them.
 template <typename T, int HD>
 cudaError_t launch_attn(PrefixArgs& a, const AttnPlan& p, uint32_t kv_heads, cudaStream_t st) {
     cudaError_t e = cudaSuccess;
     if (p.shared) {
-        a.shared = 1;
-        if ((e = launch_pass<T, HD>(a, p.pre, kv_heads, false, st))) return e;
+        a.shared = a.first = 1;
+        if ((e = launch_pass<T, HD>(a, p.pre, kv_heads, st))) return e;
     }
     a.shared = 0;
+    a.first = !p.shared;
     a.with_prefix = !p.shared;
     a.part0 = p.shared ? p.pre.parts : 0u;
     a.last = p.own.parts == 0;
     a.merge = a.last ? a.part0 : 0u;
-    if ((e = launch_pass<T, HD>(a, p.own, kv_heads, p.shared, st)) || a.last) return e;
+    if ((e = launch_pass<T, HD>(a, p.own, kv_heads, st)) || a.last) return e;
     a.n_parts = p.parts;
     return launch_ex(attn_join_kernel<T, HD>, dim3(cdiv((uint64_t)a.n_tokens * a.n_heads * (HD / 4), 128)), dim3(128), 0, st, true, a);
 }
@@ -539,13 +540,15 @@ cudaError_t launch_verify(const VerifyArgs& a, uint32_t n_seqs, uint32_t CL, cud
     cfg.gridDim = dim3(n_seqs * CL);
     cfg.blockDim = dim3(VER_THREADS);
     cfg.stream = st;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeClusterDimension;
     attr[0].val.clusterDim.x = CL;
     attr[0].val.clusterDim.y = 1;
     attr[0].val.clusterDim.z = 1;
+    attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[1].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = 2;
     g_kernel_launches.fetch_add(1, std::memory_order_relaxed);
     return cudaLaunchKernelEx(&cfg, verify_kernel<T, KIND>, a);
 }

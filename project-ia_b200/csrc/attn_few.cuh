@@ -58,7 +58,8 @@ __global__ void __launch_bounds__(FEW_THREADS, MB == 1 ? 3 : 2) attn_few_kernel(
     const uint32_t split = blockIdx.x, head = blockIdx.z;
     const uint32_t C = a.cluster ? gridDim.x : 1;
 
-    if (a.shared) pdl_trigger();  // the pass over the own rows may start beside this one
+    if (a.first) pdl_wait();
+    pdl_trigger();  // the pass after this one may start beside it
     AttnItem w;
     if (!attn_item(a, blockIdx.y, split, RV, 4 * KT, w)) {  // the same for a whole cluster
         pdl_wait();

@@ -54,6 +54,7 @@ struct PrefixArgs {
     uint32_t last;       // 1: writes out itself, after `merge` parts of the pass before it
     uint32_t merge;
     uint32_t n_parts;    // of the join
+    uint32_t first;      // waits for the stream's work before it; a later pass reads the call's inputs at once
     uint32_t cluster;    // attn_few_kernel: the splits are a cluster's
     uint32_t alternate;  // tcgen05 pass: one tile of vectors, even and odd row tiles
     uint32_t shared;     // 1: the prefix for all tokens; 0: per sequence
@@ -330,7 +331,8 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
     const uint32_t wm = warp % WM, wn = warp / WM;
     const uint32_t split = blockIdx.x, head = blockIdx.z;
 
-    if (a.shared) pdl_trigger();  // the pass over the own rows may start beside this one
+    if (a.first) pdl_wait();
+    pdl_trigger();  // the pass after this one may start beside it
     AttnItem w;
     if (!attn_item(a, blockIdx.y, split, 16 * WM, KT, w)) {
         pdl_wait();
@@ -684,6 +686,7 @@ template <typename T, int HD>
 __global__ void __launch_bounds__(128) attn_join_kernel(const __grid_constant__ PrefixArgs a) {
     const uint64_t e = (uint64_t)blockIdx.x * 128 + threadIdx.x, stride = (uint64_t)a.n_tokens * a.n_heads;
     pdl_wait();
+    pdl_trigger();
     const uint64_t id = e / (HD / 4);
     if (id >= stride) return;
     const uint32_t c = (uint32_t)(e % (HD / 4)), tok = (uint32_t)(id / a.n_heads), h = (uint32_t)(id - (uint64_t)tok * a.n_heads);

@@ -159,12 +159,8 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
     uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(drain + 1);
 
     const uint32_t tid = threadIdx.x, warp = __shfl_sync(0xffffffffu, tid >> 5, 0), lane = tid & 31, head = blockIdx.z, split = blockIdx.x;
-    pdl_trigger();  // the pass over the own rows may start beside this one
     const bool pair = !a.alternate;  // two tiles of vectors
 
-    AttnItem w;
-    const bool any = attn_item(a, blockIdx.y, split, pair ? 256 : 128, TC_ROWS, w);
-    const uint32_t n_tiles = any ? (w.r1 - w.r0 + TC_ROWS - 1) / TC_ROWS : 0;
     if (tid == 0) {
         for (uint32_t i = 0; i < NS; ++i) {
             mbar_init(&landed[i], 128);  // each copying thread's copies
@@ -187,6 +183,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
                      : "memory");
         asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
     }
+    // barriers and TMEM are set up beside the tail of the stream's work before this pass
+    pdl_wait();
+    pdl_trigger();  // the pass over the own rows may start beside this one
+    AttnItem w;
+    const bool any = attn_item(a, blockIdx.y, split, pair ? 256 : 128, TC_ROWS, w);
+    const uint32_t n_tiles = any ? (w.r1 - w.r0 + TC_ROWS - 1) / TC_ROWS : 0;
     tc_fence_before();
     __syncthreads();
     tc_fence_after();

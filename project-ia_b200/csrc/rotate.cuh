@@ -277,6 +277,8 @@ template <typename TI, typename TC, int E, int N, bool APPEND>
 __global__ void __launch_bounds__(ROT_THREADS) rotate_kernel(const __grid_constant__ RotateArgs a) {
     __shared__ __align__(16) float s_cos[ROT_ANGLES], s_sin[ROT_ANGLES];
     __shared__ uint64_t s_off[ROT_TOKENS];  // append: the token's row in the cache; ~0: none
+    pdl_wait();
+    pdl_trigger();
     const uint32_t tid = threadIdx.x, t0 = blockIdx.x * a.cta_tokens, h0 = blockIdx.y * a.cta_heads;
     const uint32_t nt = min(a.cta_tokens, a.n_tokens - t0), nh = min(a.cta_heads, a.heads - h0);
     // this thread's unit of every row that it takes: rows rsub, rsub + step, ... of the CTA's nt x nh

@@ -189,6 +189,8 @@ __global__ void __launch_bounds__(VER_THREADS, ver_ctas(KIND)) verify_kernel(con
 
     const T* target = reinterpret_cast<const T*>(a.target) + b * a.t_seq;
     const T* draft = a.draft && KIND != VER_GREEDY ? reinterpret_cast<const T*>(a.draft) + b * a.d_seq : nullptr;
+    pdl_wait();
+    pdl_trigger();
     cluster.barrier_arrive();  // every CTA of the cluster runs before its shared memory is written to
 
     // lane i of the first warp keeps draft i
