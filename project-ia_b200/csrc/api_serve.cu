@@ -189,7 +189,8 @@ q_error_code q_b200_rope(const q_b200_rope_args* r, void* stream) {
     if (!r || !r->x || !r->out || !r->pos || !r->plan) return Q_ERR_INVALID_ARG;
     if (!known(r->dtype)) return Q_ERR_INVALID_DTYPE;
     if (r->reserved || r->transpose > 1) return Q_ERR_INVALID_ARG;
-    if (r->n_tokens == 0 || r->n_heads == 0 || r->head_dim == 0 || r->head_dim > 256) return Q_ERR_INVALID_SIZE;
+    if (r->n_tokens == 0 || r->n_heads == 0 || r->n_heads > 65535 || r->head_dim == 0 || r->head_dim > 256)
+        return Q_ERR_INVALID_SIZE;
     if (q_error_code rc = check_plan(r->plan, r->head_dim)) return rc;
     const uint32_t es = size_of(r->dtype);
     if (((addr(r->x) | addr(r->out)) & (es - 1)) || (addr(r->pos) & 3)) return Q_ERR_MISALIGNED;
@@ -225,6 +226,7 @@ q_error_code q_b200_kv_append(const q_b200_append_args* r, void* stream) {
     if (r->reserved || (r->q && !r->q_out)) return Q_ERR_INVALID_ARG;
     if (r->n_tokens == 0 || r->n_seqs == 0 || r->pages_per_seq == 0 || (r->q && r->n_heads == 0)) return Q_ERR_INVALID_SIZE;
     if (r->kv.head_dim > 256 || (!r->seq && r->n_tokens > r->n_seqs)) return Q_ERR_INVALID_SIZE;
+    if ((uint64_t)2 * r->kv.n_kv_heads + (r->q ? r->n_heads : 0) > 65535) return Q_ERR_INVALID_SIZE;
     if (r->plan)
         if (q_error_code rc = check_plan(r->plan, r->kv.head_dim)) return rc;
     const uint32_t es = size_of(r->dtype), ec = size_of(r->kv.dtype);
@@ -477,6 +479,7 @@ q_error_code q_b200_attn_prefix(const q_b200_attn_args* r, void* stream) {
     if (in < 16 || to < 16) return Q_ERR_MISALIGNED;
     if ((addr(r->q_start) | addr(r->pages) | addr(r->lens) | addr(r->prefix_pages) | addr(r->prefix_len)) & 3) return Q_ERR_MISALIGNED;
     const AttnPlan p = plan_attn(r);
+    if (p.own.items > 65535 || p.pre.items > 65535) return Q_ERR_INVALID_SIZE;  // a grid's second dimension
     const size_t need = attn_bytes(r, p);
     if (need && !r->work) return Q_ERR_INVALID_ARG;
     if (need && r->work_bytes < need) return Q_ERR_INVALID_SIZE;

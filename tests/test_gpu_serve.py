@@ -400,6 +400,60 @@ def test_attn_scores_of_the_types_lowest_value():
     assert ((b.out.double() - want).abs() <= half_step("bf16") * (2 * want.abs() + A) + 2.0**-16 * A).all()
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,prefix,seqs", [
+    (8, 2, 64, 700, 3), (16, 2, 128, 1300, 5), (16, 1, 128, 4000, 9), (32, 2, 64, 2500, 20), (64, 1, 128, 1000, 9), (8, 1, 32, 900, 40)])
+def test_attn_scores_that_grow_along_the_rows(dtype, heads, kv_heads, dim, prefix, seqs):
+    # the running maximum has to move again and again, everywhere at another row: up to 16 exp2 units a tile, down, and up
+    b = Batch(dim + prefix, dtype, heads, kv_heads, dim, 16, prefix, [40 + 7 * i for i in range(seqs)], [1] * seqs, poison=False)
+    ramp = torch.rand(b.keys.shape[:3], generator=gen(1), device="cuda") * 2
+    for i, pg in enumerate(b.prefix_pages.tolist()):
+        ramp[pg] += 6.0 * (i * 16 / prefix)
+    b.keys.mul_(ramp[..., None].to(b.keys.dtype))
+    b.call()
+    b.check()
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("scale", [-0.3, 0.0])
+def test_attn_scales_that_are_not_positive(dtype, scale):
+    b = Batch(14, dtype, 16, 2, 64, 16, 300, [50, 20, 9, 9, 9], [1] * 5, poison=False)
+    a = b.args()
+    a.scale = scale
+    b.work = torch.empty(max(16, Q.lib.q_b200_attn_work_bytes(C.byref(a))), dtype=torch.uint8, device="cuda")
+    a.work, a.work_bytes = b.work.data_ptr(), b.work.numel()
+    Q.check(Q.lib.q_b200_attn_prefix(C.byref(a), stream()), "attn")
+    b.q.mul_(scale * math.sqrt(64))  # the reference's scale is 1 / sqrt(dim)
+    want, room = b.want()
+    within(b.out, want, room + (half_step(dtype) * 8 if dtype != "f32" else 0.0), dtype)  # q rounded again: scores off by H Y, Y < 4
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dim", [32, 128])
+@pytest.mark.parametrize("prefix,rows", [(0, [30, 5, 1, 9]), (1, [0, 0, 0, 0]), (129, [7, 0, 300, 2]), (0, [0, 0, 0, 0])])
+def test_attn_lengths_far_below_their_bounds(dtype, dim, prefix, rows):
+    # a plan for 5000 rows of prefix and 600 own ones meets nearly none, or none: parts without a row
+    b = Batch(15, dtype, 16, 1, dim, 16, 5000, [600] * 4, [1] * 4, poison=False)
+    b.lens.copy_(ints(rows))
+    b.prefix_len.copy_(ints([prefix]))
+    b.out.fill_(5.0)
+    b.call()
+    b.rows, b.prefix, pages = rows, prefix, b.prefix_pages
+    b.prefix_pages = pages[: -(-prefix // 16)]
+    b.check()
+
+
+def test_attn_one_token_at_every_length():
+    # the row count passes every boundary of pages, chunks and parts; one bound for all, as in a captured graph
+    for dtype, dim in (("bf16", 128), ("f32", 64)):
+        b = Batch(16, dtype, 8, 2, dim, 17, 0, [1], [1], poison=False, room_rows=400)
+        for n in list(range(0, 70)) + [127, 128, 129, 255, 256, 257, 399, 400]:
+            b.rows = [n]
+            b.lens.copy_(ints([n]))
+            b.call(max_len=400)
+            b.check()
+
+
 def test_attn_bad_pages_and_lengths_are_skipped():
     b = Batch(9, "f32", 4, 2, 64, 16, 64, [40, 30], [1, 1], poison=False)
     good = b.args()
@@ -574,7 +628,7 @@ def drafted(g, S, K, V, apart=0.7, T=1.0):
 
 @pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("kind,T", [("probs", 1.0), ("logits", 0.7), ("logits", 0.0)])
-@pytest.mark.parametrize("S,K,V", [(1, 1, 1), (3, 2, 7), (5, 4, 259), (2, 0, 1000), (17, 3, 4097), (64, 7, 2050), (1, 31, 8192), (2, 4, 128256),
+@pytest.mark.parametrize("S,K,V", [(1, 1, 1), (3, 2, 7), (5, 4, 259), (2, 0, 1000), (17, 3, 4097), (64, 7, 2050), (1, 31, 8192), (24, 2, 50001), (2, 4, 128256),
                                    (200, 2, 515)])
 def test_verify(dtype, kind, T, S, K, V):
     target, draft, tokens, u = drafted(gen(S * 100 + V), S, K, V, T=T or 1.0)
@@ -720,6 +774,77 @@ def test_a_speculative_step(dtype):
         assert np.array_equal(chosen.cpu().numpy(), got) and np.array_equal(count.cpu().numpy(), m)
         state["lens"] = [x + int(c) for x, c in zip(state["lens"], count.cpu())]
     assert Q.lib.q_b200_device_status() == 0
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_steps_without_a_wait_between_them(dtype):
+    """Each call reads what the one before it has written, twenty steps behind one another: the same bits as with a wait after
+    every call (the kernels may be set up beside the tail of the work before them)."""
+    H, KV, D, B, V = 16, 2, 64, 3, 500
+    g, p = gen(50), make_plan(D, "half")
+    b = Batch(51, dtype, H, KV, D, 16, 200, [1] * B, [1] * B, room_rows=40, poison=False)
+    pool = b.pool.clone()
+    xs = normal(g, 20, B, H + 2 * KV, D, dtype=dtype)
+    head = normal(g, H * D, V) * 0.3
+    u = torch.rand(B, 1, generator=g, device="cuda")
+    q, turned = torch.empty_like(xs[0][:, :H]), torch.empty_like(xs[0][:, :H])
+    b.q = turned
+    a = b.args(max_len=40)
+
+    def run(wait):
+        b.pool.copy_(pool)
+        b.lens.fill_(1)
+        row, seen = ints([0] * B), []
+        torch.cuda.synchronize()
+        for x in xs:
+            q.copy_(x[:, :H])
+            do_append(b.keys, b.values, dtype, x[:, H:H + KV], x[:, H + KV:], b.pages, None, row, None, p, dtype)
+            if wait: torch.cuda.synchronize()
+            do_rope(q, turned, row, p, dtype=dtype)
+            do_rope(turned, turned, row, p, dtype=dtype)
+            if wait: torch.cuda.synchronize()
+            Q.check(Q.lib.q_b200_attn_prefix(C.byref(a), stream()), "attn")
+            Q.check(Q.lib.q_b200_attn_prefix(C.byref(a), stream()), "attn")
+            if wait: torch.cuda.synchronize()
+            logits = torch.matmul(b.out.float().view(B, H * D), head).view(B, 1, V)
+            out, n = ints([[0]] * B), ints([0] * B)
+            v = Q.q_b200_verify_args(logits.data_ptr(), None, V, V, 0, 0, None, None, u.data_ptr(), out.data_ptr(), n.data_ptr(), B, 0, V,
+                                     0, Q.Q_B200_LOGITS, 1.0)
+            Q.check(Q.lib.q_b200_verify_draft(C.byref(v), stream()), "verify")
+            seen += [b.out.clone(), out.clone()]
+            if wait: torch.cuda.synchronize()
+            row += 1
+            b.lens += 1
+        torch.cuda.synchronize()
+        return seen + [b.pool.clone()]
+
+    slow, fast = run(True), run(False)
+    assert all(torch.equal(x, y) for x, y in zip(slow, fast))
+    assert Q.lib.q_b200_device_status() == 0
+
+
+def test_calls_on_two_streams_at_once():
+    streams, jobs = [torch.cuda.Stream() for _ in range(2)], []
+    for i in range(2):
+        g = gen(60 + i)
+        x, p = normal(g, 3000, 8, 128, dtype="bf16"), make_plan(128)
+        pos = torch.randint(0, 5000, (3000,), generator=g, device="cuda", dtype=torch.int32)
+        target, draft, tokens, u = drafted(g, 20, 3, 20000)
+        jobs.append((x, torch.empty_like(x), pos, p, target, draft, tokens, u, torch.zeros(20, 4, dtype=torch.int32, device="cuda"),
+                     torch.zeros(20, dtype=torch.int32, device="cuda")))
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, (x, out, pos, p, target, draft, tokens, u, chosen, n) in zip(streams, jobs):
+            do_rope(x, out, pos, p, dtype="bf16", on=s.cuda_stream)
+            v = Q.q_b200_verify_args(target.data_ptr(), draft.data_ptr(), 4 * 20000, 20000, 3 * 20000, 20000, tokens.data_ptr(), None, u.data_ptr(),
+                                     chosen.data_ptr(), n.data_ptr(), 20, 3, 20000, 0, Q.Q_B200_LOGITS, 0.8)
+            Q.check(Q.lib.q_b200_verify_draft(C.byref(v), s.cuda_stream), "verify")
+    torch.cuda.synchronize()
+    for x, out, pos, p, target, draft, tokens, u, chosen, n in jobs:
+        want, room = turn64(x, pos, p)
+        within(out, want, room, "bf16")
+        got, m = verify64(target, draft, tokens, u, "logits", 0.8)
+        assert np.array_equal(chosen.cpu().numpy(), got) and np.array_equal(n.cpu().numpy(), m)
 
 
 @pytest.mark.parametrize("call", ["rope", "append", "attn", "verify"])

@@ -80,7 +80,7 @@ def test_pointers_that_are_no_device_memory(call):
 @pytest.mark.parametrize("kw,rc", [
     (dict(x=None), ARG), (dict(out=None), ARG), (dict(pos=None), ARG), (dict(plan=None), ARG), (dict(dtype=3), DTYPE),
     (dict(reserved=1), ARG), (dict(transpose=2), ARG), (dict(n_tokens=0), SIZE), (dict(n_heads=0), SIZE), (dict(head_dim=0), SIZE),
-    (dict(head_dim=257), SIZE), (dict(head_dim=64), SIZE), (dict(x=P + 2), ALIGN), (dict(out=P + 1, dtype=1), ALIGN),
+    (dict(head_dim=257), SIZE), (dict(head_dim=64), SIZE), (dict(n_heads=65536), SIZE), (dict(x_token_stride=1 << 32), SIZE), (dict(x=P + 2), ALIGN), (dict(out=P + 1, dtype=1), ALIGN),
     (dict(pos=P + 2), ALIGN), (dict(out=P, out_head_stride=256), ALIAS)])
 def test_rope_refuses(kw, rc):
     assert rope(**kw) == rc
@@ -93,7 +93,8 @@ def test_rope_refuses(kw, rc):
     (dict(kv=cache(v=P + 2)), ALIGN), (dict(kv=cache(head_dim=512, row_stride=512)), SIZE), (dict(dtype=5), DTYPE),
     (dict(n_tokens=0), SIZE), (dict(n_seqs=0), SIZE), (dict(pages_per_seq=0), SIZE), (dict(seq=None), SIZE),
     (dict(q=P, q_out=None), ARG), (dict(q=P, q_out=2 * P, n_heads=0), SIZE), (dict(q=P, q_out=P, q_out_head_stride=64), ALIAS),
-    (dict(kv=cache(head_dim=64)), SIZE), (dict(row=P + 1), ALIGN), (dict(reserved=9), ARG)])
+    (dict(kv=cache(head_dim=64)), SIZE), (dict(row=P + 1), ALIGN), (dict(reserved=9), ARG),
+    (dict(kv=cache(head_stride=1 << 32)), SIZE), (dict(v_token_stride=1 << 40), SIZE), (dict(q=P, q_out=2 * P, n_heads=70000), SIZE)])
 def test_append_refuses(kw, rc):
     assert append(**kw) == rc
 
@@ -105,7 +106,8 @@ def test_append_refuses(kw, rc):
     (dict(n_tokens=0), SIZE), (dict(n_seqs=0), SIZE), (dict(max_q=0), SIZE), (dict(n_tokens=3), SIZE), (dict(max_q=2), SIZE),
     (dict(max_len=65), SIZE), (dict(max_prefix=1 << 30), SIZE), (dict(q=P + 4), ALIGN), (dict(out_head_stride=130), ALIGN),
     (dict(q_start=P + 2, max_q=2), ALIGN), (dict(out=P), ALIAS), (dict(work=None), ARG), (dict(work_bytes=16), SIZE),
-    (dict(work=P + 8), ALIGN), (dict(scale=math.nan), ARG), (dict(scale=math.inf), ARG), (dict(n_tokens=1 << 29, n_seqs=1 << 29), SIZE)])
+    (dict(work=P + 8), ALIGN), (dict(scale=math.nan), ARG), (dict(scale=math.inf), ARG), (dict(n_tokens=1 << 29, n_seqs=1 << 29), SIZE),
+    (dict(n_tokens=70000, n_seqs=70000), SIZE)])
 def test_attn_refuses(kw, rc):
     assert attn(**kw) == rc
 
