@@ -71,6 +71,23 @@ __global__ void __launch_bounds__(FEW_THREADS, MB == 1 ? 3 : 2) attn_few_kernel(
     const int64_t v_from_k = (const uint8_t*)a.v - (const uint8_t*)a.k;
     const uint32_t lr = lane / CH, lc = lane % CH;
     auto row_of = [&](uint32_t i) { return w.r0 + (warp + 4 * i) * KT; };
+    // Places in a tile (tile_off) as a lane's part, formed once, and a step's: a step's chunk and row
+    // bits are not the lane's, so they are exchanged by one XOR on the lane's part.
+    constexpr uint32_t RB = HD * sizeof(T);
+    constexpr bool XOR = RB >= 128;
+    const uint32_t at_k = tile_off<T, HD>(lane & 7, lane >> 3), at_v = tile_off<T, HD>(lane & 15, lane >> 4), at_c = tile_off<T, HD>(lr, lc);
+    auto k_at = [&](uint32_t n, uint32_t j) {  // row n * 8 + lane % 8, chunk 4 j + lane / 8
+        if constexpr (XOR) return (at_k ^ ((4 * j & 7) << 4)) + (4 * j >> 3) * 128 + n * 8 * RB;
+        else return tile_off<T, HD>(n * 8 + (lane & 7), 4 * j + (lane >> 3));
+    };
+    auto v_at = [&](uint32_t b, uint32_t j) {  // row b * 16 + lane % 16, chunk 2 j + lane / 16
+        if constexpr (XOR) return (at_v ^ ((2 * j & 7) << 4)) + (2 * j >> 3) * 128 + b * 16 * RB;
+        else return tile_off<T, HD>(b * 16 + (lane & 15), 2 * j + (lane >> 4));
+    };
+    auto c_at = [&](uint32_t p) {  // row p RP + lane / CH, chunk lane % CH
+        if constexpr (XOR) return (at_c ^ ((p * RP & 7) << 4)) + p * RP * RB;
+        else return tile_off<T, HD>(p * RP + lr, lc);
+    };
 
     // The page of a chunk's rows is loaded one chunk before the copies that use it.
     uint32_t page = 0;
@@ -92,8 +109,8 @@ __global__ void __launch_bounds__(FEW_THREADS, MB == 1 ? 3 : 2) attn_few_kernel(
                 const uint64_t by = o == ~0ull ? 0ull : RP * a.row_stride;
 #pragma unroll
                 for (int p = 0; p < KT / RP; ++p) {
-                    cp_async16(st + tile_off<T, HD>(p * RP + lr, lc), src, n);
-                    cp_async16(st + S::TILE + vt_off<T, HD>(p * RP + lr, lc), (const uint8_t*)src + v_from_k, n);
+                    cp_async16(st + c_at(p), src, n);
+                    cp_async16(st + S::TILE + (F32 ? vt_off<T, HD>(p * RP + lr, lc) : c_at(p)), (const uint8_t*)src + v_from_k, n);
                     src += by;
                 }
             } else {
@@ -135,7 +152,7 @@ __global__ void __launch_bounds__(FEW_THREADS, MB == 1 ? 3 : 2) attn_few_kernel(
     uint32_t qf[QREG ? HD / 16 : 1][4];
     if constexpr (QREG) {
 #pragma unroll
-        for (int j = 0; j < HD / 16; ++j) ldsm4(s_q + tile_off<T, HD>(lane & 15, 2 * j + (lane >> 4)), qf[j]);
+        for (int j = 0; j < HD / 16; ++j) ldsm4(s_q + v_at(0, j), qf[j]);
     }
 
     int32_t see[MB][2];  // vectors b * 16 + g and + 8: rows that they see
@@ -182,12 +199,12 @@ __global__ void __launch_bounds__(FEW_THREADS, MB == 1 ? 3 : 2) attn_few_kernel(
                     for (int b = 0; b < MB; ++b)
 #pragma unroll
                         for (int e = 0; e < 2; ++e)
-                            ldsm4(s_q + tile_off<T, HD>(b * 16 + (lane & 15), 2 * (2 * j + e) + (lane >> 4)), q[b][e]);
+                            ldsm4(s_q + v_at(b, 2 * j + e), q[b][e]);
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     uint32_t k[4];
-                    ldsm4(sk + tile_off<T, HD>(n * 8 + (lane & 7), 4 * j + (lane >> 3)), k);
+                    ldsm4(sk + k_at(n, j), k);
                     if constexpr (QREG) {
                         mma16(s[0][n], qf[2 * j], k[0], k[1], T());
                         mma16(s2[0][n], qf[2 * j + 1], k[2], k[3], T());
@@ -213,7 +230,7 @@ __global__ void __launch_bounds__(FEW_THREADS, MB == 1 ? 3 : 2) attn_few_kernel(
 #pragma unroll 4
             for (int j = 0; j < HD / 16; ++j) {  // two k8 steps
                 uint32_t k[4], kh[4], kl[4];
-                ldsm4(sk + tile_off<T, HD>(lane & 7, 4 * j + (lane >> 3)), k);
+                ldsm4(sk + k_at(0, j), k);
 #pragma unroll
                 for (int i = 0; i < 4; ++i) split_tf32(k[i], kh[i], kl[i]);
 #pragma unroll
@@ -222,7 +239,7 @@ __global__ void __launch_bounds__(FEW_THREADS, MB == 1 ? 3 : 2) attn_few_kernel(
 #pragma unroll
                     for (int e = 0; e < 2; ++e) {
                         uint32_t q[4], qh[4], ql[4];
-                        ldsm4(s_q + tile_off<T, HD>(b * 16 + (lane & 15), 2 * (2 * j + e) + (lane >> 4)), q);
+                        ldsm4(s_q + v_at(b, 2 * j + e), q);
 #pragma unroll
                         for (int i = 0; i < 4; ++i) split_tf32(q[i], qh[i], ql[i]);
                         mma8(hh, qh, kh[2 * e], kh[2 * e + 1]);
@@ -314,7 +331,7 @@ __global__ void __launch_bounds__(FEW_THREADS, MB == 1 ? 3 : 2) attn_few_kernel(
 #pragma unroll
             for (int n = 0; n < ND / 2; ++n) {
                 uint32_t v[4];
-                ldsm4_t(sv + tile_off<T, HD>(lane & 15, 2 * n + (lane >> 4)), v);
+                ldsm4_t(sv + v_at(0, n), v);
 #pragma unroll
                 for (int b = 0; b < MB; ++b) {
                     const uint32_t pa[4] = {pf[b][0][0], pf[b][0][1], pf[b][1][0], pf[b][1][1]};

@@ -223,6 +223,17 @@ def test_append(dtype, cache, tokens, seqs, heads, kv_heads, dim, rot, page_rows
     assert Q.lib.q_b200_device_status() == 0
 
 
+def test_append_turns_queries_in_place():
+    g, p = gen(9), make_plan(64, "interleaved")
+    pool, keys, values = new_pool(g, 4, 1, 2, 8, 64, "bf16")
+    qkv = normal(g, 4, 8, 64, dtype="bf16")
+    q, was, row = qkv[:, :4], qkv[:, :4].clone(), ints([7, -1, 3, 0])
+    do_append(keys, values, "bf16", qkv[:, 4:6], qkv[:, 6:], ints([[0], [1], [2], [3]]), None, row, None, p, "bf16", q, q)
+    want, room = turn64(was, row, p)
+    within(q[[0, 2, 3]], want[[0, 2, 3]], room[[0, 2, 3]], "bf16")
+    assert torch.equal(q[1], was[1])
+
+
 def test_append_without_sequence_and_position_lists():
     g, p = gen(1), make_plan(32)
     pool, keys, values = new_pool(g, 6, 1, 2, 4, 32, "f32")
@@ -348,6 +359,10 @@ class Batch:
     (4, 4, 128, 7, 0, [50, 3], [50, 5]),                          # a prompt from its first token; early tokens see nothing
     (8, 1, 128, 64, 5000, [1, 2, 3], [1, 1, 1]),
     (64, 8, 128, 64, 2048, [100] * 17, [1] * 17),
+    (8, 2, 128, 16, 100, [50], [1]),                              # one sequence: its prefix and own rows in one pass,
+    (8, 2, 64, 32, 96, [700], [3]),                               # the own rows in step with the pages and not
+    (48, 1, 64, 16, 33, [20], [1]),
+    (40, 1, 128, 32, 600, [40, 8], [2, 1]),
 ])
 def test_attn(dtype, heads, kv_heads, dim, page_rows, prefix, rows, new):
     b = Batch(len(rows) + dim, dtype, heads, kv_heads, dim, page_rows, prefix, rows, new, pad=3 if max(new) > 1 else 0)
