@@ -306,11 +306,13 @@ struct AttnPlan {
     uint32_t parts = 0;   // partial results in the workspace
 };
 
+uint32_t ctas_per_sm(const AttnPass& p) { return p.kern == ATTN_TC ? 1 : p.kern == ATTN_FEW && p.mb == 1 ? 3 : 2; }
+
 // A pass of attn_few_kernel (up to 32 vectors) or attn_rows_kernel: the rows
-// are cut until as many CTAs as run at once have work, each with at least two
-// tiles.  Up to 8 cuts of the own rows are one cluster's and leave nothing
+// are cut until as many CTAs as `sms` run at once have work, each with at least
+// two tiles.  Up to 8 cuts of the own rows are one cluster's and leave nothing
 // in the workspace.
-AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t rows, uint32_t step, bool own) {
+AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t rows, uint32_t step, bool own, uint32_t sms) {
     AttnPass p;
     p.kern = vecs <= 32 ? ATTN_FEW : ATTN_ROWS;
     p.mb = vecs <= 16 ? 1 : 2;
@@ -318,8 +320,7 @@ AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t row
     p.items = p.tiles * seqs;
     const uint64_t ctas = (uint64_t)p.items * kv_heads;
     const uint32_t most = std::max(1u, cdiv(rows, 2 * step));
-    const uint32_t per_sm = p.kern == ATTN_FEW && p.mb == 1 ? 3 : 2;
-    p.splits = (uint32_t)std::min<uint64_t>({std::max<uint64_t>(1, per_sm * 148 / ctas), most, 64});
+    p.splits = (uint32_t)std::min<uint64_t>({std::max<uint64_t>(1, ctas_per_sm(p) * sms / ctas), most, 64});
     if (p.kern == ATTN_FEW && own && p.splits > 1) {
         p.cluster = p.splits <= 8 || rows <= 8 * 4 * step;
         if (p.cluster) p.splits = std::min(p.splits, 8u);
@@ -329,16 +330,16 @@ AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t row
 }
 
 // The prefix on tcgen05: a tile of 128 vectors (two where there are more)
-// per CTA, one CTA per SM, the rows cut so that all SMs have one, but each
+// per CTA, one CTA per SM, the rows cut so that `sms` SMs have one, but each
 // four tiles: a shorter part costs as much to begin, and to add later, as to
-// compute, and the own rows' pass takes the SMs that are left.
-AttnPass plan_tc(uint32_t vecs, uint32_t kv_heads, uint32_t rows) {
+// compute.
+AttnPass plan_tc(uint32_t vecs, uint32_t kv_heads, uint32_t rows, uint32_t sms) {
     AttnPass p;
     p.kern = ATTN_TC;
     p.alternate = vecs <= 128;
     p.tiles = p.items = cdiv(vecs, p.alternate ? 128 : 256);
     const uint32_t ctas = p.items * kv_heads;
-    p.splits = std::min({std::max(1u, 148 / ctas), std::max(1u, rows / (4 * TC_ROWS)), ATTN_MAX_PARTS});
+    p.splits = std::min({std::max(1u, sms / ctas), std::max(1u, rows / (4 * TC_ROWS)), ATTN_MAX_PARTS});
     p.parts = p.splits;
     return p;
 }
@@ -364,13 +365,42 @@ AttnPlan plan_attn(const q_b200_attn_args* r) {
     // A pass of its own reads the prefix once instead of once per sequence
     // (from L2 after the first); it costs a launch and its parts.
     p.shared = prefix >= 2 * step && r->n_seqs > 1;
-    if (p.shared) {
+    const uint32_t heads = r->kv.n_kv_heads, own_rows = std::max(1u, r->max_len + (p.shared ? 0 : prefix));
+    auto own = [&](uint32_t sms) { return plan_pass(r->max_q * G, r->n_seqs, heads, own_rows, step, true, sms); };
+    if (!p.shared) {
+        p.own = own(148);
+    } else {
         const uint32_t vecs = r->n_tokens * G;
-        p.pre = r->kv.dtype != Q_B200_F32 && r->kv.head_dim >= 64 && r->scale > 0.0f && vecs > 32
-                    ? plan_tc(vecs, r->kv.n_kv_heads, prefix)
-                    : plan_pass(vecs, 1, r->kv.n_kv_heads, prefix, step, false);
+        const bool tc = r->kv.dtype != Q_B200_F32 && r->kv.head_dim >= 64 && r->scale > 0.0f && vecs > 32;
+        auto pre = [&](uint32_t sms) { return tc ? plan_tc(vecs, heads, prefix, sms) : plan_pass(vecs, 1, heads, prefix, step, false, sms); };
+        // The two passes run side by side where the own rows' CTAs all find
+        // room beside the prefix's (they wait for them before they add the
+        // parts): the SMs are shared by what each pass takes.  Where they do
+        // not, one pass follows the other and each has the whole GPU.  SM
+        // microseconds as measured: 3 to 5 for a CTA's begin and end; 0.9 for a
+        // tile of 128 rows on tcgen05, 1.9 for two streams' vectors; 0.95 to 1.6
+        // for a chunk (16 rows, 8 of fp32) of a warp.
+        const AttnPass one = own(0);
+        const uint64_t n_own = (uint64_t)one.items * heads;
+        const uint32_t need = cdiv(n_own, ctas_per_sm(one));
+        if (need <= 148 * 6 / 10) {
+            const AttnPass pt = pre(0);
+            const double chunk = 4.0 * ctas_per_sm(one) * (step / 4) / (step == 32 ? 1.6 : 0.95);
+            const double t_own = n_own * (0.6 * own_rows / chunk + 5.0 / ctas_per_sm(one));
+            const double n_pre = (double)pt.items * heads;
+            const double t_pre = tc ? n_pre * (prefix / 128.0 * (pt.alternate ? 0.9 : 1.9) + 4.0 * 148 / (2 * n_pre))
+                                    : n_pre * (prefix / (4.0 * ctas_per_sm(pt) * (step / 4) / (step == 32 ? 1.6 : 0.95)) + 5.0);
+            // whole sets of the own rows' CTAs, so that none of them has to wait for the prefix's SMs
+            uint32_t sets = std::max(1u, (uint32_t)std::lround(148 * t_own / (t_own + t_pre) / need));
+            while (sets > 1 && sets * need > 148 * 7 / 10) --sets;
+            p.pre = pre(148 - std::min(sets * need, 144u));
+            const uint32_t used = cdiv((uint64_t)p.pre.items * p.pre.splits * heads, ctas_per_sm(p.pre));
+            p.own = own(std::max(need, used < 148 ? 148 - used : 0u));
+        } else {
+            p.pre = pre(148);
+            p.own = own(148);
+        }
     }
-    p.own = plan_pass(r->max_q * G, r->n_seqs, r->kv.n_kv_heads, std::max(1u, r->max_len + (p.shared ? 0 : prefix)), step, true);
     p.parts = (p.shared ? p.pre.parts : 0) + p.own.parts;
     return p;
 }
