@@ -218,9 +218,9 @@ q_error_code q_b200_gemv_f32(const float* d_w, uint32_t M, uint32_t K,
  * Every pointer in the argument records is a device pointer of the current
  * device unless it is a plan (host); a pointer that is not is refused with
  * Q_ERR_INVALID_ARG.  Strides count elements and, but for page_stride, are
- * below 2^32.  Calls are asynchronous on `stream`, allocate nothing, keep no state between calls and may be
- * captured in a CUDA graph; calls on different streams may overlap as long
- * as they share no output or workspace.  What the device alone can see to be
+ * below 2^32.  Calls are asynchronous on `stream`, allocate nothing, keep no
+ * state between calls and may be captured in a CUDA graph; calls on different
+ * streams may overlap as long as they share no output or workspace.  What the device alone can see to be
  * wrong (a page, sequence or token out of range, a length above its bound)
  * is skipped and leaves code 4 in the status word (q_b200_device_status):
  * nothing out of range is touched, results that hang on it are unspecified. */
@@ -327,7 +327,10 @@ q_error_code q_b200_kv_append(const q_b200_append_args* args, void* stream);
  * h / (n_heads / n_kv_heads).  A token that sees no row gives zeros.  q and
  * out have the cache's dtype; scores, softmax and sums are fp32.  Tokens of
  * no sequence (from q_start[n_seqs] on) are left as they are in out.
- * head_dim 32, 64 or 128. */
+ * head_dim 32, 64 or 128; addresses and strides of q, out and the cache in
+ * multiples of 16 bytes.  n_seqs times the tiles of a sequence's max_q *
+ * n_heads / n_kv_heads query vectors (16 up to 16, 32 up to 32, else 64) is
+ * below 2^16. */
 typedef struct {
     q_b200_paged_kv kv;
     const void* q; /* [n_tokens][n_heads][head_dim] */
@@ -354,7 +357,7 @@ q_error_code q_b200_attn_prefix(const q_b200_attn_args* args, void* stream);
  * while uniform[b][i] * q_i(x) < p_i(x); at the first that is not, the next
  * token is drawn from max(p_i - q_i, 0), and after the last accepted draft
  * from the target's own row, by the smallest index whose running sum
- * exceeds uniform[b][n_draft] times the whole (sums in 64 bits).  p and q
+ * exceeds uniform[b][n_draft] times the whole (sums to 2^-48).  p and q
  * are rows of probabilities (PROBS; they need not sum to one) or the softmax
  * of logits / temperature (LOGITS; below 1e-6 the test is whether the draft
  * is the first maximum of the target, and q is not used).  draft NULL: q is

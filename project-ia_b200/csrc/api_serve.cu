@@ -316,7 +316,7 @@ AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t row
     AttnPass p;
     p.kern = vecs <= 32 ? ATTN_FEW : ATTN_ROWS;
     p.mb = vecs <= 16 ? 1 : 2;
-    p.tiles = cdiv(vecs, p.kern == ATTN_FEW ? 16 * p.mb : 64);
+    p.tiles = cdiv(vecs, p.kern == ATTN_FEW ? 16 * p.mb : ATTN_VECS);
     p.items = p.tiles * seqs;
     const uint64_t ctas = (uint64_t)p.items * kv_heads;
     const uint32_t most = std::max(1u, cdiv(rows, 2 * step));
@@ -451,9 +451,9 @@ cudaError_t launch_pass(PrefixArgs a, const AttnPass& p, uint32_t kv_heads, cuda
     }
     if (p.kern == ATTN_FEW)
         return p.mb == 1 ? launch_few<T, HD, 1>(a, p, kv_heads, st) : launch_few<T, HD, 2>(a, p, kv_heads, st);
-    const size_t smem = attn_rows_smem<T, HD, 4>();
-    if (cudaError_t e = ensure_smem_attr((const void*)attn_rows_kernel<T, HD, 4>, (int)smem)) return e;
-    return launch_ex(attn_rows_kernel<T, HD, 4>, dim3(p.splits, p.items, kv_heads), dim3(ATTN_THREADS), smem, st, true, a);
+    const size_t smem = attn_rows_smem<T, HD>();
+    if (cudaError_t e = ensure_smem_attr((const void*)attn_rows_kernel<T, HD>, (int)smem)) return e;
+    return launch_ex(attn_rows_kernel<T, HD>, dim3(p.splits, p.items, kv_heads), dim3(ATTN_THREADS), smem, st, true, a);
 }
 
 // The prefix's pass, then the own rows' beside its tail (programmatic

@@ -9,20 +9,22 @@
 // leaves (m, l, o) in fp32 in the workspace and attn_join_kernel adds them
 // in part order (the same result on every run).
 //
-// attn_rows_kernel: one CTA takes 16 WM query vectors (tokens x the G heads
-// that share a KV head) and a range of rows in tiles that a ring of cp.async
-// stages brings in; a row's page is looked up by the thread that copies it,
-// so pages may have any size and end anywhere in a tile.  Its 4 warps are WM
-// groups of 16 vectors x 4/WM groups of the tile's rows; with WM = 1 (a
-// decoded token's few heads) every warp has rows of its own and the warps
-// are joined at the end.  Products are mma.sync: m16n8k16 for fp16 and
-// bf16; for fp32 m16n8k8 tf32 on halves v = hi + lo of 11 bits each, hi.hi +
-// hi.lo + lo.hi (the dropped lo.lo is 2^-22 relative), with the hi.hi sums
-// folded into fp32 every few products because the tensor core truncates
-// when it accumulates.  P is rounded to the cache's type for P.V (fp16,
-// bf16), as the products' operand type asks; l sums what is multiplied.
+// This file holds what the passes share, and attn_rows_kernel, the pass for
+// more than 32 vectors of a KV head where tcgen05 is not used (fp32 caches,
+// head_dim 32, a scale that is not positive, a prompt's own rows).  One CTA
+// takes 64 query vectors (tokens x the G heads that share a KV head), 16 for
+// each of four warps, and a range of rows in tiles that a fifth warp brings
+// into a ring with cp.async; a row's page is looked up by one lane, so pages
+// may have any size and end anywhere in a tile.  Products are mma.sync:
+// m16n8k16 for fp16 and bf16; for fp32 m16n8k8 tf32 on halves v = hi + lo of
+// 11 bits each, hi.hi + hi.lo + lo.hi (the dropped lo.lo is 2^-22 relative),
+// with the hi.hi sums folded into fp32 every few products because the tensor
+// core truncates when it accumulates (errors against 64 bits come out at
+// 4e-7, half of an fp32 product's).  P is rounded to the cache's type for P.V
+// (fp16, bf16), as the products' operand type asks; l sums what is
+// multiplied.
 //
-// Bound: bytes of K and V for few query vectors per row.
+// Bound: the products (64 vectors a row of K and V).
 #pragma once
 
 #include <type_traits>
@@ -80,12 +82,13 @@ struct AttnTraits<float> {
 static constexpr uint32_t ATTN_CONSUMERS = 128;  // four warps that multiply, one that copies
 static constexpr uint32_t ATTN_THREADS = 160;
 static constexpr uint32_t ATTN_MAX_PARTS = 128;
+static constexpr uint32_t ATTN_VECS = 64;  // of a CTA of attn_rows_kernel
 
-template <typename T, int HD, int WM>
+template <typename T, int HD>
 constexpr size_t attn_rows_smem() {
-    constexpr size_t ring = (size_t)AttnTraits<T>::STAGES * AttnTraits<T>::KT * HD * sizeof(T) * 2 + 16 * WM * HD * sizeof(T);
-    constexpr size_t join = 64 * (HD + 4 + 3) * 4 + 16 * WM * 2 * 4;
-    return ring > join ? ring : join;
+    constexpr size_t ring = (size_t)AttnTraits<T>::STAGES * AttnTraits<T>::KT * HD * sizeof(T) * 2 + ATTN_VECS * HD * sizeof(T);
+    constexpr size_t out = ATTN_VECS * (HD + 4 + 2) * 4;
+    return ring > out ? ring : out;
 }
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
@@ -314,12 +317,11 @@ struct PartSum {
     }
 };
 
-template <typename T, int HD, int WM>
+template <typename T, int HD>
 __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_constant__ PrefixArgs a) {
     constexpr bool F32 = sizeof(T) == 4;
     constexpr int KT = AttnTraits<T>::KT, ST = AttnTraits<T>::STAGES;
-    constexpr int WN = 4 / WM, KW = KT / WN;       // groups of rows, rows of one warp in a tile
-    constexpr int NT = KW / 8, ND = HD / 8;        // score and output tiles of 8 columns
+    constexpr int NT = KT / 8, ND = HD / 8;        // score and output tiles of 8 columns
     constexpr int CH = HD * (int)sizeof(T) / 16;   // 16-byte chunks of a row
     constexpr int RP = 32 / CH;                    // rows that one copy instruction of the warp brings
     constexpr uint32_t TILE = KT * HD * sizeof(T);
@@ -328,13 +330,12 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
     __shared__ bool s_bad[KT];
     const uint32_t s_kv = smem_u32(smem), s_q = s_kv + ST * 2 * TILE;
     const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, t = lane & 3;
-    const uint32_t wm = warp % WM, wn = warp / WM;
     const uint32_t split = blockIdx.x, head = blockIdx.z;
 
     if (a.first) pdl_wait();
     pdl_trigger();  // the pass after this one may start beside it
     AttnItem w;
-    if (!attn_item(a, blockIdx.y, split, 16 * WM, KT, w)) {
+    if (!attn_item(a, blockIdx.y, split, ATTN_VECS, KT, w)) {
         pdl_wait();
         return;
     }
@@ -379,7 +380,7 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
     }
 
     // ---- consumers -------------------------------------------------------------------------------
-    for (uint32_t e = tid; e < 16 * WM * CH; e += ATTN_CONSUMERS) {
+    for (uint32_t e = tid; e < ATTN_VECS * CH; e += ATTN_CONSUMERS) {
         const uint32_t r = e / CH, c = e % CH;
         uint4 v = make_uint4(0, 0, 0, 0);
         if (r < w.n_vec) {
@@ -394,14 +395,14 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
     if constexpr (!F32) {
 #pragma unroll
         for (int j = 0; j < HD / 16; ++j)
-            ldsm4(s_q + tile_off<T, HD>(wm * 16 + (lane & 15), 2 * j + (lane >> 4)), qf[j]);
+            ldsm4(s_q + tile_off<T, HD>(warp * 16 + (lane & 15), 2 * j + (lane >> 4)), qf[j]);
     }
 
     // vectors g and g + 8 of this warp's 16: rows they see, running maximum and sum
     int32_t see[2];
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-        const uint32_t v = w.vec0 + wm * 16 + g + 8 * h;
+        const uint32_t v = w.vec0 + warp * 16 + g + 8 * h;
         see[h] = w.see0 + (int32_t)fast_div(v, a.by_group);
         // tokens before the first own row see the prefix alone
         if (!a.shared) see[h] = max(see[h], (int32_t)w.n_prefix);
@@ -428,7 +429,7 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
 #pragma unroll
                 for (int j = 0; j < HD / 32; ++j) {
                     uint32_t b[4];
-                    ldsm4(sk + tile_off<T, HD>(wn * KW + n * 8 + (lane & 7), 4 * j + (lane >> 3)), b);
+                    ldsm4(sk + tile_off<T, HD>(n * 8 + (lane & 7), 4 * j + (lane >> 3)), b);
                     mma16(s[n], qf[2 * j], b[0], b[1], T());
                     mma16(s[n], qf[2 * j + 1], b[2], b[3], T());
                 }
@@ -442,14 +443,14 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
 #pragma unroll
                 for (int e = 0; e < 2; ++e) {
                     uint32_t q[4];
-                    ldsm4(s_q + tile_off<T, HD>(wm * 16 + (lane & 15), 2 * (2 * j + e) + (lane >> 4)), q);
+                    ldsm4(s_q + tile_off<T, HD>(warp * 16 + (lane & 15), 2 * (2 * j + e) + (lane >> 4)), q);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) split_tf32(q[i], qh[e][i], ql[e][i]);
                 }
 #pragma unroll
                 for (int n = 0; n < NT; ++n) {
                     uint32_t b[4], bh[4], bl[4];
-                    ldsm4(sk + tile_off<T, HD>(wn * KW + n * 8 + (lane & 7), 4 * j + (lane >> 3)), b);
+                    ldsm4(sk + tile_off<T, HD>(n * 8 + (lane & 7), 4 * j + (lane >> 3)), b);
 #pragma unroll
                     for (int i = 0; i < 4; ++i) split_tf32(b[i], bh[i], bl[i]);
                     float hh[4] = {0.0f, 0.0f, 0.0f, 0.0f};
@@ -478,7 +479,7 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
             for (int i = 0; i < 4; ++i) {
                 float y = s[n][i] * a.c;
                 if (edge) {
-                    const uint32_t row = first + wn * KW + n * 8 + 2 * t + (i & 1);
+                    const uint32_t row = first + n * 8 + 2 * t + (i & 1);
                     if (row >= w.r1 || (int32_t)row >= see[i >> 1]) y = -INFINITY;
                 }
                 s[n][i] = y;
@@ -550,7 +551,7 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
 #pragma unroll
                 for (int n = 0; n < ND / 2; ++n) {
                     uint32_t b[4];
-                    ldsm4_t(sv + tile_off<T, HD>(wn * KW + j * 16 + (lane & 15), 2 * n + (lane >> 4)), b);
+                    ldsm4_t(sv + tile_off<T, HD>(j * 16 + (lane & 15), 2 * n + (lane >> 4)), b);
                     mma16(o[2 * n], pa, b[0], b[1], T());
                     mma16(o[2 * n + 1], pa, b[2], b[3], T());
                 }
@@ -570,7 +571,7 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
                 float hh[4] = {0.0f, 0.0f, 0.0f, 0.0f}, ll[4] = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    const uint32_t r = wn * KW + j * 8 + 2 * t, c = 2 * n + (g >> 2);
+                    const uint32_t r = j * 8 + 2 * t, c = 2 * n + (g >> 2);
                     uint32_t b0, b1, h0, l0, h1, l1;
                     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(b0) : "r"(sv + v32_off<HD>(r, c) + (g & 3) * 4));
                     asm volatile("ld.shared.b32 %0, [%1];" : "=r"(b1) : "r"(sv + v32_off<HD>(r + 1, c) + (g & 3) * 4));
@@ -587,7 +588,7 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
         __syncwarp();
         if (lane == 0) mbar_arrive(&empty[tile % ST]);
         if (bad) {
-            for (uint32_t r = max(hid0 - first, wn * KW); r < min(hid1 - first, (wn + 1) * KW); ++r) {
+            for (uint32_t r = hid0 - first; r < hid1 - first; ++r) {
                 uint64_t off;
                 if (!s_bad[r] || !attn_row(a, w, head, first + r, off)) continue;
                 float p[2] = {0.0f, 0.0f};  // of vectors g and g + 8, held by the quad's lane that has column r
@@ -595,7 +596,7 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
                 for (int n = 0; n < NT; ++n)
 #pragma unroll
                     for (int i = 0; i < 4; ++i)
-                        if (n == (int)((r - wn * KW) >> 3) && (uint32_t)(i & 1) == (r & 1)) p[i >> 1] = s[n][i];
+                        if (n == (int)(r >> 3) && (uint32_t)(i & 1) == (r & 1)) p[i >> 1] = s[n][i];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     p[h] = __shfl_sync(0xffffffffu, p[h], (lane & ~3u) | ((r >> 1) & 3));
@@ -615,38 +616,22 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
     }
     consumers_sync();
 
-    // ---- join the groups of rows: each warp leaves its (m, l, o), then all are added in order ------
-    constexpr int RV = 16 * WM, OP = HD + 4;
-    float* s_o = reinterpret_cast<float*>(smem);     // [WN][RV][OP]
-    float* s_ml = s_o + WN * RV * OP;                // [WN][RV][2]
-    float* s_w = s_ml + WN * RV * 2;                 // [RV][WN]: weight of each warp's share
-    float* s_res = s_w + WN * RV;                    // [RV][2]: joined (m, l)
-    const uint32_t v0 = wm * 16 + g;
+    // ---- the outputs through shared memory, for whole rows to a thread group -----------------------
+    constexpr int OP = HD + 4;
+    float* s_o = reinterpret_cast<float*>(smem);  // [64][OP]
+    float* s_res = s_o + ATTN_VECS * OP;          // [64][2]: (m, l)
+    const uint32_t v0 = warp * 16 + g;
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
         if (t == 0) {
-            s_ml[(wn * RV + v0 + 8 * h) * 2] = m[h];
-            s_ml[(wn * RV + v0 + 8 * h) * 2 + 1] = l[h];
+            s_res[(v0 + 8 * h) * 2] = m[h];
+            s_res[(v0 + 8 * h) * 2 + 1] = l[h];
         }
         if (v0 + 8 * h < w.n_vec) {
 #pragma unroll
             for (int n = 0; n < ND; ++n)
-                *reinterpret_cast<float2*>(s_o + (wn * RV + v0 + 8 * h) * OP + n * 8 + 2 * t) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
+                *reinterpret_cast<float2*>(s_o + (v0 + 8 * h) * OP + n * 8 + 2 * t) = make_float2(o[n][2 * h], o[n][2 * h + 1]);
         }
-    }
-    consumers_sync();
-    if (tid < RV) {
-        float M = -INFINITY, L = 0.0f;
-#pragma unroll
-        for (int k = 0; k < WN; ++k) M = fmaxf(M, s_ml[(k * RV + tid) * 2]);
-#pragma unroll
-        for (int k = 0; k < WN; ++k) {
-            const float mk = s_ml[(k * RV + tid) * 2], f = mk == -INFINITY ? 1.0f : exp2f(mk - M);
-            s_w[tid * WN + k] = f;  // 1 where there is nothing, or a NaN, to add
-            L += s_ml[(k * RV + tid) * 2 + 1] * f;
-        }
-        s_res[tid * 2] = M;
-        s_res[tid * 2 + 1] = L;
     }
     consumers_sync();
     pdl_wait();  // what an earlier pass left is complete
@@ -655,16 +640,7 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
         const uint32_t r = e / (HD / 4), c = e % (HD / 4);
         const uint32_t i = fast_div(w.vec0 + r, a.by_group), h = head * a.group + (w.vec0 + r - i * a.group);
         const uint64_t tok = w.tok0 + i;
-        float4 x = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-#pragma unroll
-        for (int k = 0; k < WN; ++k) {
-            const float4 y = *reinterpret_cast<const float4*>(s_o + (k * RV + r) * OP + c * 4);
-            const float f = s_w[r * WN + k];
-            x.x = fmaf(y.x, f, x.x);
-            x.y = fmaf(y.y, f, x.y);
-            x.z = fmaf(y.z, f, x.z);
-            x.w = fmaf(y.w, f, x.w);
-        }
+        const float4 x = *reinterpret_cast<const float4*>(s_o + r * OP + c * 4);
         const float L = s_res[r * 2 + 1];
         if (a.last) {
             PartSum<HD> sum;

@@ -22,20 +22,21 @@
 // there; V is used as it lies in the cache, [row][dim], as an MN-major B
 // operand.
 //
-// What it took (512 vectors x 32768 rows x 8 KV heads, head_dim 128, 29 tiles
-// a CTA): scores of 64 rows with two buffers a stream instead of 128 with
-// one keep the streams apart from their own products, but a product of
-// 64 columns takes 53 clocks and not 32 (its operands come from shared memory
-// at 128 bytes a clock); the fence between the copies and the products cost
-// the issuing warp 500 clocks a tile.
+// Tried: scores of 64 rows with two buffers a stream, instead of 128 with one,
+// keep a stream's exponentials apart from its own products, but a product of
+// 64 columns takes 57 clocks where one of 128 takes 64 (operands come from
+// shared memory at 128 bytes a clock).  A warp that polls both streams and
+// takes whichever is ready spends 3000 clocks a tile on doing so.
 //
 // The running maximum moves only when a half tile exceeds it by 2^8: then the
 // output is rescaled in TMEM; until then exponentials may reach 256, which
 // fp16 holds, and the quotient o / l is the same.
 //
 // Bound: for up to 128 vectors the bytes of K and V; beyond, the tensor pipe
-// and, at head_dim 128 nearly as long, the exponentials (128 x 128 of them a
-// tile and stream on 16 lanes of the special function unit).
+// (4 x 128 x 128 x head_dim flops a tile and stream) with the exponentials (128
+// x 128 of them, a quarter on the multiply-add units) in its way: 512 vectors x
+// 32768 rows x 8 KV heads of 128 take 71 us, 0.97 PFLOP/s, 3450 clocks a tile
+// of which the tensor pipe works 2048, at the 1.6 GHz that the power cap leaves.
 #pragma once
 
 #include "attn_prefix.cuh"

@@ -18,8 +18,11 @@
 // are issued before the angles are formed, so that they are under way
 // meanwhile.  Neighbouring threads take neighbouring units of a head: every
 // access is coalesced.  (Angles formed by every thread for its own unit took
-// 300 instructions a unit: 70 us against 26 us of bytes for 8191 x 40 x 128
-// bf16.)
+// 300 instructions a unit: 70 us for 8191 x 40 x 128 bf16, where this takes 32.)
+//
+// Measured back to back: the 168 MB of that in 31.5 us and the 67 MB of 2048 x
+// 32 x 128 fp32 in 12.5 us, 0.81 of a plain copy's rate; one token 3.3 us, the
+// time of a launch.
 #pragma once
 
 #include <cuda_bf16.h>
