@@ -298,7 +298,7 @@ q_error_code q_b200_rope(const q_b200_rope_args* args, void* stream);
 
 /* Token t's keys (rotated by pos[t]) and values go to row row[t] of sequence
  * seq[t]'s pages; with q its queries are rotated into q_out beside them.  A
- * token with a negative row is padding: nothing of it is read or written.
+ * token with a negative row is padding: nothing of it is written.
  * Two tokens must not name the same row of the same page. */
 typedef struct {
     q_b200_paged_kv kv;

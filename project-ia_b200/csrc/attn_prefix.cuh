@@ -148,10 +148,13 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
 // v = hi + lo, each of 11 significant bits rounded to nearest (the tensor
-// core reads the upper 19 bits of an operand).
+// core reads the upper 19 bits of an operand).  The addition that rounds may
+// carry a NaN's bits over into the sign, and hi is a zero then: lo, v - hi, is
+// a NaN too and is kept from the same (and is one for infinities).
 __device__ __forceinline__ void split_tf32(uint32_t v, uint32_t& hi, uint32_t& lo) {
     hi = (v + 0x1000u) & 0xffffe000u;
-    lo = __float_as_uint(__uint_as_float(v) - __uint_as_float(hi)) + 0x1000u;
+    const float d = __uint_as_float(v) - __uint_as_float(hi);
+    lo = (uint32_t)min(__float_as_int(d), 0x7fffe000) + 0x1000u;
 }
 
 // 16-byte chunk c of row r in a tile of HD-wide rows: chunks are exchanged

@@ -110,6 +110,13 @@ __device__ __forceinline__ F2 ex2_series(F2 x) {
     return F2(__uint_as_float(__float_as_uint(p) + (__float_as_uint(s) << 23)), __uint_as_float(__float_as_uint(q) + (__float_as_uint(t) << 23)));
 }
 
+// The largest of three, NaN if one of them is.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+    float r;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+    return r;
+}
+
 // 16 and 64 consecutive columns of this warp's 32 TMEM lanes.
 __device__ __forceinline__ void tmem_ld16(uint32_t taddr, uint32_t (&r)[16]) {
     asm volatile(
@@ -239,10 +246,12 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
             float mx = -INFINITY, my = -INFINITY;
 #pragma unroll
             for (int i = 0; i < 64; i += 4) {
-                mx = fmaxf(fmaxf(mx, __uint_as_float(v[i])), __uint_as_float(v[i + 1]));
-                my = fmaxf(fmaxf(my, __uint_as_float(v[i + 2])), __uint_as_float(v[i + 3]));
+                mx = max_nan(mx, __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+                my = max_nan(my, __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
             }
-            mx = fmaxf(mx, my) * a.c;  // c > 0
+            mx = max_nan(mx, my, my) * a.c;  // c > 0
+            // a score that is no number or infinite: so is the sum, and every output (the series' clamp would hide a NaN)
+            const bool lost = !(mx < INFINITY);
             const bool move = mx > m + 8.0f;  // also from -infinity
             if (__any_sync(0xffffffffu, move)) {
                 const float f = move ? (m == -INFINITY ? 0.0f : ex2(m - mx)) : 1.0f;
@@ -288,6 +297,7 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
                 }
                 tmem_st16(ts + k * 16, p);
             }
+            if (lost) sum = F2(__int_as_float(0x7fffffff), 0.0f);
             asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory");
             tc_fence_before();
             __syncwarp();

@@ -404,6 +404,35 @@ def test_attn_newer_rows_do_not_reach_older_tokens(dtype, value, prefix):
     within(clean, want, room, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,prefix,seqs", [
+    (8, 2, 64, 200, 3),     # few vectors of a KV head: up to 16,
+    (24, 2, 128, 200, 2),   # up to 32,
+    (32, 2, 64, 300, 5),    # up to 128,
+    (64, 2, 128, 300, 9),   # and more
+    (64, 2, 32, 130, 4)])
+def test_attn_seen_rows_that_are_no_numbers(dtype, heads, kv_heads, dim, prefix, seqs):
+    # wherever in a tile the row lies and whatever bits the NaN has, all that see it get no finite number and nobody else notices
+    b = Batch(dim + seqs, dtype, heads, kv_heads, dim, 16, prefix, [20 + i for i in range(seqs)], [1] * seqs, poison=False)
+    b.q[..., 0] = b.q[..., 0].abs() + 0.5  # an infinite key's score is +inf
+    bits, tops = (torch.int32, (0x7F800000, 0x7FC00000, 0x7FFFFFFF, -1)) if dtype == "f32" else (
+        torch.int16, (0x7C00 if dtype == "f16" else 0x7F80, 0x7FC0 if dtype == "bf16" else 0x7E00, 0x7FFF, -1))
+    b.call()
+    clean = b.out.clone()
+    G = heads // kv_heads
+    for i, r in enumerate([0, 1, 2, 3, 4, 5, 6, 7, 30, 63, 64, 126, 127, 129]):
+        for x, outs in ((b.keys, slice(None)), (b.values, slice(0, 1))):
+            page = x[b.prefix_pages[r // 16].long()]  # a view
+            old = page[0, r % 16, 0].clone()
+            page[0, r % 16, :1].view(bits).fill_(tops[i % 4])
+            b.call()
+            page[0, r % 16, 0] = old
+            assert not torch.isfinite(b.out[:, :G, outs].float()).any(), (r, tops[i % 4])
+            same = b.out.clone()
+            same[:, :G, outs] = clean[:, :G, outs]
+            assert torch.equal(same, clean)
+
+
 def test_attn_scores_of_the_types_lowest_value():
     # keys that push every score far down, or all of them to the same value, leave the weights as they are in 64 bits
     b = Batch(6, "bf16", 4, 2, 64, 16, 65, [20, 3], [1, 1], poison=False)
