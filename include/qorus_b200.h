@@ -330,7 +330,10 @@ q_error_code q_b200_kv_append(const q_b200_append_args* args, void* stream);
  * head_dim 32, 64 or 128; addresses and strides of q, out and the cache in
  * multiples of 16 bytes.  n_seqs times the tiles of a sequence's max_q *
  * n_heads / n_kv_heads query vectors (16 up to 16, 32 up to 32, else 64) is
- * below 2^16. */
+ * below 2^16; behind a prefix n_tokens * n_heads / n_kv_heads is at most
+ * 65535 * 64 (256 for fp16 and bf16 of width 64 or 128 and a positive scale);
+ * n_tokens * n_heads, n_seqs * max_q * n_heads and max_len + max_prefix are
+ * below 2^30. */
 typedef struct {
     q_b200_paged_kv kv;
     const void* q; /* [n_tokens][n_heads][head_dim] */

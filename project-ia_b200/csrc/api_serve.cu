@@ -351,7 +351,8 @@ q_error_code check_attn(const q_b200_attn_args* r) {
     if (kv.head_dim != 32 && kv.head_dim != 64 && kv.head_dim != 128) return Q_ERR_INVALID_SIZE;
     if (r->n_tokens == 0 || r->n_seqs == 0 || r->n_heads == 0 || r->max_q == 0 || r->pages_per_seq == 0) return Q_ERR_INVALID_SIZE;
     if (r->n_heads % kv.n_kv_heads || kv.n_kv_heads > 65535) return Q_ERR_INVALID_SIZE;
-    if ((uint64_t)r->n_tokens * r->n_heads >= (1u << 30) || (uint64_t)r->n_seqs * r->max_q * r->n_heads >= (1u << 30))
+    const uint64_t most_q = (uint64_t)r->n_seqs * r->max_q;  // bounded before it is multiplied on: three factors can pass 2^64
+    if ((uint64_t)r->n_tokens * r->n_heads >= (1u << 30) || most_q >= (1u << 30) || most_q * r->n_heads >= (1u << 30))
         return Q_ERR_INVALID_SIZE;
     if ((uint64_t)r->max_len + r->max_prefix >= (1u << 30)) return Q_ERR_INVALID_SIZE;
     if ((uint64_t)r->pages_per_seq * kv.page_rows < r->max_len) return Q_ERR_INVALID_SIZE;
@@ -404,6 +405,9 @@ AttnPlan plan_attn(const q_b200_attn_args* r) {
     p.parts = (p.shared ? p.pre.parts : 0) + p.own.parts;
     return p;
 }
+
+// Items are a grid's second dimension.
+bool plan_fits(const AttnPlan& p) { return p.own.items <= 65535 && p.pre.items <= 65535; }
 
 size_t attn_bytes(const q_b200_attn_args* r, const AttnPlan& p) {
     return (size_t)p.parts * r->n_tokens * r->n_heads * (r->kv.head_dim * 4 + 8);
@@ -491,7 +495,8 @@ extern "C" {
 
 size_t q_b200_attn_work_bytes(const q_b200_attn_args* r) {
     if (!r || check_attn(r) != Q_OK) return 0;
-    return attn_bytes(r, plan_attn(r));
+    const AttnPlan p = plan_attn(r);
+    return plan_fits(p) ? attn_bytes(r, p) : 0;
 }
 
 q_error_code q_b200_attn_prefix(const q_b200_attn_args* r, void* stream) {
@@ -509,7 +514,7 @@ q_error_code q_b200_attn_prefix(const q_b200_attn_args* r, void* stream) {
     if (in < 16 || to < 16) return Q_ERR_MISALIGNED;
     if ((addr(r->q_start) | addr(r->pages) | addr(r->lens) | addr(r->prefix_pages) | addr(r->prefix_len)) & 3) return Q_ERR_MISALIGNED;
     const AttnPlan p = plan_attn(r);
-    if (p.own.items > 65535 || p.pre.items > 65535) return Q_ERR_INVALID_SIZE;  // a grid's second dimension
+    if (!plan_fits(p)) return Q_ERR_INVALID_SIZE;
     const size_t need = attn_bytes(r, p);
     if (need && !r->work) return Q_ERR_INVALID_ARG;
     if (need && r->work_bytes < need) return Q_ERR_INVALID_SIZE;

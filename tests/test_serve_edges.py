@@ -1,0 +1,37 @@
+"""Argument checks and plans of the serving operators at their limits, without a GPU (helpers: test_serve.py)."""
+import ctypes as C
+import math
+
+import numpy as np
+import pytest
+
+import qorus_b200 as Q
+from test_serve import ALIAS, ARG, P, SIZE, attn, attn_args, cache, plan, scale, verify
+
+
+def work_bytes(**kw):
+    return Q.lib.q_b200_attn_work_bytes(C.byref(attn_args(**kw)))
+
+
+# ---- sizes whose products pass 2^64, or the grid ---------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kw", [
+    dict(n_seqs=1 << 31, max_q=1 << 31, n_heads=4, kv=cache(n_kv_heads=4)),  # 2^64
+    dict(n_seqs=1 << 31, max_q=1 << 30, n_heads=8), dict(n_seqs=1 << 16, max_q=1 << 16, n_heads=1 << 31),
+    dict(n_seqs=0xFFFFFFFF, max_q=0xFFFFFFFF, n_heads=0xFFFFFFFE), dict(n_seqs=1, max_q=1 << 30, n_heads=2),
+    dict(n_tokens=0xFFFFFFFF, n_seqs=1, n_heads=0xFFFFFFFE)])
+def test_attn_products_of_sizes_do_not_wrap(kw):
+    kw = dict(dict(q_start=8 * P, n_tokens=2), **kw)
+    assert work_bytes(**kw) == 0
+    assert attn(**kw) == SIZE
+
+
+@pytest.mark.parametrize("kw", [
+    dict(n_tokens=70000, n_seqs=70000, n_heads=2),                              # own rows: a tile for each sequence
+    dict(n_tokens=70000, n_seqs=1000, max_q=70, n_heads=128, q_start=8 * P),    # 70 tiles for each of 1000
+    dict(n_tokens=4_194_241, n_seqs=2, max_q=8, n_heads=2, q_start=8 * P)])     # the prefix: 65536 tiles of 64 for all tokens
+def test_attn_work_bytes_is_zero_where_the_call_is_refused(kw):
+    kw = dict(kw, kv=cache(n_kv_heads=2))
+    assert work_bytes(**kw) == 0
+    assert attn(**kw) == SIZE
