@@ -163,10 +163,11 @@ __device__ __forceinline__ double warp_sum_f64(double v) {
     return v;
 }
 
-// Order-preserving key of (value, lowest index first); 0 for NaN.
+// Order-preserving key of (value, lowest index first); 0 for NaN.  Adding
+// zero makes -0 the +0 that it is equal to.
 __device__ __forceinline__ unsigned long long argmax_key64(float v, uint32_t i) {
     if (!(v == v)) return 0ull;
-    const uint32_t u = __float_as_uint(v);
+    const uint32_t u = __float_as_uint(v + 0.0f);
     const uint32_t o = (u & 0x80000000u) ? ~u : (u | 0x80000000u);
     return ((unsigned long long)o << 32) | (uint32_t)~i;
 }
