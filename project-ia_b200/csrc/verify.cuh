@@ -101,23 +101,29 @@ struct RowPart {
     }
 };
 
-// 2^(y / 1024) for -1010 < y / 1024 <= 1 to about 1e-11: y = k + r, a table
-// of 2^(j/1024) and the series of e^(r ln 2 / 1024) to the second power
+// 2^(d c / 1024) for -1010 < d c / 1024 <= 1 to about 1e-11: d c = k + r, a
+// table of 2^(j/1024) and the series of e^(r ln 2 / 1024) to the second power
 // (its argument is below 3.4e-4).  k comes out of the low word of
-// y + 1.5 * 2^52, which rounds there.
+// d c + 1.5 * 2^52, which rounds there.
 static constexpr uint32_t VER_TABLE = 1024;
-__device__ __forceinline__ double exp2_table(double y, const double* table) {
+__device__ __forceinline__ double exp2_table(double d, double c, const double* table) {
     const double big = 6755399441055744.0;
-    const double t = y + big, r = y - (t - big);
+    const double t = fma(d, c, big), r = fma(d, c, big - t);
     const int ki = __double2loint(t);
     constexpr double c1 = 0.69314718055994530942 / VER_TABLE, c2 = c1 * c1 / 2.0;
     const double p = fma(r, fma(r, c2, c1), 1.0) * table[ki & (VER_TABLE - 1)];
     return __hiloint2double(__double2hiint(p) + ((ki >> 10) << 20), __double2loint(p));
 }
-// 2^((v - m) c) for a logit v, with c and m c times 1024; exactly zero far
-// below m (v <= low), and for NaN.
-__device__ __forceinline__ double logit_weight(float v, float low, double c, double mc, const double* table) {
-    const double w = exp2_table(fma((double)fmaxf(v, low), c, -mc), table);
+// Logits up to this weigh nothing beside the maximum m: a thousand halvings
+// below it, or the fp32 number next to it where one step is more than that.
+__device__ __forceinline__ float logit_low(float m, float c) {
+    return m < INFINITY ? fminf(m - 1000.0f / c, nextafterf(m, -INFINITY)) : m;
+}
+// 2^((v - m) c / 1024) for a logit v; exactly zero far below m (v <= low), and
+// for NaN.  The difference comes first: v c and m c of great logits (a row
+// masked with the type's lowest value) would lose it.
+__device__ __forceinline__ double logit_weight(float v, float low, double c, double m, const double* table) {
+    const double w = exp2_table((double)fmaxf(v, low) - m, c, table);
     return v > low ? w : 0.0;
 }
 
@@ -408,8 +414,8 @@ __global__ void __launch_bounds__(VER_THREADS, ver_ctas(KIND)) verify_kernel(con
         }
         for (int k = 0; k < 2; ++k) {
             const T* row = k ? qrow : prow;
-            const double mc = (double)m[k] * ct;
-            const float low = m[k] - 1000.0f / a.c;
+            const double top = (double)m[k];
+            const float low = logit_low(m[k], a.c);
             double s = 0.0;
             if (row && m[k] > -INFINITY && m[k] < INFINITY)
                 for (uint32_t i0 = g0; i0 < g1; i0 += VER_VECS * 32 * E) {
@@ -420,7 +426,7 @@ __global__ void __launch_bounds__(VER_THREADS, ver_ctas(KIND)) verify_kernel(con
                         float v[E];
                         to_float(x.v[q], v);
 #pragma unroll
-                        for (int j = 0; j < E; ++j) s += logit_weight(v[j], low, ct, mc, s_table);
+                        for (int j = 0; j < E; ++j) s += logit_weight(v[j], low, ct, top, s_table);
                     }
                 }
             s = warp_sum_f64(s);
@@ -436,8 +442,8 @@ __global__ void __launch_bounds__(VER_THREADS, ver_ctas(KIND)) verify_kernel(con
         }
         __syncthreads();
     }
-    const double mp = KIND == VER_LOGITS ? (double)s_m[0] * ct : 0.0, mq = KIND == VER_LOGITS ? (double)s_m[1] * ct : 0.0;
-    const float lp = KIND == VER_LOGITS ? s_m[0] - 1000.0f / a.c : 0.0f, lq = KIND == VER_LOGITS ? s_m[1] - 1000.0f / a.c : 0.0f;
+    const double mp = KIND == VER_LOGITS ? (double)s_m[0] : 0.0, mq = KIND == VER_LOGITS ? (double)s_m[1] : 0.0;
+    const float lp = KIND == VER_LOGITS ? logit_low(s_m[0], a.c) : 0.0f, lq = KIND == VER_LOGITS ? logit_low(s_m[1], a.c) : 0.0f;
     const double zp = KIND == VER_LOGITS ? s_z[0] : 1.0, zq = KIND == VER_LOGITS ? s_z[1] : 1.0;
     // weights in fp64 of E entries from index i on; past the end and NaN: zero
     const float none = KIND == VER_LOGITS ? -INFINITY : 0.0f;
