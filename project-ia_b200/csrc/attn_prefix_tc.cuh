@@ -93,12 +93,14 @@ __device__ __forceinline__ bool elect_one() {
 }
 
 // 2^x for two numbers on the multiply-add units: x = k + f with |f| <= 1/2 (x
-// + 1.5 * 2^23 rounds there), the exponential's series to f^4 (off by 4e-5 of
-// the value, a tenth of fp16's half step), and k added to the exponent.
+// + 1.5 * 2^23 rounds there), the exponential's series to f^4 (off by 5.6e-5
+// of the value, a ninth of fp16's half step), and k added to the exponent.
+// 2^-127 and all below it come out as zero, as a score of -infinity has to;
+// between there and 2^-126 it is something up to 2^-126.
 __device__ __forceinline__ F2 ex2_series(F2 x) {
     float a, b, p, q, s, t;
     x.get(a, b);
-    x = F2(fmaxf(a, -126.0f), fmaxf(b, -126.0f));
+    x = F2(fmaxf(a, -127.0f), fmaxf(b, -127.0f));
     const F2 big(12582912.0f, 12582912.0f), r = add2(x, big);
     const F2 f = sub2(x, sub2(r, big));
     F2 e = fma2(f, F2(0.00961813f, 0.00961813f), F2(0.05550411f, 0.05550411f));

@@ -1,11 +1,62 @@
 """The serving operators at values, lengths and tables past those of test_gpu_serve.py, whose helpers and tolerances they use."""
+import math
+
 import numpy as np
 import pytest
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from test_gpu_serve import TYPES, do_verify, gen, ints, verify64  # noqa: E402
+from test_gpu_serve import TYPES, Batch, do_verify, gen, half_step, ints, verify64, within  # noqa: E402
+
+# ---- attention -------------------------------------------------------------------------------------------------------
+
+
+def weighted(b):
+    """(result, room) of one token a sequence, as Batch.want gives them, with scores of -infinity: a row of weight zero adds
+    nothing, whatever its value, and a vector without any weight gives zeros."""
+    G, outs, rooms = b.heads // b.keys.shape[1], [], []
+    flat = lambda x, p: x[p.long()].transpose(1, 2).reshape(-1, x.shape[1], b.dim).double()  # noqa: E731
+    for i, L in enumerate(b.rows):
+        k, v = (torch.cat([flat(x, b.prefix_pages)[: b.prefix], flat(x, b.pages[i])[:L]]).repeat_interleave(G, 1) for x in (b.keys, b.values))
+        q = b.q[i].double()
+        y = torch.einsum("hd,lhd->hl", q, k) / math.sqrt(b.dim)
+        p = torch.softmax(y, -1).nan_to_num(0.0)
+        v = torch.where(p.T[..., None] > 0, v, 0.0)
+        o, A = torch.einsum("hl,lhd->hd", p, v), torch.einsum("hl,lhd->hd", p, v.abs())
+        size = torch.einsum("hd,lhd->hl", q.abs(), k.abs()) / math.sqrt(b.dim)
+        Y = torch.where(p > 0, size, 0.0).amax(-1, keepdim=True)
+        room = A * (2 * (2.0**-20 * Y + 2.0**-21) + 2.0**-18)
+        outs.append(o)
+        rooms.append(room if b.dtype == "f32" else room + half_step(b.dtype) * (A + o.abs()))
+    return torch.stack(outs), torch.stack(rooms)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,prefix,seqs", [
+    (8, 2, 64, 200, 3), (24, 2, 128, 200, 2),                        # up to 16 and 32 vectors of a KV head,
+    (32, 2, 64, 300, 5), (64, 2, 128, 300, 9), (64, 2, 64, 300, 9),  # up to 128 and more
+    (64, 2, 32, 130, 4), (8, 2, 128, 0, 3)])                         # without tcgen05, without a prefix
+def test_attn_scores_of_minus_infinity(dtype, heads, kv_heads, dim, prefix, seqs):
+    top = torch.finfo(TYPES[dtype][0]).max
+    b = Batch(dim + seqs, dtype, heads, kv_heads, dim, 16, prefix, [20 + i for i in range(seqs)], [1] * seqs, poison=False)
+    b.q[..., 0] = b.q[..., 0].abs() + 0.5  # a key of -infinity scores -infinity
+    keys, values = b.keys.clone(), b.values.clone()
+    off = torch.rand(b.keys.shape[0], kv_heads, 16, generator=gen(1), device="cuda")
+    for part, huge in ((0.3, True), (0.9, True), (2.0, False)):  # some rows, most of them, every row
+        for h in (0, 1):  # every row of the first KV head's, some of the second's
+            gone = off[:, h] < (part if h == 0 else part / 3)
+            b.keys[:, h, :, 0] = torch.where(gone, -math.inf, keys[:, h, :, 0])
+            if huge:
+                b.values[:, h] = torch.where(gone[..., None], top, values[:, h])
+            else:
+                b.values[:, h] = values[:, h]
+        b.call()
+        want, room = weighted(b)
+        if not huge:
+            assert (want[:, : heads // kv_heads] == 0).all()
+        within(b.out, want, room, dtype)
+
 
 # ---- verification of drafts ------------------------------------------------------------------------------------------
 
