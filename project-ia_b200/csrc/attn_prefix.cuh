@@ -147,14 +147,17 @@ __device__ __forceinline__ void mma8(float (&c)[4], const uint32_t (&a)[4], uint
         : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-// v = hi + lo, each of 11 significant bits rounded to nearest (the tensor
-// core reads the upper 19 bits of an operand).  The addition that rounds may
-// carry a NaN's bits over into the sign, and hi is a zero then: lo, v - hi, is
-// a NaN too and is kept from the same (and is one for infinities).
+// v = hi + lo: hi of 11 significant bits rounded to nearest, lo the rest, of
+// which the tensor core reads the upper 19 bits (all but the last bit of the
+// 12 it can have).  hi stays finite: v near the type's largest would be
+// rounded to infinity, whose product with a weight of zero is no number.  So
+// an infinity or a NaN (whose bits the rounding could carry into the sign) is
+// in lo alone, and reaches the sum from there.
 __device__ __forceinline__ void split_tf32(uint32_t v, uint32_t& hi, uint32_t& lo) {
-    hi = (v + 0x1000u) & 0xffffe000u;
-    const float d = __uint_as_float(v) - __uint_as_float(hi);
-    lo = (uint32_t)min(__float_as_int(d), 0x7fffe000) + 0x1000u;
+    float c;
+    asm("min.xorsign.abs.f32 %0, %1, %2;" : "=f"(c) : "f"(__uint_as_float(v)), "f"(__uint_as_float(0x7f7fe000u)));
+    hi = (__float_as_uint(c) + 0x1000u) & 0xffffe000u;
+    lo = __float_as_uint(__uint_as_float(v) - __uint_as_float(hi));
 }
 
 // 16-byte chunk c of row r in a tile of HD-wide rows: chunks are exchanged

@@ -32,7 +32,7 @@ def weighted(b):
     return torch.stack(outs), torch.stack(rooms)
 
 
-@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
 @pytest.mark.parametrize("heads,kv_heads,dim,prefix,seqs", [
     (8, 2, 64, 200, 3), (24, 2, 128, 200, 2),                        # up to 16 and 32 vectors of a KV head,
     (32, 2, 64, 300, 5), (64, 2, 128, 300, 9), (64, 2, 64, 300, 9),  # up to 128 and more
@@ -56,6 +56,39 @@ def test_attn_scores_of_minus_infinity(dtype, heads, kv_heads, dim, prefix, seqs
         if not huge:
             assert (want[:, : heads // kv_heads] == 0).all()
         within(b.out, want, room, dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads", [8, 40])
+@pytest.mark.parametrize("sign", [-1, 1])
+def test_attn_newer_rows_of_the_types_largest_numbers_do_not_reach_older_tokens(dtype, heads, sign):
+    b = Batch(4, dtype, heads, 2, 64, 16, 100, [90, 8], [6, 5], poison=False)
+    b.call()
+    clean = b.out.clone()
+    for x in (b.keys, b.values):
+        for r in (88, 89):
+            x[b.pages[0, r // 16].long(), :, r % 16] = sign * torch.finfo(x.dtype).max
+        x[b.pages[1, 0].long(), :, 7] = sign * torch.finfo(x.dtype).max
+    b.call()
+    assert torch.equal(b.out[:4], clean[:4]) and torch.equal(b.out[6:10], clean[6:10])
+
+
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads", [8, 80])
+def test_attn_one_row_of_the_types_largest_numbers(dtype, heads):
+    # alone it is the result itself; beside keys that score more it weighs nothing
+    b = Batch(5, dtype, heads, 2, 64, 16, 0, [1, 40], [1, 1], poison=False)
+    top = torch.finfo(TYPES[dtype][0]).max
+    b.q[..., 0] = b.q[..., 0].abs() + 0.5
+    for i in range(2):
+        page = b.pages[i, 0].long()
+        b.values[page, :, 0] = torch.where(torch.arange(64, device="cuda") % 2 == 0, top, -top).to(b.values.dtype)
+        b.keys[page, :, 0, 0] = -top / 64  # q.k is finite
+    b.call()
+    # fp32's largest number has 24 bits, of which its two halves hold 11 each: off by 2^-22, within the room for products
+    want, room = weighted(b)
+    assert want[0].abs().min() == top
+    within(b.out, want, room, dtype)
 
 
 # ---- verification of drafts ------------------------------------------------------------------------------------------
