@@ -306,12 +306,20 @@ struct AttnPlan {
     uint32_t parts = 0;   // partial results in the workspace
 };
 
+// Most rows of one running sum.  The tensor core truncates what it adds to a
+// sum, 2^-24.4 of it for each product of 16 rows on tcgen05 and 2^-23.4 on
+// mma.sync (a million equal values in one sum came out 0.3% and 0.15% low), so
+// a sum ends after 1024 and 512 of them: 5e-5 at most, a tenth of fp16's half
+// step.  Rows past that are cut into more parts, which are added in fp32.  The
+// sums of fp32 caches are rounded instead, which equal values share too.
+constexpr uint32_t TC_SUM_ROWS = 1024 * 16, WARP_SUM_ROWS = 512 * 16;
+
 uint32_t ctas_per_sm(const AttnPass& p) { return p.kern == ATTN_TC ? 1 : p.kern == ATTN_FEW && p.mb == 1 ? 3 : 2; }
 
 // A pass of attn_few_kernel (up to 32 vectors) or attn_rows_kernel: the rows
 // are cut until as many CTAs as `sms` run at once have work, each with at least
-// two tiles.  Up to 8 cuts of the own rows are one cluster's and leave nothing
-// in the workspace.
+// two tiles, and a warp's sums end in time.  Up to 8 cuts of the own rows are
+// one cluster's and leave nothing in the workspace.
 AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t rows, uint32_t step, bool own, uint32_t sms) {
     AttnPass p;
     p.kern = vecs <= 32 ? ATTN_FEW : ATTN_ROWS;
@@ -321,6 +329,8 @@ AttnPass plan_pass(uint32_t vecs, uint32_t seqs, uint32_t kv_heads, uint32_t row
     const uint64_t ctas = (uint64_t)p.items * kv_heads;
     const uint32_t most = std::max(1u, cdiv(rows, 2 * step));
     p.splits = (uint32_t)std::min<uint64_t>({std::max<uint64_t>(1, ctas_per_sm(p) * sms / ctas), most, 64});
+    // the rows are shared out over four warps (FEW), or all four take each
+    p.splits = std::max(p.splits, cdiv(rows, p.kern == ATTN_FEW ? 4 * WARP_SUM_ROWS : WARP_SUM_ROWS));
     if (p.kern == ATTN_FEW && own && p.splits > 1) {
         p.cluster = p.splits <= 8 || rows <= 8 * 4 * step;
         if (p.cluster) p.splits = std::min(p.splits, 8u);
@@ -340,6 +350,7 @@ AttnPass plan_tc(uint32_t vecs, uint32_t kv_heads, uint32_t rows, uint32_t sms) 
     p.tiles = p.items = cdiv(vecs, p.alternate ? 128 : 256);
     const uint32_t ctas = p.items * kv_heads;
     p.splits = std::min({std::max(1u, sms / ctas), std::max(1u, rows / (4 * TC_ROWS)), ATTN_MAX_PARTS});
+    p.splits = std::max(p.splits, cdiv(rows, p.alternate ? 2 * TC_SUM_ROWS : TC_SUM_ROWS));
     p.parts = p.splits;
     return p;
 }

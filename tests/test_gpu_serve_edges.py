@@ -91,6 +91,27 @@ def test_attn_one_row_of_the_types_largest_numbers(dtype, heads):
     within(b.out, want, room, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,seqs,rows,prefix", [
+    (400, 100, 4, 1 << 20, 0), (320, 8, 4, 1 << 20, 0), (4, 1, 1, 300000, 0),         # own rows: up to 32 vectors, more, one sequence
+    (1280, 160, 9, 300, 1 << 20), (1280, 160, 40, 300, 1 << 18), (320, 160, 3, 20, 1 << 20)])  # the prefix: up to 128 vectors, more, few
+def test_attn_sums_of_many_rows(dtype, heads, kv_heads, seqs, rows, prefix):
+    # A page table that names the same pages again and again.  Queries of zero weigh all rows alike, exactly, so the result is the
+    # values' own: off by what the sums lose (a product truncates its sum by two steps of 2^-24 of it at most, half of that on the
+    # average over a growing sum, 512 of them, or 1024 that truncate once; fp32 rounds 1024 times by 2^-24 at most) and by one rounding.
+    b = Batch(2, dtype, heads, kv_heads, 64, 16, 288, [288] * seqs, [1] * seqs, poison=False)
+    b.q = torch.zeros_like(b.q)
+    value = torch.linspace(0.3, 3.0, 64, device="cuda").to(TYPES[dtype][0])
+    b.values.copy_(value.expand_as(b.values))
+    again = lambda p, n: p[..., torch.arange(-(-n // 16), device="cuda") % 18].contiguous()  # noqa: E731
+    b.pages, b.prefix_pages = again(b.pages, rows), again(b.prefix_pages, prefix) if prefix else b.prefix_pages
+    b.per, b.rows, b.prefix = b.pages.shape[1], [rows - i for i in range(seqs)], prefix
+    b.lens, b.prefix_len = ints(b.rows), ints([prefix])
+    b.call()
+    want = value.double().expand(seqs, heads, 64)
+    within(b.out, want, want * 2.0**-14, dtype)
+
+
 # ---- verification of drafts ------------------------------------------------------------------------------------------
 
 
