@@ -478,9 +478,10 @@ __global__ void __launch_bounds__(VER_THREADS, ver_ctas(KIND)) verify_kernel(con
             xp.load(prow, i0, g1, a.vec, none);
             if (two) xq.load(qrow, i0, g1, a.vec, none);
             double part = 0.0;
-            if (KIND == VER_PROBS && !(rest && gone - i0 < VER_VECS * 32 * E)) {
-                part = rest_sum(xp, xq, two);
-            } else {
+            const bool pairs = KIND == VER_PROBS && !(rest && gone - i0 < VER_VECS * 32 * E);
+            if (pairs) part = rest_sum(xp, xq, two);
+            if (!pairs || !(part < INFINITY)) {  // weights near the type's largest pass fp32
+                part = 0.0;
 #pragma unroll
                 for (int k = 0; k < VER_VECS; ++k) {
                     double w[E];

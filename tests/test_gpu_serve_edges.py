@@ -151,3 +151,18 @@ def test_verify_logits_far_from_zero(dtype, T, offset, spread):
         # (weights of so low a temperature are one or zero with either)
         want, m = verify64(t, draft, xs, us, "logits", float(np.nextafter(np.float32(T), np.float32(1))) if T == 1e-6 else T)
         assert np.array_equal(n, m) and np.array_equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("S,K,V", [(1, 0, 5000), (1, 2, 128256), (40, 1, 20001)])
+def test_verify_weights_whose_sum_passes_fp32(dtype, S, K, V):
+    # rows of weights need not sum to one, nor to anything that fp32 holds
+    g = gen(V)
+    target = (torch.rand(S, K + 1, V, generator=g, device="cuda") * 3e38).to(TYPES[dtype][0])
+    draft = (torch.rand(S, K, V, generator=g, device="cuda") * 3e38).to(TYPES[dtype][0]) if K else None
+    x = torch.randint(0, V, (S, max(1, K)), generator=g, device="cuda", dtype=torch.int32)
+    u = torch.rand(S, K + 1, generator=g, device="cuda")
+    for d in (draft, None):
+        got, n = do_verify(target, d, x, u, "probs", 1.0, None, dtype)
+        want, m = verify64(target, d, x, u)
+        assert np.array_equal(n, m) and np.array_equal(got, want)
