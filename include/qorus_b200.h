@@ -366,7 +366,7 @@ q_error_code q_b200_attn_prefix(const q_b200_attn_args* args, void* stream);
  * is the first maximum of the target, and q is not used).  draft NULL: q is
  * one at the drafted token.  NaN and negative weights count as zero; where
  * the difference has no weight the row p is used, and a row without weight
- * gives token 0. */
+ * gives token 0.  tokens and n_tokens overlap none of the other arrays. */
 typedef enum { Q_B200_PROBS = 0, Q_B200_LOGITS = 1 } q_b200_verify_kind;
 typedef struct {
     const void* target; /* [n_seqs][n_draft + 1][vocab] */

@@ -59,6 +59,10 @@ bool short_strides(std::initializer_list<uint64_t> v) {
 }
 uint64_t addr(const void* p) { return (uint64_t)(uintptr_t)p; }
 
+bool overlap(const void* a, uint64_t an, const void* b, uint64_t bn) {
+    return a && b && an && bn && addr(a) < addr(b) + bn && addr(b) < addr(a) + an;
+}
+
 q_error_code check_cache(const q_b200_paged_kv& kv) {
     if (!kv.k || !kv.v) return Q_ERR_INVALID_ARG;
     if (!known(kv.dtype)) return Q_ERR_INVALID_DTYPE;
@@ -625,8 +629,12 @@ q_error_code q_b200_verify_draft(const q_b200_verify_args* r, void* stream) {
     if (((addr(r->target) | addr(r->draft)) & (es - 1)) ||
         ((addr(r->draft_tokens) | addr(r->draft_len) | addr(r->uniform) | addr(r->tokens) | addr(r->n_tokens)) & 3))
         return Q_ERR_MISALIGNED;
-    if ((const void*)r->tokens == (const void*)r->draft_tokens || (const void*)r->tokens == (const void*)r->n_tokens)
-        return Q_ERR_ALIASING;
+    // one sequence's outputs would be written over what another has yet to read
+    const uint64_t S = r->n_seqs, K = r->n_draft, tb = S * (K + 1) * 4, nb = S * 4;
+    for (const auto& in : {std::make_pair((const void*)r->draft_tokens, S * K * 4), std::make_pair((const void*)r->draft_len, nb),
+                           std::make_pair((const void*)r->uniform, tb)})
+        if (overlap(r->tokens, tb, in.first, in.second) || overlap(r->n_tokens, nb, in.first, in.second)) return Q_ERR_ALIASING;
+    if (overlap(r->tokens, tb, r->n_tokens, nb)) return Q_ERR_ALIASING;
     if (!DevicePtrs()(r->target)(r->draft)(r->draft_tokens)(r->draft_len)(r->uniform)(r->tokens)(r->n_tokens).ok)
         return Q_ERR_INVALID_ARG;
     VerifyArgs a{};

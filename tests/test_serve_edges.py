@@ -35,3 +35,17 @@ def test_attn_work_bytes_is_zero_where_the_call_is_refused(kw):
     kw = dict(kw, kv=cache(n_kv_heads=2))
     assert work_bytes(**kw) == 0
     assert attn(**kw) == SIZE
+
+
+# ---- outputs that lie over what is still read ------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("kw,rc", [  # 2 sequences of 4 drafts: tokens and uniform 40 bytes, draft_tokens 32, the others 8
+    (dict(tokens=3 * P + 28), ALIAS), (dict(tokens=3 * P - 36), ALIAS), (dict(tokens=3 * P + 32), ARG), (dict(tokens=3 * P - 40), ARG),
+    (dict(tokens=4 * P), ALIAS), (dict(tokens=4 * P + 36), ALIAS), (dict(tokens=4 * P + 40), ARG),
+    (dict(n_tokens=3 * P + 16), ALIAS), (dict(n_tokens=4 * P + 12), ALIAS), (dict(n_tokens=5 * P + 36), ALIAS),
+    (dict(n_tokens=5 * P + 40), ARG), (dict(n_tokens=5 * P - 4), ALIAS), (dict(n_tokens=5 * P - 8), ARG),
+    (dict(draft_len=7 * P, tokens=7 * P + 4), ALIAS), (dict(draft_len=7 * P, n_tokens=7 * P), ALIAS), (dict(draft_len=7 * P, n_tokens=7 * P + 8), ARG)])
+def test_verify_refuses_outputs_over_its_inputs(kw, rc):
+    # ARG: no overlap, so the refusal is the one of pointers that are no device memory
+    assert verify(**kw) == rc
