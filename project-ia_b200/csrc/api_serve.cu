@@ -17,6 +17,8 @@ using namespace qb200;
 
 namespace {
 
+constexpr uint32_t SMS = 148;  // of a B200; plans are made without a device too
+
 uint32_t size_of(uint32_t dtype) { return dtype == Q_B200_F32 ? 4u : 2u; }
 bool known(uint32_t dtype) { return dtype <= Q_B200_BF16; }
 
@@ -93,7 +95,7 @@ cudaError_t launch_rotate_units(RotateArgs& a, cudaStream_t st) {
     const uint64_t all = (uint64_t)a.n_tokens * a.heads * U;
     const uint32_t most = a.rot ? std::min(ROT_TOKENS, ROT_ANGLES / (a.rot / 2)) : ROT_TOKENS;
     uint32_t N = 0, filled = 0;
-    for (uint32_t n = all >= 148ull * 8 * ROT_THREADS ? 2 : 1, last = n == 1 ? 1 : 3; n <= last; ++n) {
+    for (uint32_t n = all >= 8ull * SMS * ROT_THREADS ? 2 : 1, last = n == 1 ? 1 : 3; n <= last; ++n) {
         const uint32_t room = n * a.row_step, h = std::min(a.heads, room), t = std::min({a.n_tokens, std::max(1u, room / h), most});
         if (N && h * t * 1000 / room <= filled) continue;
         N = n;
@@ -318,6 +320,13 @@ struct AttnPlan {
 // sums of fp32 caches are rounded instead, which equal values share too.
 constexpr uint32_t TC_SUM_ROWS = 1024 * 16, WARP_SUM_ROWS = 512 * 16;
 
+// CTAs on an SM that a pass is cut for: those that run there at once, by
+// registers and shared memory, but for attn_rows_kernel on fp32 rows of 128,
+// whose ring (131 KB) leaves room for one.  Parts for two share out better
+// there: 16 x 1 tokens of 32/8 heads over 4096 + 1024 rows take 101 us and 112
+// with parts for one, 8 x 5 of 64/8 heads over 4096 + 512 rows 296 and 354, 4 x
+// 32 of 32/8 heads over 1024 + 512 rows 157 and 191 (1 x 64 over 2048 own rows
+// alone 72 and 65).
 uint32_t ctas_per_sm(const AttnPass& p) { return p.kern == ATTN_TC ? 1 : p.kern == ATTN_FEW && p.mb == 1 ? 3 : 2; }
 
 // A pass of attn_few_kernel (up to 32 vectors) or attn_rows_kernel: the rows
@@ -384,37 +393,42 @@ AttnPlan plan_attn(const q_b200_attn_args* r) {
     const uint32_t heads = r->kv.n_kv_heads, own_rows = std::max(1u, r->max_len + (p.shared ? 0 : prefix));
     auto own = [&](uint32_t sms) { return plan_pass(r->max_q * G, r->n_seqs, heads, own_rows, step, true, sms); };
     if (!p.shared) {
-        p.own = own(148);
+        p.own = own(SMS);
     } else {
         const uint32_t vecs = r->n_tokens * G;
         const bool tc = r->kv.dtype != Q_B200_F32 && r->kv.head_dim >= 64 && r->scale > 0.0f && vecs > 32;
         auto pre = [&](uint32_t sms) { return tc ? plan_tc(vecs, heads, prefix, sms) : plan_pass(vecs, 1, heads, prefix, step, false, sms); };
-        // The two passes run side by side where the own rows' CTAs all find
+        // The two passes may run side by side, if the own rows' CTAs all find
         // room beside the prefix's (they wait for them before they add the
-        // parts): the SMs are shared by what each pass takes.  Where they do
-        // not, one pass follows the other and each has the whole GPU.  SM
-        // microseconds as measured: 3 to 5 for a CTA's begin and end; 0.9 for a
-        // tile of 128 rows on tcgen05, 1.9 for two streams' vectors; 0.95 to 1.6
-        // for a chunk (16 rows, 8 of fp32) of a warp.
-        const AttnPass one = own(0);
-        const uint64_t n_own = (uint64_t)one.items * heads;
-        const uint32_t need = cdiv(n_own, ctas_per_sm(one));
-        if (need <= 148 * 6 / 10) {
-            const AttnPass pt = pre(0);
-            const double chunk = 4.0 * ctas_per_sm(one) * (step / 4) / (step == 32 ? 1.6 : 0.95);
-            const double t_own = n_own * (0.6 * own_rows / chunk + 5.0 / ctas_per_sm(one));
-            const double n_pre = (double)pt.items * heads;
-            const double t_pre = tc ? n_pre * (prefix / 128.0 * (pt.alternate ? 0.9 : 1.9) + 4.0 * 148 / (2 * n_pre))
-                                    : n_pre * (prefix / (4.0 * ctas_per_sm(pt) * (step / 4) / (step == 32 ? 1.6 : 0.95)) + 5.0);
-            // whole sets of the own rows' CTAs, so that none of them has to wait for the prefix's SMs
-            uint32_t sets = std::max(1u, (uint32_t)std::lround(148 * t_own / (t_own + t_pre) / need));
-            while (sets > 1 && sets * need > 148 * 7 / 10) --sets;
-            p.pre = pre(148 - std::min(sets * need, 144u));
+        // parts): the SMs are shared by what each pass takes, in whole sets of
+        // the own rows' CTAs, so that (fp32 rows of 128 aside) none has to wait
+        // for the prefix's SMs.  Or one pass follows the other and each has the
+        // whole GPU.  SM microseconds as measured: 3 to 5 for a CTA's begin and
+        // end; 0.9 for a tile of 128 rows on tcgen05, 1.9 for two streams'
+        // vectors; 0.95 to 1.6 for a chunk (16 rows, 8 of fp32) of a warp.
+        // Lengths are taken to be spread over max_len, 0.6 of it on the average.
+        const AttnPass one = own(0), pt = pre(0);
+        const double n_own = (double)one.items * heads, n_pre = (double)pt.items * heads;
+        const double need = std::ceil(n_own / ctas_per_sm(one));
+        const double chunk = 4.0 * ctas_per_sm(one) * (step / 4) / (step == 32 ? 1.6 : 0.95);
+        const double t_own = n_own * (0.6 * own_rows / chunk + 5.0 / ctas_per_sm(one));
+        const double t_pre = tc ? n_pre * (prefix / 128.0 * (pt.alternate ? 0.9 : 1.9) + 4.0 * SMS / (2 * n_pre))
+                                : n_pre * (prefix / (4.0 * ctas_per_sm(pt) * (step / 4) / (step == 32 ? 1.6 : 0.95)) + 5.0);
+        double sets = std::max(1.0, std::round(SMS * t_own / (t_own + t_pre) / need));
+        while (sets > 1.0 && sets * need > SMS * 0.7) --sets;  // the prefix's CTAs are the longer ones
+        // Side by side saves one begin and end, 6 us, but a set can be far more
+        // than the own rows' share.  Measured, side by side and one after the
+        // other, bf16, 32/8 heads of 128: 16 x 1 tokens over 4096 + 1024 rows 15.8
+        // and 22.7 us, 40 x 1 24.8 and 38.1, 48 x 1 41.3 and 39.7; 16 x 4 over 16384
+        // + 256 rows 39.3 and 37.6, 24 x 4 64 and 48, 32 x 4 96 and 52.
+        const double left = SMS - sets * need;
+        if (left >= 4.0 && std::max(t_pre / left, t_own / (sets * need)) <= 1.25 * ((t_own + t_pre) / SMS + 6.0)) {
+            p.pre = pre((uint32_t)left);
             const uint32_t used = cdiv((uint64_t)p.pre.items * p.pre.splits * heads, ctas_per_sm(p.pre));
-            p.own = own(std::max(need, used < 148 ? 148 - used : 0u));
+            p.own = own(std::max((uint32_t)need, used < SMS ? SMS - used : 0u));
         } else {
-            p.pre = pre(148);
-            p.own = own(148);
+            p.pre = pre(SMS);
+            p.own = own(SMS);
         }
     }
     p.parts = (p.shared ? p.pre.parts : 0) + p.own.parts;
@@ -664,7 +678,7 @@ q_error_code q_b200_verify_draft(const q_b200_verify_args* r, void* stream) {
     // GPU has room for, only for a few sequences
     const uint32_t once = ver_vecs(kind) * 32 * (16 / es) * VER_WARPS;
     uint32_t CL = r->n_seqs <= 4 ? 16 : 8;
-    while (CL > 1 && ((uint64_t)r->n_seqs * CL > 148u * ver_ctas(kind) || (uint64_t)(CL / 2) * once >= r->vocab)) CL /= 2;
+    while (CL > 1 && ((uint64_t)r->n_seqs * CL > (uint64_t)SMS * ver_ctas(kind) || (uint64_t)(CL / 2) * once >= r->vocab)) CL /= 2;
     a.seg = (cdiv(r->vocab, (uint64_t)CL * VER_WARPS) + 7) & ~7u;
     cudaStream_t st = (cudaStream_t)stream;
     switch (r->dtype) {

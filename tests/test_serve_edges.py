@@ -49,3 +49,16 @@ def test_attn_work_bytes_is_zero_where_the_call_is_refused(kw):
 def test_verify_refuses_outputs_over_its_inputs(kw, rc):
     # ARG: no overlap, so the refusal is the one of pointers that are no device memory
     assert verify(**kw) == rc
+
+
+# ---- plans -----------------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("seqs,new,prefix,rows", [(32, 4, 16384, 256), (24, 4, 16384, 256), (32, 4, 8192, 64)])
+def test_attn_prefix_gets_the_sms_that_its_work_asks_for(seqs, new, prefix, rows):
+    # bf16, 32/8 heads of 128: 16 CTAs for each part of the prefix, whose work is 0.85 of the whole or more.  The own rows (8 splits
+    # of a cluster at most) leave nothing in the workspace, so its parts are the prefix's: as many as the 148 SMs run at once.
+    kw = dict(n_tokens=seqs * new, n_seqs=seqs, max_q=new, n_heads=32, max_prefix=prefix, max_len=rows, q_start=8 * P, pages_per_seq=rows // 32,
+              kv=cache(n_kv_heads=8, dtype=Q.Q_B200_BF16))
+    parts, rest = divmod(work_bytes(**kw), seqs * new * 32 * (128 * 4 + 8))
+    assert rest == 0 and 0.85 * 148 <= parts * 16 <= 148
