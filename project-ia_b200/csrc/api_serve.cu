@@ -107,12 +107,14 @@ cudaError_t launch_rotate_units(RotateArgs& a, cudaStream_t st) {
     a.by_heads = fast_div_of(a.cta_heads);
     a.by_pairs = fast_div_of(std::max(1u, a.rot / 2));
     const dim3 grid(cdiv(a.n_tokens, a.cta_tokens), cdiv(a.heads, a.cta_heads));
-    constexpr bool same = std::is_same<TI, TC>::value;
-    if (a.row || !same)
-        return launch_ex(N == 3 ? rotate_kernel<TI, TC, E, 3, true> : N == 2 ? rotate_kernel<TI, TC, E, 2, true> : rotate_kernel<TI, TC, E, 1, true>,
+    auto go = [&](auto append) {
+        constexpr bool A = decltype(append)::value;
+        return launch_ex(N == 3 ? rotate_kernel<TI, TC, E, 3, A> : N == 2 ? rotate_kernel<TI, TC, E, 2, A> : rotate_kernel<TI, TC, E, 1, A>,
                          grid, dim3(ROT_THREADS), 0, st, true, a);
-    return launch_ex(N == 3 ? rotate_kernel<TI, TI, E, 3, false> : N == 2 ? rotate_kernel<TI, TI, E, 2, false> : rotate_kernel<TI, TI, E, 1, false>,
-                     grid, dim3(ROT_THREADS), 0, st, true, a);
+    };
+    if constexpr (std::is_same<TI, TC>::value)
+        if (!a.row) return go(std::false_type());
+    return go(std::true_type());  // q_b200_kv_append; types that differ are its alone
 }
 
 template <typename TI, typename TC>
