@@ -1,8 +1,11 @@
 """The serving operators at values, lengths and tables past those of test_gpu_serve.py, whose helpers and tolerances they use."""
+import ctypes as C
 import math
 
 import numpy as np
 import pytest
+
+import qorus_b200 as Q
 
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
@@ -110,6 +113,41 @@ def test_attn_sums_of_many_rows(dtype, heads, kv_heads, seqs, rows, prefix):
     b.call()
     want = value.double().expand(seqs, heads, 64)
     within(b.out, want, want * 2.0**-14, dtype)
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64)])
+@pytest.mark.parametrize("G,seqs,prefix", [(4, 20, 4100), (4, 40, 4173), (1, 300, 6143), (2, 64, 12289)])
+def test_attn_prefix_parts_of_many_tiles(dtype, dim, G, seqs, prefix):
+    # 160 KV heads leave one part each: 33 tiles of 128 rows and more in one CTA, so that its ring of 5 or 9 slots and all of its
+    # barriers go round many times, for one tile of vectors (80, 128) and two (160, 300)
+    KV, L, R = 160, 3, 32
+    g = gen(prefix)
+    shared = -(-prefix // R)
+    pool = torch.randn(shared + seqs, KV, R, 2 * dim, generator=g, device="cuda", dtype=torch.float16).to(TYPES[dtype][0])
+    keys, values = pool[..., :dim], pool[..., dim:]
+    q = torch.randn(seqs, KV * G, dim, generator=g, device="cuda").to(TYPES[dtype][0])
+    out, ids = torch.zeros_like(q), torch.randperm(shared + seqs, generator=g, device="cuda").to(torch.int32)
+    prefix_pages, pages, lens, n = ids[:shared].contiguous(), ids[shared:].contiguous(), ints([L] * seqs), ints([prefix])
+    kv = Q.q_b200_paged_kv(keys.data_ptr(), values.data_ptr(), pool.stride(0), pool.stride(1), pool.stride(2), shared + seqs, R, KV, dim,
+                           TYPES[dtype][1], 0)
+    a = Q.q_b200_attn_args(kv, q.data_ptr(), out.data_ptr(), q.stride(0), dim, q.stride(0), dim, None, pages.data_ptr(), lens.data_ptr(),
+                           prefix_pages.data_ptr(), n.data_ptr(), None, 0, seqs, seqs, KV * G, 1, 1, L, prefix, 1 / math.sqrt(dim))
+    work = torch.empty(Q.lib.q_b200_attn_work_bytes(C.byref(a)), dtype=torch.uint8, device="cuda")
+    assert work.numel() == seqs * KV * G * (dim * 4 + 8)  # one part
+    a.work, a.work_bytes = work.data_ptr(), work.numel()
+    Q.check(Q.lib.q_b200_attn_prefix(C.byref(a), torch.cuda.current_stream().cuda_stream), "attn")
+    assert Q.lib.q_b200_device_status() == 0
+    for h in range(0, KV, 9):
+        rows = lambda x: torch.cat([x[prefix_pages.long(), h].reshape(-1, dim)[:prefix].expand(seqs, -1, -1), x[pages.long(), h, :L]], 1)  # noqa: E731
+        k, v, x = rows(keys).double(), rows(values).double(), q[:, h * G: (h + 1) * G].double()
+        y = x @ k.transpose(1, 2) / math.sqrt(dim)
+        w = torch.softmax(y, -1)
+        o, A = w @ v, w @ v.abs()
+        Y = (x.abs() @ k.abs().transpose(1, 2) / math.sqrt(dim)).amax(-1, keepdim=True)
+        # the rooms of test_gpu_serve.py with what this pass adds: a quarter of the exponentials good to 5.6e-5 < 2^-14, and a sum
+        # that up to 1024 products truncate, by 2^-24 of it each on the average
+        room = A * (2 * (2.0**-20 * Y + 2.0**-14) + 2.0**-14) + half_step(dtype) * (A + o.abs())
+        within(out[:, h * G: (h + 1) * G], o, room, dtype)
 
 
 # ---- verification of drafts ------------------------------------------------------------------------------------------
