@@ -385,7 +385,11 @@ q_error_code q_b200_verify_draft(const q_b200_verify_args* args, void* stream);
 
 /* The paged caches of a batched context as one layer's q_b200_paged_kv, with
  * the device page table (the caches' own, current after the last call that
- * took or wrote rows). */
+ * took or wrote rows).  The view takes no pages: rows have them once they were
+ * written (q_b200_batch_kv_write) or decoded, and an append to others leaves
+ * code 4.  The call waits for the context's stream where pages changed hands
+ * since the last one, so it is made outside a capture; operators on the view
+ * run on q_b200_stream(ctx) or are synchronised with it. */
 q_error_code q_b200_batch_kv_view(q_context* ctx, uint32_t layer, q_b200_paged_kv* kv, const uint32_t** pages,
                                   uint32_t* pages_per_seq);
 

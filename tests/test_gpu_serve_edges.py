@@ -10,7 +10,7 @@ import qorus_b200 as Q
 pytestmark = pytest.mark.gpu
 torch = pytest.importorskip("torch")
 
-from test_gpu_serve import TYPES, Batch, do_verify, gen, half_step, ints, verify64, within  # noqa: E402
+from test_gpu_serve import TYPES, Batch, do_verify, gen, half_step, ints, make_plan, turn64, verify64, within  # noqa: E402
 
 # ---- attention -------------------------------------------------------------------------------------------------------
 
@@ -148,6 +148,79 @@ def test_attn_prefix_parts_of_many_tiles(dtype, dim, G, seqs, prefix):
         # that up to 1024 products truncate, by 2^-24 of it each on the average
         room = A * (2 * (2.0**-20 * Y + 2.0**-14) + 2.0**-14) + half_step(dtype) * (A + o.abs())
         within(out[:, h * G: (h + 1) * G], o, room, dtype)
+
+
+# ---- the batch's own pages ---------------------------------------------------------------------------------------------
+
+
+def test_rows_appended_through_the_view_are_the_frameworks_own(tmp_path):
+    cfg = Q.config(vocab=259, dim=256, hidden=512, layers=2, heads=8, kv_heads=2, max_seq=256)
+    Q.write_model(str(tmp_path / "m.qorus"), cfg, seed=0, threads=1)
+    N, hd = 130, 32
+    ms = [Q.Model(str(tmp_path / "m.qorus")) for _ in range(2)]
+    for m in ms:
+        Q.check(Q.lib.q_b200_batch_init_paged(C.byref(m.ctx), C.byref(m.model), 2, 128, 6), "batch_init_paged")
+    first, second = ms
+    vocab, logits, nxt = cfg.vocab_size, [np.zeros((2, cfg.vocab_size), np.float32) for _ in ms], [np.zeros(2, np.uint32) for _ in ms]
+
+    def decode(i, tokens, pos):
+        t, p = np.array(tokens, np.uint32), np.array(pos, np.uint32)
+        Q.check(Q.lib.q_b200_decode_batch(C.byref(ms[i].model), C.byref(ms[i].ctx), Q.ptr(t), Q.ptr(p), Q.ptr(logits[i]), Q.ptr(nxt[i])), "decode")
+
+    rng = np.random.default_rng(0)
+    tokens = rng.integers(0, vocab, (N, 2))
+    tokens[100] = tokens[0]  # the same tokens at row 0, where nothing turns, and at row 100
+    for n in range(N):
+        decode(0, tokens[n], [n, n])
+    rows = np.zeros((2, 2, 2, 256, 2 * hd), np.float32)  # [seq][layer][head][row][K|V]
+    for b in range(2):
+        Q.check(Q.lib.q_b200_batch_kv_read(C.byref(first.ctx), b, 0, Q.ptr(rows[b]), rows[b].nbytes), "kv_read")
+    none = np.zeros((N, 2 * hd), np.float32)
+    for b in range(2):  # rows that are written take pages
+        Q.check(Q.lib.q_b200_batch_kv_write(C.byref(second.ctx), b, 0, Q.ptr(none), none.nbytes), "kv_write")
+    kv, pages, per = Q.q_b200_paged_kv(), C.c_void_p(), C.c_uint32()
+    seq, row = ints([b for b in range(2) for _ in range(N)]), ints(list(range(N)) * 2)
+
+    def append(layer, k, v, seq, row, plan):
+        Q.check(Q.lib.q_b200_batch_kv_view(C.byref(second.ctx), layer, C.byref(kv), C.byref(pages), C.byref(per)), "view")
+        a = Q.q_b200_append_args(kv, k.data_ptr(), v.data_ptr(), None, None, k.stride(0), k.stride(1), v.stride(0), v.stride(1), 0, 0, 0, 0, pages,
+                                 seq.data_ptr(), row.data_ptr(), None, C.addressof(plan) if plan else None, len(row), 2, per.value, 0, Q.Q_B200_F32, 0)
+        torch.cuda.synchronize()
+        Q.check(Q.lib.q_b200_kv_append(C.byref(a), second.stream), "append")
+        torch.cuda.synchronize()
+
+    # rotation: the framework's row 0 (layer 0 knows the token alone), turned to row 100 here, is the framework's row 100.  Its angles
+    # are fp32 products: off by 100 * 2^-22 (frequency and product), beside what turn64 allows for this side
+    plan = make_plan(hd, "interleaved")
+    raw = torch.from_numpy(rows[:, 0, :, 0]).cuda()
+    append(0, raw[..., :hd], raw[..., hd:], ints([0, 1]), ints([100, 100]), plan)
+    mine = np.zeros((2, 256, 2 * hd), np.float32)
+    for b in range(2):
+        Q.check(Q.lib.q_b200_batch_kv_read(C.byref(second.ctx), b, 0, Q.ptr(mine), mine.nbytes), "kv_read")
+        want, room = turn64(raw[b:b + 1, :, :hd], ints([100]), plan)
+        got = torch.from_numpy(mine[:, 100]).cuda()
+        within(got[None, :, :hd], want, room, "f32")
+        theirs = torch.from_numpy(rows[b, 0, :, 100]).cuda().double()
+        assert ((got[:, :hd].double() - theirs[:, :hd]).abs() <= 2 * room[0] * (1 + 100 * 2.0**-22 / 2.0**-20)).all()
+        assert torch.equal(got[:, hd:].double(), theirs[:, hd:])
+    # the framework's rows, appended as they are: the next step has the same bits
+    for layer in range(2):
+        x = torch.from_numpy(rows[:, layer, :, :N]).cuda().transpose(1, 2).reshape(2 * N, 2, 2 * hd)
+        append(layer, x[..., :hd], x[..., hd:], seq, row, None)
+    for step in range(3):
+        for i in range(2):
+            decode(i, nxt[i] if step else tokens[0], [N + step] * 2)
+        assert np.array_equal(logits[0], logits[1]) and np.array_equal(nxt[0], nxt[1])
+    # a row past the pages that the sequence has is skipped: the view takes none
+    assert Q.lib.q_b200_device_status() == 0
+    x = torch.ones(1, 2, 2 * hd, device="cuda")
+    append(0, x[..., :hd], x[..., hd:], ints([1]), ints([256]), None)
+    assert Q.lib.q_b200_device_status() == 4
+    Q.check(Q.lib.q_b200_batch_release(C.byref(second.ctx), 1), "release")
+    append(0, x[..., :hd], x[..., hd:], ints([1]), ints([0]), None)
+    assert Q.lib.q_b200_device_status() == 4
+    for m in ms:
+        m.close()
 
 
 # ---- verification of drafts ------------------------------------------------------------------------------------------
