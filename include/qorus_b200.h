@@ -250,8 +250,9 @@ typedef enum { Q_B200_ROPE_INTERLEAVED = 0, Q_B200_ROPE_HALF = 1 } q_b200_rope_l
  *           between
  *   YARN    the same by pair index: pairs that turn more than `high` times
  *           in original_len are kept, those that turn less than `low` times
- *           slowed, linear in the index between; cosine and sine are
- *           multiplied by gain (0: 0.1 ln(factor) + 1) */
+ *           slowed, linear in the index between (from the whole index before
+ *           the one to that behind the other, within 0 and rot_dim - 1);
+ *           cosine and sine are multiplied by gain (0: 0.1 ln(factor) + 1) */
 typedef enum {
     Q_B200_ROPE_PLAIN = 0,
     Q_B200_ROPE_LINEAR = 1,

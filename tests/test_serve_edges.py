@@ -62,3 +62,30 @@ def test_attn_prefix_gets_the_sms_that_its_work_asks_for(seqs, new, prefix, rows
               kv=cache(n_kv_heads=8, dtype=Q.Q_B200_BF16))
     parts, rest = divmod(work_bytes(**kw), seqs * new * 32 * (128 * 4 + 8))
     assert rest == 0 and 0.85 * 148 <= parts * 16 <= 148
+
+
+# ---- frequencies -----------------------------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("rot", [2, 6, 48, 128, 256])
+@pytest.mark.parametrize("base", [10000.0, 500000.0])
+@pytest.mark.parametrize("factor,low,high,length", [
+    (8.0, 1.0, 32.0, 8192.0), (4.0, 1.0, 32.0, 4096.0), (40.0, 0.5, 3.0, 1000.0),
+    (16.0, 1.0, 1.5, 131072.0),                                # a ramp of a pair or two
+    (2.0, 1.0, 32.0, 50.0),                                    # every wave turns less than 32 times: the ramp begins before pair 0
+    (2.0, 1e-9, 1e-8, 4096.0), (0.5, 1.0, 32.0, 1e30)])        # it ends behind the last pair; every pair turns more than that
+def test_yarn_frequencies_pair_by_pair(rot, base, factor, low, high, length):
+    p = plan(rot, base=base, scale=scale(3, factor, low, high, length))
+    # the pair (a fraction) whose wave turns n times in `length` positions: n 2 pi = length base^(-2i/rot)
+    pair = lambda n: rot / 2 * math.log(length / (2 * math.pi * n), base)  # noqa: E731
+    ends = [pair(high), pair(low)]
+    if any(abs(e - round(e)) < 1e-9 * max(1.0, abs(e)) for e in ends):
+        pytest.skip("an end on a pair: a matter of rounding")
+    first, last = max(math.floor(ends[0]), 0), min(math.ceil(ends[1]), rot - 1)
+    for i in range(rot // 2):
+        f = base ** (-2 * i / rot)
+        kept = 1.0 - min(max((i - first) / max(last - first, 0.001), 0.0), 1.0)
+        want = kept * f + (1.0 - kept) * f / factor
+        # roundings of 2^-53: the power's (its exponent's times ln base < 14), a dozen others
+        assert abs(p.turns[i] * 2 * math.pi - want) <= 1e-14 * want, i
+    assert p.gain == np.float32(0.1 * math.log(factor) + 1.0) and p.rot_dim == rot
