@@ -282,8 +282,7 @@ __global__ void __launch_bounds__(FEW_THREADS, MB == 1 ? 3 : 2) attn_few_kernel(
             for (int h = 0; h < 2; ++h) {
                 mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
                 mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-                // the maximum moves only past 2^8 times the old one (fp16 holds that): few outputs are rescaled
-                const float M = mx[h] > m[b][h] + 8.0f ? mx[h] : m[b][h];
+                const float M = attn_reference<T>(m[b][h], mx[h]);
                 const float base = M == -INFINITY ? 0.0f : M;  // nothing seen yet: 2^-inf = 0
                 corr[b][h] = M == m[b][h] ? 1.0f : ex2(m[b][h] - base);
                 m[b][h] = M;

@@ -3,9 +3,9 @@
 //
 //   o = sum_j p_j v_j / sum_j p_j,  p_j = 2^(y_j - m),  y_j = scale log2(e) q.k_j
 //
-// over the rows j that the token sees, in one pass: a running maximum m and
-// sum l, and the accumulated output multiplied by 2^(m_old - m_new) when m
-// moves.  The rows may be cut into parts that different CTAs take; a part
+// over the rows j that the token sees, in one pass: a running reference m near
+// the maximum and sum l, and the accumulated output multiplied by 2^(m_old -
+// m_new) when m moves.  The rows may be cut into parts that different CTAs take; a part
 // leaves (m, l, o) in fp32 in the workspace and attn_join_kernel adds them
 // in part order (the same result on every run).
 //
@@ -105,6 +105,20 @@ __device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wai
 __device__ __forceinline__ void cp_async_arrive(uint64_t* bar) {
     asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(bar)) : "memory");
 }
+// Weights are 2^(y - m) for a reference m that moves only when the largest
+// score y exceeds it by LIFT + 8, and then to LIFT below that score: few
+// outputs are rescaled, and the quotient o / l is the same.  fp16 loses bits
+// of weights below 2^-14 and all of 2^-25 (thousands of rows far below one
+// that outweighs each of them can still be the result), so they lie as high as
+// its range has room for the largest, at 2^7 to 2^15; bf16 and fp32 have the
+// exponents, and weights of at most 1 keep sums of great values finite.
+template <typename T>
+constexpr float ATTN_LIFT = std::is_same<T, __half>::value ? 7.0f : -8.0f;
+template <typename T>
+__device__ __forceinline__ float attn_reference(float m, float top) {
+    return top > m + (ATTN_LIFT<T> + 8.0f) ? top - ATTN_LIFT<T> : m;
+}
+
 // Barrier of the consumer warps alone.
 __device__ __forceinline__ void consumers_sync() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
 __device__ __forceinline__ bool consumers_or(bool v) {
@@ -478,7 +492,7 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
 
         // ---- mask, running maximum, exponentials ----------------------------------------
         const bool edge = first + KT > w.r1 || (int32_t)(first + KT) > w.see0;
-        float mx[2] = {m[0], m[1]};
+        float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int n = 0; n < NT; ++n)
 #pragma unroll
@@ -497,8 +511,9 @@ __global__ void __launch_bounds__(ATTN_THREADS) attn_rows_kernel(const __grid_co
         for (int h = 0; h < 2; ++h) {
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
             mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-            corr[h] = m[h] == mx[h] ? 1.0f : exp2f(m[h] - mx[h]);
-            m[h] = mx[h];
+            const float M = attn_reference<T>(m[h], mx[h]);
+            corr[h] = m[h] == M ? 1.0f : exp2f(m[h] - M);
+            m[h] = M;
             l[h] *= corr[h];
         }
         uint32_t pf[F32 ? 1 : NT][2];

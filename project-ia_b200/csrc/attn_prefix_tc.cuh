@@ -28,9 +28,8 @@
 // shared memory at 128 bytes a clock).  A warp that polls both streams and
 // takes whichever is ready spends 3000 clocks a tile on doing so.
 //
-// The running maximum moves only when a half tile exceeds it by 2^8: then the
-// output is rescaled in TMEM; until then exponentials may reach 256, which
-// fp16 holds, and the quotient o / l is the same.
+// The reference of the weights (attn_reference) moves seldom: then the output
+// is rescaled in TMEM.
 //
 // Bound: for up to 128 vectors the bytes of K and V; beyond, the tensor pipe
 // (4 x 128 x 128 x head_dim flops a tile and stream) with the exponentials (128
@@ -254,10 +253,11 @@ __global__ void __launch_bounds__(TC_THREADS, 1) attn_prefix_tc_kernel(const __g
             mx = max_nan(mx, my, my) * a.c;  // c > 0
             // a score that is no number or infinite: so is the sum, and every output (the series' clamp would hide a NaN)
             const bool lost = !(mx < INFINITY);
-            const bool move = mx > m + 8.0f;  // also from -infinity
+            const float M = attn_reference<T>(m, mx);  // NaN moves nothing
+            const bool move = M != m;                  // also from -infinity
             if (__any_sync(0xffffffffu, move)) {
-                const float f = move ? (m == -INFINITY ? 0.0f : ex2(m - mx)) : 1.0f;
-                if (move) m = mx;
+                const float f = move ? (m == -INFINITY ? 0.0f : ex2(m - M)) : 1.0f;
+                m = M;
                 float s0, s1;
                 sum.get(s0, s1);
                 sum = F2(s0 * f, s1 * f);

@@ -115,6 +115,50 @@ def test_attn_sums_of_many_rows(dtype, heads, kv_heads, seqs, rows, prefix):
     within(b.out, want, want * 2.0**-14, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["f32", "f16", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,prefix,seqs", [
+    (8, 2, 64, 8000, 3), (24, 2, 128, 8000, 2), (32, 2, 64, 8000, 5), (64, 2, 128, 8000, 9), (64, 2, 32, 8000, 4), (8, 2, 128, 0, 3), (80, 2, 64, 0, 2),
+    (320, 160, 64, 4000, 3)])  # so many KV heads that a warp takes a quarter of all rows
+@pytest.mark.parametrize("sink", [0, -1])
+def test_attn_weights_far_below_the_largest(dtype, heads, kv_heads, dim, prefix, seqs, sink):
+    # one row that outweighs each of the thousands of others by 2^14 to 2^28, and has no value of its own, as the first token of a
+    # prompt often does: the others are the result.  16 bits lose nothing but their own step of fp16 weights (2^-25, where the
+    # largest is 2^7 at least): 2^-32 of it for each row.
+    rows = 8000 if not prefix else 20
+    b = Batch(dim + seqs, dtype, heads, kv_heads, dim, 16, prefix, [rows] * seqs, [1] * seqs, poison=False)
+    b.q.zero_()
+    b.q[..., 0] = 1.0
+    b.keys[..., 0] *= 0.25
+    b.values.add_(1.0)
+    pages = [b.prefix_pages] if prefix else list(b.pages)
+    n = prefix or rows
+    at = 0 if sink == 0 else n - 1
+    for gap in (14.0, 18.3, 22.5, 25.4, 28.0):
+        for p in pages:
+            b.keys[p[at // 16].long(), :, at % 16, 0] = gap * math.log(2) * math.sqrt(dim)
+            b.values[p[at // 16].long(), :, at % 16] = 0.0
+        b.call()
+        want, room = weighted(b)
+        within(b.out, want, room + (2.0**-32 * (prefix + rows) * float(b.values.abs().max()) if dtype == "f16" else 0.0), dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("heads,kv_heads,dim,seqs", [(8, 2, 64, 3), (24, 2, 128, 2), (32, 2, 64, 5), (64, 2, 128, 9), (64, 2, 32, 4)])
+def test_attn_largest_values_behind_smaller_scores(dtype, heads, kv_heads, dim, seqs):
+    # the last row of the prefix weighs 2^7.5 times each other and has the type's largest values: its share of them is finite
+    b = Batch(dim + seqs, dtype, heads, kv_heads, dim, 16, 200, [20] * seqs, [1] * seqs, poison=False)
+    b.q.zero_()
+    b.q[..., 0] = 1.0
+    b.keys[..., 0] = 0.0
+    page = b.prefix_pages[199 // 16].long()
+    b.keys[page, :, 199 % 16, 0] = 7.5 * math.log(2) * math.sqrt(dim)
+    b.values[page, :, 199 % 16] = torch.finfo(TYPES[dtype][0]).max
+    b.call()
+    want, room = weighted(b)
+    assert torch.isfinite(want).all()
+    within(b.out, want, room, dtype)
+
+
 @pytest.mark.parametrize("dtype,dim", [("bf16", 128), ("f16", 64)])
 @pytest.mark.parametrize("G,seqs,prefix", [(4, 20, 4100), (4, 40, 4173), (1, 300, 6143), (2, 64, 12289)])
 def test_attn_prefix_parts_of_many_tiles(dtype, dim, G, seqs, prefix):
