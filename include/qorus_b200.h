@@ -220,10 +220,12 @@ q_error_code q_b200_gemv_f32(const float* d_w, uint32_t M, uint32_t K,
  * Q_ERR_INVALID_ARG.  Strides count elements and, but for page_stride, are
  * below 2^32.  Calls are asynchronous on `stream`, allocate nothing, keep no
  * state between calls and may be captured in a CUDA graph; calls on different
- * streams may overlap as long as they share no output or workspace.  What the device alone can see to be
- * wrong (a page, sequence or token out of range, a length above its bound)
- * is skipped and leaves code 4 in the status word (q_b200_device_status):
- * nothing out of range is touched, results that hang on it are unspecified. */
+ * streams may overlap as long as they share no output or workspace.  Outputs
+ * overlap no input but where an operator says so.  Equal arguments give equal
+ * bits on every run.  What the device alone can see to be wrong (a page,
+ * sequence or token out of range, a length above its bound) is skipped and
+ * leaves code 4 in the status word (q_b200_device_status): nothing out of
+ * range is touched, results that hang on it are unspecified. */
 
 typedef enum { Q_B200_F32 = 0, Q_B200_F16 = 1, Q_B200_BF16 = 2 } q_b200_dtype;
 
@@ -298,9 +300,9 @@ typedef struct {
 q_error_code q_b200_rope(const q_b200_rope_args* args, void* stream);
 
 /* Token t's keys (rotated by pos[t]) and values go to row row[t] of sequence
- * seq[t]'s pages; with q its queries are rotated into q_out beside them.  A
- * token with a negative row is padding: nothing of it is written.
- * Two tokens must not name the same row of the same page. */
+ * seq[t]'s pages; with q its queries are rotated into q_out beside them (which
+ * may be q with q's strides).  A token with a negative row is padding: nothing
+ * of it is written.  Two tokens must not name the same row of the same page. */
 typedef struct {
     q_b200_paged_kv kv;
     const void* k; /* [n_tokens][n_kv_heads][head_dim] */
@@ -325,9 +327,12 @@ q_error_code q_b200_kv_append(const q_b200_append_args* args, void* stream);
  * sequence's own rows (0..lens[b]-1 in pages[b], its new tokens' rows last
  * among them).  The i-th of sequence b's n new tokens sees the whole prefix
  * and its own rows 0..lens[b]-n+i; head h reads KV head
- * h / (n_heads / n_kv_heads).  A token that sees no row gives zeros.  q and
- * out have the cache's dtype; scores, softmax and sums are fp32.  Tokens of
- * no sequence (from q_start[n_seqs] on) are left as they are in out.
+ * h / (n_heads / n_kv_heads).  A token that sees no row, or no score above
+ * -infinity, gives zeros; rows that it does not see do not reach it, whatever
+ * they hold.  q and out have the cache's dtype; scores, maxima and sums are
+ * fp32, and a weight is rounded to the dtype where it meets its row of v (for
+ * fp16 and bf16 that is an error of the size of the result's own rounding).
+ * Tokens of no sequence (from q_start[n_seqs] on) are left as they are in out.
  * head_dim 32, 64 or 128; addresses and strides of q, out and the cache in
  * multiples of 16 bytes.  n_seqs times the tiles of a sequence's max_q *
  * n_heads / n_kv_heads query vectors (16 up to 16, 32 up to 32, else 64) is
@@ -361,9 +366,9 @@ q_error_code q_b200_attn_prefix(const q_b200_attn_args* args, void* stream);
  * while uniform[b][i] * q_i(x) < p_i(x); at the first that is not, the next
  * token is drawn from max(p_i - q_i, 0), and after the last accepted draft
  * from the target's own row, by the smallest index whose running sum
- * exceeds uniform[b][n_draft] times the whole (sums to 2^-48).  p and q
- * are rows of probabilities (PROBS; they need not sum to one) or the softmax
- * of logits / temperature (LOGITS; below 1e-6 the test is whether the draft
+ * exceeds uniform[b][n_draft] times the whole (probabilities summed to 2^-48;
+ * a logit's weight is good to 2^-37).  p and q are rows of probabilities
+ * (PROBS; they need not sum to one) or the softmax of logits / temperature (LOGITS; below 1e-6 the test is whether the draft
  * is the first maximum of the target, and q is not used).  draft NULL: q is
  * one at the drafted token.  NaN and negative weights count as zero; where
  * the difference has no weight the row p is used, and a row without weight

@@ -21,8 +21,10 @@
 // with the hi.hi sums folded into fp32 every few products because the tensor
 // core truncates when it accumulates (errors against 64 bits come out at
 // 4e-7, half of an fp32 product's).  P is rounded to the cache's type for P.V
-// (fp16, bf16), as the products' operand type asks; l sums what is
-// multiplied.
+// (fp16, bf16), as the products' operand type asks: an error of the size of the
+// result's own rounding (with it 1.3 to 1.45 times the error against 64 bits
+// of a result that is rounded once).  l sums what is multiplied here and in
+// attn_few_kernel, the weights before their rounding in the tcgen05 pass.
 //
 // Bound: the products (64 vectors a row of K and V).
 #pragma once

@@ -34,8 +34,10 @@
 // Bound: for up to 128 vectors the bytes of K and V; beyond, the tensor pipe
 // (4 x 128 x 128 x head_dim flops a tile and stream) with the exponentials (128
 // x 128 of them, a quarter on the multiply-add units) in its way: 512 vectors x
-// 32768 rows x 8 KV heads of 128 take 71 us, 0.97 PFLOP/s, 3450 clocks a tile
-// of which the tensor pipe works 2048, at the 1.6 GHz that the power cap leaves.
+// 32768 rows x 8 KV heads of 128 take 78 us by themselves, 0.88 PFLOP/s with the
+// tensor pipe busy half of the time: 29 tiles a CTA at 3450 clocks, of which the
+// pipe works 2048 (62 us at the 1.66 GHz that the power cap leaves), and a CTA's
+// begin and end.
 #pragma once
 
 #include "attn_prefix.cuh"

@@ -21,8 +21,13 @@
 // 300 instructions a unit: 70 us for 8191 x 40 x 128 bf16, where this takes 32.)
 //
 // Measured back to back: the 168 MB of that in 31.5 us and the 67 MB of 2048 x
-// 32 x 128 fp32 in 12.5 us, 0.81 of a plain copy's rate; one token 3.3 us, the
-// time of a launch.
+// 32 x 128 fp32 in 12.5 us, 0.81 of a plain copy's rate (of a warp's time
+// between two instructions a third goes to the barrier behind the angles, the
+// rest to loads and results on their way); one token 3.3 to 4.4 us, the
+// time of a launch.  An append of 4093 tokens (32/8 heads of 128, bf16) takes 23.6
+// us, 0.65: 62 registers leave room for four CTAs on an SM, so its 2047 are 3.46
+// waves, the last half empty, and every token's page and three tensors' rows are
+// looked up (issue slots 41% busy).
 #pragma once
 
 #include <cuda_bf16.h>

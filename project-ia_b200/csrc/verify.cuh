@@ -8,24 +8,28 @@
 // A whole token hangs on these comparisons, and a running sum over 128 K
 // entries has as many borders: with fp32 sums (2^-24 each) about one draw in
 // forty would fall on the wrong side of one.  So r and its sums are fp64 (of
-// probabilities within a lane: pairs of fp32), and so is the softmax of the row
-// that is drawn from; the accepting tests, one border each, take their
-// normalisers from fp32 sums.
+// probabilities within a lane: pairs of fp32, exact to 2^-48), and so is the
+// softmax of the row that is drawn from, of weights good to 2^-37; the
+// accepting tests, one border each, take their normalisers from fp32 sums.
 //
 // One thread-block cluster per sequence: the vocabulary is cut into one
 // contiguous segment per warp of the cluster, segment sums go to every CTA
 // through distributed shared memory, and the warp whose segment holds the
-// border searches it (its data is still in L1/L2).  Sums are added in index
-// order, so a result does not depend on the launch.  Every row that the test
-// needs is read from HBM once.
+// border searches it (its data is still in L1/L2).  Segments are added in index
+// order and lanes in a fixed one, so that equal calls give equal results; how
+// the row is cut hangs on the number of sequences, and with it the sums' last
+// bits.  Every row that the test needs is read from HBM once.
 //
 // Bound: for one sequence the dependent steps (draft id -> its probabilities
 // -> the row -> the search, 6.5 us with the launch), which is why the row's
 // work is spread over up to 16 CTAs, and a batch over as many as run at once.
-// For a batch the bytes are a third of the time and the instructions for each
-// entry the rest: 64 sequences x 128256 bf16 probabilities 18 us (33 MB, 5 us
-// of copying), fp32 logits 47 us (66 MB, 10 us; an exponential in fp64 costs
-// three fp64 operations and a table look-up).
+// For a batch neither the bytes (a third of the time) nor the issue slots (37%
+// busy) but the waits of the few warps that the registers leave: of a warp's
+// time between two instructions a quarter goes to loads, a fifth to barriers
+// and a sixth to results on their way.  64 sequences x 128256 bf16
+// probabilities 18 us (33 MB, 5 us of copying), fp32 logits 48 us (66 MB, 10 us;
+// an exponential in fp64 costs four fp64 operations, a series and a table
+// look-up, and 64 registers spill 52 bytes; 16-bit logits spill 222 to 264).
 #pragma once
 
 #include <cooperative_groups.h>
